@@ -316,6 +316,87 @@ int gpuxSumInt32NoAlloc(void *queue, const int32_t *data, size_t n, int64_t *out
  * nothing: the word is read with a 4-byte copy into a local variable. */
 int gpuxSumInt32NoAllocStatus(void *queue);
 
+/* ---- rows picked, grouped and added by index ------------------------------
+ *
+ * The lookups, scatters and sorts by index that the reference's users write as
+ * a[m], a[m] += b and argsort (numba_mlir/mlir/tests/test_numpy.py:
+ * test_getitem_offset is the first of them), as library routines over rows: an
+ * embedding table and its gradient, tokens sorted by expert and back.
+ * Conventions of all of them: asynchronous on the queue's stream, 0 on success
+ * and non-zero with the error set (gpuxGetLastError) when an argument is
+ * refused, in which case nothing was enqueued.  A workspace is the caller's
+ * (256-byte aligned, any content, unused by anything else until the call has
+ * run) or NULL: then the call takes one from the stream-ordered pool and gives
+ * it back behind its last kernel.  The calling thread's current device is left
+ * as it was.  An index outside its range picks nothing: its row is zero, it adds
+ * nothing and it has no gradient.  Sums run in float32 (float64 for float64
+ * rows), in an order that does not depend on the run. */
+
+/* Element types of rows; a GPUX_ELEM_BF16 is the upper half of a float32. */
+enum { GPUX_ELEM_F32 = 0, GPUX_ELEM_F64 = 1, GPUX_ELEM_F16 = 2, GPUX_ELEM_BF16 = 3 };
+
+/* rows x cols elements; row r begins `stride` elements after row r - 1 (any
+ * sign; results: at least cols, or -cols at most), a row is contiguous. */
+typedef struct GPUXRows {
+  void *data;
+  int64_t rows;
+  int64_t cols;
+  int64_t stride;
+  int32_t type;
+  int32_t reserved;
+} GPUXRows;
+
+/* count contiguous indices of `bytes` (4 or 8) bytes each, signed. */
+typedef struct GPUXIndex {
+  const void *data;
+  int64_t count;
+  int32_t bytes;
+  int32_t reserved;
+} GPUXIndex;
+
+/* out[i,:] = scale * table[ids[i],:].  out has ids->count rows; its type is the
+ * table's, or one of the pair is float32 and the other 16 bits wide. */
+int _mlir_ciface_nmb_take_rows_device(void *queue, const GPUXRows *table, const GPUXIndex *ids,
+                                      double scale, const GPUXRows *out);
+
+/* The gradient of the above with respect to the table:
+ * out[v,:] = scale * (sum of dout[i,:] over ids[i] == v), i ascending; with
+ * `accumulate` it is added to what out holds and rows without an index stay
+ * untouched.  A given workspace holds at least
+ * _mlir_ciface_nmb_take_rows_grad_workspace bytes (`type`: dout's). */
+size_t _mlir_ciface_nmb_take_rows_grad_workspace(int64_t count, int64_t rows, int64_t cols, int type);
+int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRows *dout, const GPUXIndex *ids,
+                                           double scale, const GPUXRows *out, int accumulate,
+                                           void *workspace, size_t workspaceBytes);
+
+/* Stable sort of entries by group: order[j] is the entry at position j of the
+ * sorted list (groups ascending, the entries' own order within a group, the
+ * entries outside [0, groups) last), place[order[j]] = j, offsets[g] the
+ * position of group g's first entry; offsets holds groups + 1 values, the last
+ * is the number of entries inside the range.  count < 2^31, groups < 2^31 - 1. */
+size_t _mlir_ciface_nmb_group_rows_workspace(int64_t count, int64_t groups);
+int _mlir_ciface_nmb_group_rows_device(void *queue, const GPUXIndex *ids, int64_t groups, int32_t *order,
+                                       int32_t *place, int32_t *offsets, void *workspace,
+                                       size_t workspaceBytes);
+
+/* out[place[t * k + j],:] = x[t,:] for the x->rows tokens t with k entries each
+ * (k = place's length / x->rows); positions at or past *kept get zero rows. */
+int _mlir_ciface_nmb_dispatch_rows_device(void *queue, const GPUXRows *x, int64_t k, const int32_t *place,
+                                          const int32_t *kept, const GPUXRows *out);
+
+/* out[t,:] = sum over j < k of weights[t * k + j] * ys[place[t * k + j],:],
+ * entries whose position is outside [0, *kept) left out; weights NULL: ones. */
+int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows *ys, int64_t k, const int32_t *place,
+                                         const int32_t *kept, const void *weights, int weightType,
+                                         const GPUXRows *out);
+
+/* The gradients of the above for the incoming gradient dout:
+ * dys[place[t * k + j],:] = weights[t * k + j] * dout[t,:] (zero at positions
+ * past *kept), dweights[t * k + j] = dout[t,:] . ys[place[t * k + j],:]. */
+int _mlir_ciface_nmb_combine_rows_grad_device(void *queue, const GPUXRows *dout, const GPUXRows *ys, int64_t k,
+                                              const int32_t *place, const int32_t *kept, const void *weights,
+                                              int weightType, const GPUXRows *dys, void *dweights);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,6 +16,19 @@ from .device_array import (  # noqa: F401
     zeros,
 )
 
+from .rows import (  # noqa: F401
+    RowGroups,
+    bfloat16,
+    combine_rows,
+    combine_rows_grad,
+    dispatch_rows,
+    dispatch_rows_grad,
+    group_rows,
+    group_rows_workspace,
+    take_rows,
+    take_rows_grad,
+    take_rows_grad_workspace,
+)
 from .streaming import HostPipeline, map_host  # noqa: F401,E402
 
 __version__ = "0.1.0"

@@ -2198,7 +2198,7 @@ class Plan:
         """Runs the recorded steps on `args`; allocations and launches go to
         `queue` (the queue of the call's arguments), the recording queue by
         default."""
-        from . import contraction, reduce_ops
+        from . import contraction, reduce_ops, rows
 
         slots = self.slots
         arrays = [None] * len(slots)
@@ -2238,6 +2238,8 @@ class Plan:
                 # a `prange` loop cut out of the function: its own compiled kernel
                 real = [get(s[1]) if s[0] == "slot" else args[s[1]] if s[0] == "arg" else s[1] for s in step[2]]
                 step[1]._call_parfor(tuple(real))
+            elif tag == "rows":
+                rows.run_step(step, get, args)
         for i in _result_slots(self.result_spec):
             get(i)
         return _build_result(self.result_spec, arrays)

@@ -44,7 +44,7 @@ class Memref2f(ctypes.Structure):
 
 
 # Every symbol the header include/numba_mlir_gpu_runtime_cuda.h declares.
-_vp, _sz, _i, _cp = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_char_p
+_vp, _sz, _i, _cp, _i64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_char_p, ctypes.c_int64
 SIGNATURES = {
     "gpuxQueueCreate": (_vp, [_cp]),
     "gpuxQueueDestroy": (None, [_vp]),
@@ -99,6 +99,15 @@ SIGNATURES = {
         [_vp, ctypes.POINTER(Memref2f), ctypes.POINTER(Memref2f), ctypes.c_float, _i, _vp, _i, _vp, _i,
          ctypes.POINTER(Memref2f)],
     ),
+    # rows picked, grouped and added by index (numba_mlir_b200.rows)
+    "_mlir_ciface_nmb_take_rows_device": (_i, [_vp, _vp, _vp, ctypes.c_double, _vp]),
+    "_mlir_ciface_nmb_take_rows_grad_workspace": (_sz, [_i64, _i64, _i64, _i]),
+    "_mlir_ciface_nmb_take_rows_grad_device": (_i, [_vp, _vp, _vp, ctypes.c_double, _vp, _i, _vp, _sz]),
+    "_mlir_ciface_nmb_group_rows_workspace": (_sz, [_i64, _i64]),
+    "_mlir_ciface_nmb_group_rows_device": (_i, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz]),
+    "_mlir_ciface_nmb_dispatch_rows_device": (_i, [_vp, _vp, _i64, _vp, _vp, _vp]),
+    "_mlir_ciface_nmb_combine_rows_device": (_i, [_vp, _vp, _i64, _vp, _vp, _vp, _i, _vp]),
+    "_mlir_ciface_nmb_combine_rows_grad_device": (_i, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i, _vp, _vp]),
     "gpuxMemcpy": (_vp, [_vp, _vp, _vp, _sz, _i, _vp]),
     "gpuxMemset": (_vp, [_vp, _vp, _i, _sz, _vp]),
     "gpuxRecordEvent": (_vp, [_vp]),
