@@ -95,8 +95,19 @@ struct Results {
   int32_t *offsets;
 };
 
+// Words of the caller's that the first kernel sets to zero.
+struct Clear {
+  uint32_t *words;
+  int64_t count;
+  __device__ __forceinline__ void run() const {
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (int64_t)gridDim.x * blockDim.x)
+      words[i] = 0;
+  }
+};
+
 __global__ void __launch_bounds__(kOneThreads)
-    nmb_sort_one(const Ids ids, int n, int bits, int passes, const Results res) {
+    nmb_sort_one(const Ids ids, int n, int bits, int passes, const Results res, const Clear clear) {
+  clear.run();
   extern __shared__ uint32_t smem[];
   uint32_t *counts = smem;                 // [warps][bins]
   uint32_t *keys = smem + 32 * kBins;      // [n]
@@ -190,7 +201,8 @@ struct Pass {
   __device__ __forceinline__ uint32_t digit(uint32_t k) const { return (k >> shift) & (uint32_t)(bins - 1); }
 };
 
-__global__ void __launch_bounds__(kThreads) nmb_sort_count(const Pass p) {
+__global__ void __launch_bounds__(kThreads) nmb_sort_count(const Pass p, const Clear clear) {
+  clear.run();
   __shared__ uint32_t count[kBins];
   for (int b = threadIdx.x; b < p.bins; b += kThreads)
     count[b] = 0;
@@ -352,7 +364,8 @@ size_t sortBytes(int64_t count, int64_t groups) {
 }
 
 bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t groups, int32_t *order,
-               uint32_t *keys, int32_t *place, int32_t *offsets, void *workspace) {
+               uint32_t *keys, int32_t *place, int32_t *offsets, void *workspace, uint32_t *clear,
+               int64_t clearWords) {
   const int64_t n = ids.count;
   const Ids in{ids.data, ids.bytes, (uint32_t)groups};
   const int bits = bitsOf(groups), passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
@@ -383,7 +396,8 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
     // as many warps as there are rows of 32 entries
     const int warps = (int)(n + 31) / 32 < 32 ? (int)(n + 31) / 32 : 32;
     nmb_sort_one<<<1, warps * 32, kOneSmem, s.stream>>>(in, (int)n, bits, passes,
-                                                        Results{order, keys, place, passes == 1 ? offsets : nullptr});
+                                                        Results{order, keys, place, passes == 1 ? offsets : nullptr},
+                                                        Clear{clear, clearWords});
     if (!launched(who))
       return false;
   } else {
@@ -401,7 +415,7 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
       // sorted keys into buffer 0 (see above)
       const int to = (passes - 1 - pass) & 1;
       p.shift = pass * digitBits;
-      nmb_sort_count<<<(unsigned)blocks, kThreads, 0, s.stream>>>(p);
+      nmb_sort_count<<<(unsigned)blocks, kThreads, 0, s.stream>>>(p, Clear{clear, pass == 0 ? clearWords : 0});
       if (!launched(who))
         return false;
       nmb_sort_prefix<<<(unsigned)((p.bins + kWarps - 1) / kWarps), kThreads, 0, s.stream>>>(counts, totals,

@@ -124,14 +124,26 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // -------------------------------------------------------------- take_grad ---
-// The entries arrive sorted by row (order, keys), so a row's entries are
-// neighbours: the threads of a row find them with a binary search and add them
-// up in order.  A row without entries becomes zero.
-__device__ __forceinline__ int64_t lower_bound(const uint32_t *keys, int64_t n, uint32_t key) {
-  int64_t lo = 0, hi = n;
+// The entries arrive sorted by row (keys, order), so a row's entries are a run
+// of neighbours.  The sorted list is cut into chunks of `span` entries; a group
+// of `lanes` threads takes a chunk, a thread one access's width of columns, and
+// adds up the runs that begin in the chunk, eight incoming rows in flight.
+// Every incoming row is read once, every row of the result written once.
+//
+// A run that goes on past its chunk is finished by the group it began in, up
+// to the first chunk that lies inside the run as a whole.  Those inner chunks
+// add up their own entries, so a frequent token (padding, the end of a line)
+// does not keep one group busy: all of the run's groups leave partial sums in
+// the workspace, and the one that draws the last ticket adds them up in the
+// order of the chunks.  The order of additions is a function of the ids alone.
+//
+// Rows without entries are set to zero by blocks of their own, which look their
+// rows up in the sorted keys, one row a lane.
+__device__ __forceinline__ int64_t lower_bound(const uint32_t *__restrict__ keys, int64_t lo, int64_t hi,
+                                               uint32_t key) {
   while (lo < hi) {
     const int64_t mid = (lo + hi) / 2;
-    if (keys[mid] < key)
+    if (__ldg(keys + mid) < key)
       lo = mid + 1;
     else
       hi = mid;
@@ -139,31 +151,124 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t *keys, int64_t n, 
   return lo;
 }
 
+// Barrier over the threads of a group: part of a warp, a warp, or several.
+__device__ __forceinline__ void group_sync(int lane_bits, int group) {
+  if (lane_bits < 5)
+    __syncwarp(((1u << (1 << lane_bits)) - 1) << ((threadIdx.x & 31) & ~((1 << lane_bits) - 1)));
+  else if (lane_bits == 5)
+    __syncwarp();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(1 << lane_bits) : "memory");
+}
+
+constexpr int kGradBatch = 8;   // incoming rows in flight per thread
+constexpr int kZeroRows = 32;   // rows looked up by a block that clears
+
+struct GradPlan {
+  const int32_t *order;
+  const uint32_t *keys;
+  int64_t n;
+  int span;
+  unsigned slabs;          // groups side by side over the columns
+  unsigned chunk_blocks;   // blocks over chunks (times slabs), the rest clears
+  void *partials;          // [chunks][cols]
+  uint32_t *tickets;       // [chunks][slabs], zero
+  int lane_bits;
+  int accumulate;
+};
+
+// The threads of a group walk over entries [j, end) of one or several runs;
+// `flush` gets each run's row and sum when the next begins.
+template <typename I, int V, typename A, typename F>
+__device__ __forceinline__ void walk_runs(const I *__restrict__ dout, int64_t stride, const GradPlan &p, int64_t j,
+                                          int64_t end, uint32_t &row, A (&sum)[V], F &&flush) {
+  while (j < end) {
+    int32_t at[kGradBatch];
+    uint32_t key[kGradBatch];
+    Pack<I, V> x[kGradBatch];
+#pragma unroll
+    for (int u = 0; u < kGradBatch; ++u)
+      if (j + u < end) {
+        at[u] = __ldg(p.order + j + u);
+        key[u] = __ldg(p.keys + j + u);
+      }
+#pragma unroll
+    for (int u = 0; u < kGradBatch; ++u)
+      if (j + u < end)
+        x[u] = load<I, V>(dout + (int64_t)at[u] * stride);
+#pragma unroll
+    for (int u = 0; u < kGradBatch; ++u)
+      if (j + u < end) {
+        if (key[u] != row) {
+          flush(row, sum);
+          row = key[u];
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            sum[e] = A(0);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          sum[e] += up(x[u].v[e]);
+      }
+    j += kGradBatch;
+  }
+}
+
 template <typename I, typename O, int V>
 __global__ void __launch_bounds__(kThreads)
-    nmb_take_rows_grad(const I *__restrict__ dout, int64_t stride, const int32_t *__restrict__ order,
-                       const uint32_t *__restrict__ keys, int64_t n, typename Acc<I>::type scale, O *out, int64_t rows,
-                       int64_t out_stride, int accumulate, int64_t vecs, int lane_bits) {
+    nmb_take_rows_grad(const I *__restrict__ dout, int64_t stride, const GradPlan p, typename Acc<I>::type scale, O *out,
+                       int64_t rows, int64_t out_stride, int64_t vecs) {
   using A = typename Acc<I>::type;
-  const int lane = threadIdx.x & ((1 << lane_bits) - 1);
-  const int64_t v = (int64_t)blockIdx.x * (kThreads >> lane_bits) + (threadIdx.x >> lane_bits);
-  if (v >= rows)
-    return;
-  const int64_t begin = lower_bound(keys, n, (uint32_t)v);
-  O *dst = out + v * out_stride;
-  if (accumulate && (begin >= n || keys[begin] != (uint32_t)v))
-    return;
-  for (int64_t c = lane; c < vecs; c += 1 << lane_bits) {
-    A sum[V] = {};
-    for (int64_t j = begin; j < n && keys[j] == (uint32_t)v; ++j) {
-      const Pack<I, V> x = load<I, V>(dout + (int64_t)order[j] * stride + c * V);
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        sum[e] += up(x.v[e]);
+  __shared__ uint32_t shared_word[kThreads / 64 + 1];
+  const int lanes = 1 << p.lane_bits, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> p.lane_bits;
+  const int groups = kThreads >> p.lane_bits;
+
+  if (blockIdx.x >= p.chunk_blocks * p.slabs) { // rows without entries
+    const int64_t first = (int64_t)(blockIdx.x - p.chunk_blocks * p.slabs) * kZeroRows;
+    if (threadIdx.x < 32) {
+      const int64_t v = first + threadIdx.x;
+      bool absent = v < rows;
+      if (absent) {
+        const int64_t at = lower_bound(p.keys, 0, p.n, (uint32_t)v);
+        absent = at >= p.n || __ldg(p.keys + at) != (uint32_t)v;
+      }
+      const uint32_t mask = __ballot_sync(kAll, absent);
+      if (threadIdx.x == 0)
+        shared_word[0] = mask;
     }
+    __syncthreads();
+    const uint32_t mask = shared_word[0];
+    Pack<O, V> zero;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      zero.v[e] = down<O, A>(A(0));
+    for (int r = group; r < kZeroRows; r += groups)
+      if (mask >> r & 1)
+        for (int64_t c = lane; c < vecs; c += lanes)
+          store<O, V>(out + (first + r) * out_stride + c * V, zero);
+    return;
+  }
+
+  const unsigned slab = blockIdx.x % p.slabs;
+  const int64_t chunk = (int64_t)(blockIdx.x / p.slabs) * groups + group;
+  const int64_t column = (int64_t)slab * lanes + lane; // of accesses; a group's spare lanes idle through the barriers
+  const bool active = column < vecs;
+  const int64_t begin = chunk * p.span;
+  if (begin >= p.n)
+    return;
+  const int64_t end = min(begin + p.span, p.n);
+  const uint32_t first_key = __ldg(p.keys + begin), last_key = __ldg(p.keys + end - 1);
+  const uint32_t prev_key = begin > 0 ? __ldg(p.keys + begin - 1) : 0xffffffffu;
+  if (first_key >= rows)
+    return;
+  const I *src = dout + (active ? column : 0) * V;
+  O *dst = out + (active ? column : 0) * V;
+  auto write = [&](uint32_t row, const A(&sum)[V]) {
+    if (!active)
+      return;
     Pack<O, V> y;
-    if (accumulate) {
-      y = load<O, V>(dst + c * V);
+    if (p.accumulate) {
+      y = load<O, V>(dst + (int64_t)row * out_stride);
 #pragma unroll
       for (int e = 0; e < V; ++e)
         y.v[e] = down<O, A>(madd(scale, sum[e], up(y.v[e])));
@@ -172,8 +277,89 @@ __global__ void __launch_bounds__(kThreads)
       for (int e = 0; e < V; ++e)
         y.v[e] = down<O, A>(scale * sum[e]);
     }
-    store<O, V>(dst + c * V, y);
+    store<O, V>(dst + (int64_t)row * out_stride, y);
+  };
+
+  A sum[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    sum[e] = A(0);
+  int64_t owner = chunk, inner = 0; // where the long run began, its inner chunks
+  uint32_t row;
+  if (begin > 0 && prev_key == first_key && last_key == first_key && end - begin == p.span) {
+    // inside a long run as a whole
+    row = first_key;
+    walk_runs<I, V>(src, stride, p, begin, end, row, sum, [](uint32_t, const A(&)[V]) {});
+    owner = lower_bound(p.keys, 0, begin, row) / p.span;
+    const int64_t run_end = lower_bound(p.keys, end, p.n, row + 1);
+    inner = (run_end - (owner + 1) * p.span) / p.span;
+  } else {
+    // entries of a run that began before belong to the group it began in
+    int64_t j = prev_key == first_key ? lower_bound(p.keys, begin, end, first_key + 1) : begin;
+    const int64_t stop = last_key >= rows ? lower_bound(p.keys, j, end, (uint32_t)rows) : end;
+    if (j >= stop)
+      return;
+    row = __ldg(p.keys + j);
+    walk_runs<I, V>(src, stride, p, j, stop, row, sum, write);
+    if (stop == end && end < p.n && __ldg(p.keys + end) == row) {
+      const int64_t run_end = lower_bound(p.keys, end, p.n, row + 1);
+      inner = (run_end - end) / p.span;
+      walk_runs<I, V>(src, stride, p, end + inner * p.span, run_end, row, sum, write);
+    }
+    if (inner == 0) {
+      write(row, sum);
+      return;
+    }
   }
+
+  // a long run: leave the partial sum, the last of its groups adds them up
+  A *partials = static_cast<A *>(p.partials) + column * V;
+  const int64_t width = vecs * V;
+  if (active) {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      __stcg(partials + chunk * width + e, sum[e]);
+  }
+  __threadfence();
+  group_sync(p.lane_bits, group);
+  uint32_t drawn = 0;
+  if (lane == 0)
+    drawn = atomicAdd(p.tickets + owner * p.slabs + slab, 1u);
+  if (p.lane_bits <= 5) {
+    const int base = (threadIdx.x & 31) & ~(lanes - 1);
+    const uint32_t mask = p.lane_bits == 5 ? kAll : ((1u << lanes) - 1) << base;
+    drawn = __shfl_sync(mask, drawn, base);
+  } else {
+    if (lane == 0)
+      shared_word[group] = drawn;
+    group_sync(p.lane_bits, group);
+    drawn = shared_word[group];
+  }
+  if (drawn != (uint32_t)inner || !active)
+    return;
+  __threadfence();
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    sum[e] = A(0);
+#pragma unroll 8
+  for (int64_t c = owner; c <= owner + inner; ++c) {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      sum[e] += __ldcg(partials + c * width + e);
+  }
+  write(row, sum);
+}
+
+// Entries per chunk: 32, or fewer (down to 4) where that leaves less than four
+// blocks a multiprocessor.  With 777 entries of 1000 float32 chunks of 4 give
+// 195 blocks, chunks of 32 only 25.
+int gradSpan(int64_t n, int64_t vecs) {
+  const int bits = laneBits(vecs, kThreadBits);
+  const int64_t slabs = (vecs + (int64_t(1) << bits) - 1) >> bits;
+  int span = 32;
+  while (span > 4 && (n / span >> (kThreadBits - bits)) * slabs < 148 * 4)
+    span /= 2;
+  return span;
 }
 
 // --------------------------------------------------------------- dispatch ---
@@ -421,10 +607,26 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_device(void *queue, const GPUXRows *t
   return launched(who) ? 0 : 1;
 }
 
+namespace {
+// The workspace of take_grad: order, sorted keys, tickets, partial sums, the
+// sort's own.  It depends on the shape alone: the widest access (8 elements)
+// gives the shortest chunks, the narrowest the most slabs.
+struct GradMemory {
+  size_t entries, tickets, partials, sort;
+  GradMemory(int64_t n, int64_t rows, int64_t cols, int type) {
+    const int span = gradSpan(n, (cols + 7) / 8);
+    const int64_t chunks = (n + span - 1) / span;
+    entries = padded((size_t)n * 4);
+    tickets = padded((size_t)chunks * (size_t)((cols + kThreads - 1) / kThreads) * 4);
+    partials = padded((size_t)chunks * (size_t)cols * (type == GPUX_ELEM_F64 ? 8 : 4));
+    sort = nmb::rows::sortBytes(n, rows);
+  }
+  size_t total() const { return 2 * entries + tickets + partials + sort; }
+};
+} // namespace
+
 GPUX_EXPORT size_t _mlir_ciface_nmb_take_rows_grad_workspace(int64_t count, int64_t rows, int64_t cols, int type) {
-  (void)cols;
-  (void)type;
-  return count < 0 ? 0 : 2 * padded((size_t)count * 4) + nmb::rows::sortBytes(count, rows);
+  return count < 0 || rows < 0 || cols < 0 ? 0 : GradMemory(count, rows, cols, type).total();
 }
 
 GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRows *dout, const GPUXIndex *ids,
@@ -439,22 +641,21 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
                   (long long)ids->count, (long long)out->rows);
     return 1;
   }
-  if (out->rows == 0 || out->cols == 0)
+  if (out->rows == 0 || out->cols == 0 || (accumulate && ids->count == 0))
     return 0;
   Stream s(queue);
   if (!s.ok)
     return 1;
-  nmb::rows::Workspace memory(
-      s, who, workspace, workspaceBytes,
-      _mlir_ciface_nmb_take_rows_grad_workspace(ids->count, out->rows, out->cols, dout->type));
+  const GradMemory need(ids->count, out->rows, out->cols, dout->type);
+  nmb::rows::Workspace memory(s, who, workspace, workspaceBytes, need.total());
   if (!memory.ok)
     return 1;
-  const size_t entries = padded((size_t)ids->count * 4);
   unsigned char *ws = static_cast<unsigned char *>(memory.data);
   int32_t *order = reinterpret_cast<int32_t *>(ws);
-  uint32_t *keys = reinterpret_cast<uint32_t *>(ws + entries);
-  if (!nmb::rows::sortByKey(s, who, *ids, out->rows, order, keys, nullptr, nullptr, ws + 2 * entries))
-    return 1;
+  uint32_t *keys = reinterpret_cast<uint32_t *>(ws + need.entries);
+  uint32_t *tickets = reinterpret_cast<uint32_t *>(ws + 2 * need.entries);
+  void *partials = ws + 2 * need.entries + need.tickets;
+  bool ok = true;
   withPair(dout->type, out->type, [&](auto i, auto o) {
     using I = decltype(i);
     using O = decltype(o);
@@ -462,13 +663,29 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
     const int v = accessElems(out->cols, most, {dout, out});
     const int64_t vecs = out->cols / v;
     const int bits = laneBits(vecs, kThreadBits);
+    const int span = gradSpan(ids->count, vecs);
+    const int64_t chunks = (ids->count + span - 1) / span;
+    const unsigned slabs = (unsigned)((vecs + (int64_t(1) << bits) - 1) >> bits);
+    const unsigned zeros = accumulate ? 0 : (unsigned)((out->rows + kZeroRows - 1) / kZeroRows);
+    const GradPlan plan{order, keys,    ids->count, span, slabs, blocksFor(chunks, bits), partials,
+                        tickets, bits, accumulate};
+    const int64_t blocks = (int64_t)plan.chunk_blocks * slabs + zeros;
+    if (blocks >= (int64_t(1) << 31)) {
+      nmb::setError("%s: too many indices for their width", who);
+      ok = false;
+      return;
+    }
+    ok = nmb::rows::sortByKey(s, who, *ids, out->rows, order, keys, nullptr, nullptr,
+                              ws + 2 * need.entries + need.tickets + need.partials, tickets, chunks * slabs);
+    if (!ok)
+      return;
     withElems<most>(v, [&](auto V) {
-      nmb_take_rows_grad<I, O, V.value><<<blocksFor(out->rows, bits), kThreads, 0, s.stream>>>(
-          static_cast<const I *>(dout->data), dout->stride, order, keys, ids->count, (typename Acc<I>::type)scale,
-          static_cast<O *>(out->data), out->rows, out->stride, accumulate, vecs, bits);
+      nmb_take_rows_grad<I, O, V.value><<<(unsigned)blocks, kThreads, 0, s.stream>>>(
+          static_cast<const I *>(dout->data), dout->stride, plan, (typename Acc<I>::type)scale,
+          static_cast<O *>(out->data), out->rows, out->stride, vecs);
     });
   });
-  return launched(who) ? 0 : 1;
+  return ok && launched(who) ? 0 : 1;
 }
 
 GPUX_EXPORT int _mlir_ciface_nmb_dispatch_rows_device(void *queue, const GPUXRows *x, int64_t k, const int32_t *place,

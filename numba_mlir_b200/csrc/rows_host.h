@@ -174,10 +174,12 @@ inline int laneBits(int64_t vecs, int most) {
 // Stable sort of the indices by key, key = id inside [0, groups), groups for
 // every other id.  Any of the results may be null: order[j] = entry at sorted
 // position j, keys[j] its key, place[order[j]] = j, offsets[g] = position of
-// the first key >= g for g <= groups.
+// the first key >= g for g <= groups.  `clear` words of the caller's are set to
+// zero on the way.
 size_t sortBytes(int64_t count, int64_t groups);
 bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t groups, int32_t *order,
-               uint32_t *keys, int32_t *place, int32_t *offsets, void *workspace);
+               uint32_t *keys, int32_t *place, int32_t *offsets, void *workspace, uint32_t *clear = nullptr,
+               int64_t clearWords = 0);
 
 } // namespace rows
 } // namespace nmb
