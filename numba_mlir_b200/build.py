@@ -24,6 +24,8 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 # CPython extension with the native launch path of the Python front end
 # (argument unboxing + GPUParamDesc + launch); plain C++, no CUDA.
 FASTCALL_SRC = os.path.join(CSRC, "fastcall", "fastcall.cpp")
+FASTCALL_DEPS = (FASTCALL_SRC, os.path.join(CSRC, "fastcall", "rows_call.h"),
+                 os.path.join(HERE, "..", "include", "numba_mlir_gpu_runtime_cuda.h"), os.path.abspath(__file__))
 FASTCALL_PATH = os.path.join(HERE, "_fastcall.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -95,8 +97,7 @@ def build_fastcall(force=False):
     import sysconfig
 
     if (not force and os.path.exists(FASTCALL_PATH)
-            and os.path.getmtime(FASTCALL_PATH) > os.path.getmtime(FASTCALL_SRC)
-            and os.path.getmtime(FASTCALL_PATH) > os.path.getmtime(os.path.abspath(__file__))):
+            and all(os.path.getmtime(FASTCALL_PATH) > os.path.getmtime(p) for p in FASTCALL_DEPS)):
         return FASTCALL_PATH
     cxx = shutil.which("g++") or shutil.which("c++")
     if cxx is None:

@@ -14,6 +14,7 @@
 //                                          one @kernel launch from its Python arguments
 //   replay(queue, launches, args)          the launches of a recorded njit plan
 //   signature(args)                        the plan-cache key of a call's arguments
+//   rows_*(queue, ...)                     the row operators (rows_call.h)
 //
 // Nothing here touches the device; a failed launch (NULL event) is reported as
 // RuntimeError and the Python side reads the runtime's message.
@@ -24,6 +25,8 @@
 #include <chrono>
 #include <cstdint>
 #include <cstring>
+
+#include "rows_call.h"
 
 namespace {
 
@@ -459,6 +462,7 @@ PyMethodDef kMethods[] = {
      "launch_kernel(queue, kernel, grid, block, layout, args, tail[, repeat])"},
     {"replay", py_replay, METH_VARARGS, "replay(queue, launches, args)"},
     {"signature", py_signature, METH_VARARGS, "signature(args, array_type)"},
+    ROWSCALL_METHODS,
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fastcall",

@@ -31,6 +31,7 @@ from typing import Any, NamedTuple
 
 import numpy as np
 
+from . import lazy
 from . import runtime as _rt
 from .device_array import DeviceArray, as_device_array, empty
 
@@ -86,7 +87,36 @@ def _torch_type(dtype):
         t = sys.modules["torch"]
         _torch_types.update({t.float32: (0, 0, 4), t.float64: (1, 0, 8), t.float16: (2, 0, 2),
                              t.bfloat16: (3, 0, 2), t.int32: (None, 4, 4), t.int64: (None, 8, 8)})
+        _fast_torch()
     return _torch_types.get(dtype)
+
+
+def _torch_raw_stream(device):
+    """Handle of torch's current stream of a device."""
+    return sys.modules["torch"].cuda.current_stream(device).cuda_stream
+
+
+_native = None
+_native_types = {np.dtype(t): (-1 if k > 3 else k, 0 if k <= 3 else k, np.dtype(t).itemsize)
+                 for t, k in list(_FLOATS.items()) + list(_INTS.items())}
+
+
+def _fast():
+    """The native call path (csrc/fastcall/rows_call.h), bound on first use."""
+    global _native
+    fast, lib = _rt.fastcall(), _rt.load()
+    entries = ("take_rows", "take_rows_grad", "group_rows", "dispatch_rows", "combine_rows", "combine_rows_grad")
+    fast.rows_init(tuple(ctypes.cast(getattr(lib, f"_mlir_ciface_nmb_{e}_device"), ctypes.c_void_p).value
+                         for e in entries), _native_types, DeviceArray)
+    _native = fast
+    return fast
+
+
+def _fast_torch():
+    """Lets the native path take torch's tensors, from the first one on."""
+    torch = sys.modules["torch"]
+    _native_types.update({t: (-1 if k is None else k, i, n) for t, (k, i, n) in _torch_types.items()})
+    (_native or _fast()).rows_torch(torch.Tensor, getattr(torch._C, "_cuda_getCurrentRawStream", _torch_raw_stream))
 
 
 def _operand(obj, name):
@@ -96,7 +126,7 @@ def _operand(obj, name):
     gradient, CUDA only)."""
     op = _Operand()
     op.obj = obj
-    if type(obj) is not DeviceArray and type(obj).__module__.startswith("torch"):
+    if type(obj) is not DeviceArray and "torch" in sys.modules and isinstance(obj, sys.modules["torch"].Tensor):
         known = _torch_type(obj.dtype)
         if known is not None and obj.is_cuda:
             if obj.requires_grad:
@@ -240,11 +270,10 @@ _stream_queues = {}
 
 def _torch_stream(device):
     """Queue over torch's current stream of the device, made once per stream."""
-    cuda = sys.modules["torch"].cuda
-    stream = cuda.current_stream(device).cuda_stream
+    stream = _torch_raw_stream(device)
     q = _stream_queues.get((device, stream))
     if q is None:
-        with cuda.device(device):
+        with sys.modules["torch"].cuda.device(device):
             q = _stream_queues[(device, stream)] = _rt.Queue.from_stream(stream)
     return q
 
@@ -288,7 +317,7 @@ class _On:
                 if torch_seen:
                     continue
                 torch_seen = True
-                if sys.modules["torch"].cuda.current_stream(op.device).cuda_stream == mine:
+                if _torch_raw_stream(op.device) == mine:
                     continue
                 q = _torch_stream(op.device)
             if _raw_stream(q) != mine:
@@ -335,14 +364,35 @@ def _workspace(workspace, name):
 _ref = ctypes.byref
 
 
+def _default(queue, first):
+    """The queue of a call whose arrays are like `first` (None: not known)."""
+    if queue is not None:
+        return queue
+    if type(first) is DeviceArray:
+        return first._buf.queue
+    if "torch" in sys.modules and isinstance(first, sys.modules["torch"].Tensor) and first.is_cuda:
+        return _torch_stream(first.get_device())
+    return None
+
+
+def _done(code):
+    """Whether the native path ran the call (it leaves what is not ordinary)."""
+    if code == 2:
+        _rt.check()
+        raise _rt.GpuRuntimeError("a row operation failed")
+    return code
+
+
 # ---------------------------------------------------------------- routines ---
 def take_rows(table, ids, scale=1.0, out=None, queue=None):
     """`scale * table[ids]`: out[i..., :] = scale * table[ids[i...], :] for a
     table (R, D) and ids of any shape; zero rows for ids outside [0, R).  `out`
     has the table's type, or one of the two is float32 and the other 16 bits
     wide; the product is rounded once, to that type."""
-    if _traced(table, ids, scale, out):
+    if lazy.current_trace() is not None:
         return _trace_take(table, ids, scale, out)
+    if out is not None and _done((_native or _fast()).rows_take(_default(queue, table), table, ids, scale, out)):
+        return out
     t, i = _operand(table, "table"), _operand(ids, "ids")
     o = _operand(out, "out") if out is not None else None
     on = _On(queue, (t, i) if o is None else (t, i, o))
@@ -372,8 +422,11 @@ def take_rows_grad(dout, ids, rows=None, scale=1.0, out=None, accumulate=False, 
     to `out` and touches only the rows that an id names.  `workspace`: a device
     array of at least `take_rows_grad_workspace(...)` bytes; without one the call
     takes memory from the stream-ordered pool."""
-    if _traced(dout, ids, scale, out):
+    if lazy.current_trace() is not None:
         return _trace_take_grad(dout, ids, rows, scale, out, accumulate)
+    if out is not None and rows is None and workspace is None and _done((_native or _fast()).rows_take_grad(
+            _default(queue, dout), dout, ids, scale, out, bool(accumulate))):
+        return out
     d, i = _operand(dout, "dout"), _operand(ids, "ids")
     o = _operand(out, "out") if out is not None else None
     ws, ws_bytes, w = _workspace(workspace, "workspace")
@@ -417,8 +470,11 @@ def group_rows(ids, groups, plan=None, workspace=None, queue=None):
     """Sorts the entries of `ids` (any shape) by group, `groups` groups, keeping
     their order within a group; entries outside [0, groups) come last.  Returns
     RowGroups, written into the arrays of `plan` when one is given."""
-    if _traced(ids, groups, *(plan or ())):
+    if lazy.current_trace() is not None:
         return _trace_group(ids, groups, plan)
+    if plan is not None and workspace is None and _done((_native or _fast()).rows_group(
+            _default(queue, ids), ids, groups, plan)):
+        return RowGroups(*plan)
     i = _operand(ids, "ids")
     results = [_operand(x, n) for x, n in zip(plan, RowGroups._fields)] if plan is not None else []
     ws, ws_bytes, w = _workspace(workspace, "workspace")
@@ -452,10 +508,15 @@ def dispatch_rows(x, ids, groups=None, out=None, plan=None, queue=None):
     choice (plan.offsets[-1]) are zero.  `out` may have more rows, which are left
     as they are; `plan` holds arrays to write the RowGroups into.  A RowGroups in
     the place of `ids` is used as it is."""
-    if _traced(x, out, *(ids if isinstance(ids, tuple) else (ids,)), *(plan or ())):
+    if lazy.current_trace() is not None:
         return _trace_dispatch(x, ids, groups, out, plan)
-    r = _operand(x, "x")
     sorted_already = isinstance(ids, RowGroups)
+    if out is not None and (plan is None if sorted_already else plan is not None):
+        known, entries = (ids, None) if sorted_already else (plan, ids)
+        if (groups is None) == sorted_already and _done((_native or _fast()).rows_dispatch(
+                _default(queue, x), x, entries, groups, known, out)):
+            return out, RowGroups(*known)
+    r = _operand(x, "x")
     if sorted_already:
         if groups is not None or plan is not None:
             raise ValueError("groups and plan are for ids that are not sorted yet")
@@ -490,7 +551,7 @@ def dispatch_rows(x, ids, groups=None, out=None, plan=None, queue=None):
 
 
 class _Quiet:
-    """`on` for a first step of a call: errors are raised, streams of other
+    """`on` for the first step of a call: errors are raised, streams of other
     arrays wait only for the last step."""
 
     __slots__ = ("queue", "on")
@@ -527,12 +588,14 @@ def combine_rows(ys, plan, weights=None, out=None, queue=None):
     weights[t, j] * ys[plan.place[t, j], :], choices that were dropped left out.
     `weights` has the shape of plan.place (ones when it is None) and any
     floating-point type; `out` (T, D) has the type of ys."""
-    if _traced(ys, weights, out, *plan):
+    if lazy.current_trace() is not None:
         return _trace_combine(ys, plan, weights, out)
     return _combine(ys, plan, weights, out, queue, "ys")
 
 
 def _combine(ys, plan, weights, out, queue, name):
+    if out is not None and _done((_native or _fast()).rows_combine(_default(queue, ys), ys, plan, weights, out)):
+        return out
     y = _operand(ys, name)
     results = [_operand(plan[1], "place"), _operand(plan[2], "offsets")]
     w = _operand(weights, "weights") if weights is not None else None
@@ -563,7 +626,7 @@ def _combine(ys, plan, weights, out, queue, name):
 def dispatch_rows_grad(dxs, plan, out=None, queue=None):
     """The gradient of `dispatch_rows` with respect to x: the sum of the rows at
     a token's places, out[t, :] = sum over j of dxs[plan.place[t, j], :]."""
-    if _traced(dxs, out, *plan):
+    if lazy.current_trace() is not None:
         return _trace_combine(dxs, plan, None, out)
     return _combine(dxs, plan, None, out, queue, "dxs")
 
@@ -574,8 +637,11 @@ def combine_rows_grad(dout, ys, plan, weights=None, out=None, dweights=None, que
     dout[t, :] . ys[plan.place[t, j], :]; both zero for dropped choices.
     Returns (dys, dweights), written into `out` and `dweights` when given;
     dweights has the type of the weights (float32 when they are None)."""
-    if _traced(dout, ys, weights, out, dweights, *plan):
+    if lazy.current_trace() is not None:
         return _trace_combine_grad(dout, ys, plan, weights, out, dweights)
+    if out is not None and dweights is not None and _done((_native or _fast()).rows_combine_grad(
+            _default(queue, dout), dout, ys, plan, weights, out, dweights)):
+        return out, dweights
     d, y = _operand(dout, "dout"), _operand(ys, "ys")
     results = [_operand(plan[1], "place"), _operand(plan[2], "offsets")]
     w = _operand(weights, "weights") if weights is not None else None
@@ -617,33 +683,20 @@ def _check_pair(a, b, name):
 # ------------------------------------------------- inside a traced function ---
 # A routine called while an `njit` function is traced runs at once on the arrays
 # of the trace and is a step of the recorded plan, like a reduction or a product.
-def _traced(*args):
-    from . import lazy
-
-    return lazy.current_trace() is not None and any(isinstance(a, lazy.LazyArray) for a in args)
-
-
 def _step(routine, arrays, consts, results):
     """Runs `routine(**arrays, **consts, **results)` inside the active trace.
     `results`: name -> (shape, dtype) of a new array or an existing one to write;
     returns the results' arrays, in order."""
-    from . import lazy
-
     trace = lazy.current_trace()
 
-    def slot_of(a):
-        if not isinstance(a, lazy.LazyArray):
-            a = lazy.LazyArray(trace, lazy._as_node(trace, a))
-        return trace.materialize(a)
-
-    slots = {name: ("slot", slot_of(a)) for name, a in arrays.items() if a is not None}
+    slots = {name: ("slot", trace.materialize(a)) for name, a in arrays.items() if a is not None}
     outs = {}
     for name, r in results.items():
         if isinstance(r, tuple):
             outs[name] = trace.add_tmp_slot(*r)
         else:
-            if not isinstance(r, lazy.LazyArray) or r.node.kind != "leaf":
-                raise TypeError(f"{name} must be an array")
+            if r.node.kind != "leaf":
+                raise TypeError(f"{name} must be an array, not an expression")
             outs[name] = trace.materialize(r)
             trace.before_direct_write(outs[name])
         slots[name] = ("slot", outs[name])
@@ -659,7 +712,8 @@ def _step(routine, arrays, consts, results):
     step = ("rows", routine, tuple(slots.items()))
     trace.steps.append(step)
     if not trace.dry:
-        run_step(step, trace.arrays.__getitem__, trace.args)
+        with lazy._TraceScope(None):
+            run_step(step, trace.arrays.__getitem__, trace.args)
     return [trace.leaf(s) for s in outs.values()]
 
 
@@ -670,6 +724,19 @@ def run_step(step, get, args):
     routine(**kwargs)
 
 
+def _lift(a):
+    """An array argument as an array of the active trace.  One that is not an
+    argument of the traced function is captured: such a call is not replayed."""
+    if a is None or isinstance(a, lazy.LazyArray):
+        return a
+    if not isinstance(a, DeviceArray):
+        if not hasattr(a, "__cuda_array_interface__"):
+            raise TypeError(f"an array is needed, not {type(a).__name__}")
+        a = as_device_array(a)
+    trace = lazy.current_trace()
+    return lazy.LazyArray(trace, lazy._as_node(trace, a))
+
+
 def _row_type(a):
     dt = np.dtype(a.dtype)
     if dt.names is not None or dt.str not in _FLOATS:
@@ -678,6 +745,7 @@ def _row_type(a):
 
 
 def _trace_take(table, ids, scale, out):
+    table, ids, out = _lift(table), _lift(ids), _lift(out)
     shape = tuple(ids.shape) + (table.shape[-1],)
     (res,) = _step(take_rows, {"table": table, "ids": ids}, {"scale": scale},
                    {"out": out if out is not None else (shape, _row_type(table))})
@@ -685,6 +753,7 @@ def _trace_take(table, ids, scale, out):
 
 
 def _trace_take_grad(dout, ids, rows, scale, out, accumulate):
+    dout, ids, out = _lift(dout), _lift(ids), _lift(out)
     if out is None and rows is None:
         raise ValueError("the number of rows of the table is needed: rows or out")
     if out is None:
@@ -703,7 +772,7 @@ def _run_group(ids, order, place, offsets, groups):
 
 
 def _trace_group(ids, groups, plan):
-    groups = int(groups)
+    ids, plan, groups = _lift(ids), None if plan is None else tuple(map(_lift, plan)), int(groups)
     if plan is None:
         i32 = np.dtype(np.int32)
         plan = ((_size(ids.shape),), i32), (tuple(ids.shape), i32), ((groups + 1,), i32)
@@ -716,10 +785,11 @@ def _run_dispatch(x, place, offsets, out):
 
 
 def _trace_dispatch(x, ids, groups, out, plan):
+    x, out = _lift(x), _lift(out)
     if isinstance(ids, RowGroups):
         if groups is not None or plan is not None:
             raise ValueError("groups and plan are for ids that are not sorted yet")
-        plan = ids
+        plan = RowGroups(*map(_lift, ids))
     else:
         if groups is None:
             raise ValueError("the number of groups is needed")
@@ -735,6 +805,7 @@ def _run_combine(ys, place, offsets, out, weights=None):
 
 
 def _trace_combine(ys, plan, weights, out):
+    ys, weights, out, plan = _lift(ys), _lift(weights), _lift(out), (None, _lift(plan[1]), _lift(plan[2]))
     shape = (plan[1].shape[0], ys.shape[-1])
     (res,) = _step(_run_combine, {"ys": ys, "place": plan[1], "offsets": plan[2], "weights": weights}, {},
                    {"out": out if out is not None else (shape, _row_type(ys))})
@@ -746,6 +817,8 @@ def _run_combine_grad(dout, ys, place, offsets, out, dweights, weights=None):
 
 
 def _trace_combine_grad(dout, ys, plan, weights, out, dweights):
+    dout, ys, weights, out, dweights = map(_lift, (dout, ys, weights, out, dweights))
+    plan = (None, _lift(plan[1]), _lift(plan[2]))
     wt = _row_type(weights) if weights is not None else np.dtype(np.float32)
     return tuple(_step(
         _run_combine_grad,

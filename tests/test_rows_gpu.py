@@ -666,3 +666,82 @@ def test_positions_outside_are_left_out(queue):
     dys, dw = nm.combine_rows_grad(dev(np.ones((2, 3), np.float32)), ys, plan, out=out)
     assert dw.copy_to_host().tolist() == [[3.0, 0.0], [0.0, 0.0]]
     assert dys.copy_to_host().tolist() == [[1.0] * 3] + [[9.0] * 3] * 3
+
+
+@pytest.mark.parametrize("source", ["device", "torch"])
+def test_native_path_takes_ordinary_calls(queue, source):
+    """The native call path answers 1 for calls in order, 0 for the others, and
+    writes what the Python path writes."""
+    import torch
+
+    import numba_mlir_b200 as nm
+    from numba_mlir_b200 import rows
+
+    rng = np.random.default_rng(4)
+    ids = rng.integers(-1, 9, (50, 2)).astype(np.int32)
+    host = {"table": rng.standard_normal((9, 24)).astype(np.float32), "ids": ids, "x": rng.standard_normal((50, 24)).astype(np.float32),
+            "w": rng.random((50, 2)).astype(np.float32)}
+    if source == "torch":
+        put = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+        new = lambda shape, dt=np.float32: torch.zeros(shape, dtype=torch.float32 if dt == np.float32 else torch.int32, device="cuda")  # noqa: E731
+        get = lambda t: t.cpu().numpy()  # noqa: E731
+        q = rows._torch_stream(0)
+        nm.take_rows(put(host["table"]), put(ids), out=new((50, 2, 24)))  # the first tensor binds
+    else:
+        put, get, q = dev, (lambda t: t.copy_to_host()), queue
+        new = lambda shape, dt=np.float32: nm.zeros(shape, dt, queue=queue)  # noqa: E731
+        nm.take_rows(put(host["table"]), put(ids), out=new((50, 2, 24)))
+    rows._raw_stream(q)
+    fast = rows._fast()
+    table, i, x, w = (put(host[n]) for n in ("table", "ids", "x", "w"))
+    picked, grad = new((50, 2, 24)), new((9, 24))
+    plan = nm.RowGroups(new((100,), np.int32), new((50, 2), np.int32), new((10,), np.int32))
+    xs, y, dys, dw = new((100, 24)), new((50, 24)), new((100, 24)), new((50, 2))
+    assert fast.rows_take(q, table, i, 1.5, picked) == 1
+    assert fast.rows_take_grad(q, picked, i, 1.5, grad, False) == 1
+    assert fast.rows_group(q, i, 9, plan) == 1
+    assert fast.rows_dispatch(q, x, None, None, plan, xs) == 1
+    assert fast.rows_dispatch(q, x, i, 9, plan, xs) == 1
+    assert fast.rows_combine(q, xs, plan, w, y) == 1
+    assert fast.rows_combine(q, xs, plan, None, y) == 1
+    assert fast.rows_combine(q, xs, plan, w, y) == 1
+    assert fast.rows_combine_grad(q, x, xs, plan, w, dys, dw) == 1
+    d = {n: dev(a) for n, a in host.items()}
+    picked2 = nm.take_rows(d["table"], d["ids"], 1.5)
+    grad2 = nm.take_rows_grad(picked2, d["ids"], 9, 1.5)
+    xs2, plan2 = nm.dispatch_rows(d["x"], d["ids"], 9)
+    y2 = nm.combine_rows(xs2, plan2, d["w"])
+    dys2, dw2 = nm.combine_rows_grad(d["x"], xs2, plan2, d["w"])
+    for a, b in ((picked, picked2), (grad, grad2), (xs, xs2), (y, y2), (dys, dys2), (dw, dw2), *zip(plan, plan2)):
+        assert get(a).tobytes() == b.copy_to_host().tobytes()
+    # out of order: another queue, a wrong shape, type or overlap, a missing result
+    other = nm.runtime.Queue("cuda:0")
+    rows._raw_stream(other)
+    assert fast.rows_take(other, table, i, 1.5, picked) == 0
+    assert fast.rows_take(q, table, i, 1.5, xs) == 0
+    assert fast.rows_take(q, table, w, 1.5, picked) == 0
+    assert fast.rows_take(q, table, i, "x", picked) == 0
+    assert fast.rows_take(q, table, i, 1.5, None) == 0
+    assert fast.rows_take(q, host["table"], i, 1.5, picked) == 0
+    assert fast.rows_dispatch(q, xs[:50], None, None, plan, xs) == 0
+    assert fast.rows_combine(q, xs, plan, w[:40], y) == 0
+    assert fast.rows_combine(q, xs, (1, 2), w, y) == 0
+    assert fast.rows_combine_grad(q, x, xs[:90], plan, w, dys, dw) == 0
+
+
+def test_arrays_captured_by_a_traced_function(queue):
+    """A routine called inside a traced function on arrays that are not its
+    arguments runs in every call, not only in the traced one."""
+    import numba_mlir_b200 as nm
+
+    table, ids, out = dev(np.ones((4, 3), np.float32)), dev(np.array([1, 2], np.int32)), nm.zeros((2, 3), np.float32, queue=queue)
+
+    @nm.njit(parallel=True)
+    def f(a):
+        nm.take_rows(table, ids, 2.0, out=out)
+        return a + np.float32(1)
+
+    for v in (1.0, 5.0):
+        table.copy_from_host(np.full((4, 3), v, np.float32))
+        f(dev(np.zeros(3, np.float32)))
+        assert (out.copy_to_host() == 2 * v).all()
