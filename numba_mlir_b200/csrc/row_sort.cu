@@ -6,15 +6,18 @@
 // to 1023 groups (experts), two up to a million (a vocabulary).  Nothing
 // depends on the order in which blocks or atomics run: a block counts its own
 // entries, counts are added up in block order, and the rank of an entry among
-// the equal digits of its warp's 32 comes from a match over the warp.
+// the equal digits of its warp's 32 comes from votes over the warp.
 //
-// What it costs is latency, not bandwidth (an entry is 8 bytes).  Up to 8192
-// entries stay in one block's shared memory for all passes: one launch.  More
-// take three launches a pass: blocks count tiles of 4096 entries, a warp per
-// digit adds the counts up over the blocks, blocks scatter their tiles.
+// What it costs is latency, not bandwidth (an entry is 8 bytes), so the number
+// of dependent steps is what the three forms differ in.  Up to 4096 entries
+// stay in one block's shared memory for all passes: one launch.  Up to about a
+// million take two launches a pass: blocks of 1024 threads count their tiles,
+// then scatter them, each adding up the counts of all blocks for itself (at
+// most 148 of them).  Beyond that a launch in between adds the counts up.
 #include "rows_host.h"
 
 #include <atomic>
+#include <type_traits>
 
 #define GPUX_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -34,22 +37,6 @@ struct Ids {
     return id >= 0 && id < (int64_t)groups ? (uint32_t)id : groups;
   }
 };
-
-// Rank of this lane's digit among the equal digits of the lanes before it, and
-// the running count of that digit in `count` (one word per digit, this warp's
-// own): the first lane of each set of equals adds the set's size.
-__device__ __forceinline__ uint32_t warp_rank(uint32_t digit, bool live, uint32_t *count) {
-  const int lane = threadIdx.x & 31;
-  const unsigned peers = __match_any_sync(kAll, live ? digit : 0xffffffffu);
-  const int first = __ffs(peers) - 1;
-  uint32_t base = 0;
-  if (live && lane == first) {
-    base = count[digit];
-    count[digit] = base + __popc(peers);
-  }
-  base = __shfl_sync(kAll, base, first);
-  return base + __popc(peers & ((1u << lane) - 1));
-}
 
 // Exclusive prefix of v over the block's threads (blockDim.x a multiple of 32);
 // `sums` holds 32 words.
@@ -82,11 +69,10 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *sums) {
   return before;
 }
 
-// ---- one block ----------------------------------------------------------------
-constexpr int kOneThreads = 1024;
-constexpr int kOnePerThread = 8;
-constexpr int kOneMax = kOneThreads * kOnePerThread;
-constexpr int kOneSmem = (32 * kBins + 2 * kOneMax + 32 + 1) * 4; // counts, keys, entries, prefix sums, total
+constexpr int kThreads = 1024;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMostPerThread = 8;
+constexpr int kMostBlocks = 148;
 
 struct Results {
   int32_t *order;
@@ -105,131 +91,165 @@ struct Clear {
   }
 };
 
-__global__ void __launch_bounds__(kOneThreads)
-    nmb_sort_one(const Ids ids, int n, int bits, int passes, const Results res, const Clear clear) {
-  clear.run();
-  extern __shared__ uint32_t smem[];
-  uint32_t *counts = smem;                 // [warps][bins]
-  uint32_t *keys = smem + 32 * kBins;      // [n]
-  uint32_t *entries = keys + kOneMax;      // [n]
-  uint32_t *sums = entries + kOneMax;      // [32]
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int warps = blockDim.x >> 5;
-  const int digit_bits = (bits + passes - 1) / passes, bins = 1 << digit_bits;
-  // a warp owns a contiguous run of `span` entries, 32 at a time
-  const int span = ((n + warps - 1) / warps + 31) / 32 * 32;
-  const int begin = warp * span;
+// Ranks of a block's entries among its entries of equal digit, and where each
+// digit's entries go.  `counts` are per warp: counts[w][d] holds, in turn, the
+// entries of digit d in warp w and the digit's entries in the warps before w.
+// A digit is looked after by blockDim.x / bins threads, each of which adds up
+// its share of the warps (and of the blocks).
+struct Digits {
+  uint16_t *counts;  // [warps][bins]
+  uint32_t *local;   // [threads]: a thread's share, then [bins] where the digit begins
+  uint32_t *sums;    // [32]
+  int bins, shift;
+  __device__ __forceinline__ uint32_t of(uint32_t key) const { return (key >> shift) & (uint32_t)(bins - 1); }
 
-  for (int i = tid; i < n; i += blockDim.x) {
-    keys[i] = ids.key(i);
-    entries[i] = i;
+  __device__ __forceinline__ void clear() const {
+    uint32_t *words = reinterpret_cast<uint32_t *>(counts);
+    for (int i = threadIdx.x; i < (int)(blockDim.x >> 5) * bins / 2; i += blockDim.x)
+      words[i] = 0;
+  }
+
+  // Rank of this lane's digit among the equal digits of the lanes before it and
+  // of the calls before this one.  The lanes with the same digit find one
+  // another bit by bit; the first of them moves the warp's count.
+  __device__ __forceinline__ uint32_t rank(uint32_t digit, bool live) const {
+    const int lane = threadIdx.x & 31;
+    unsigned peers = __ballot_sync(kAll, live);
+    for (int b = 1; b < bins; b <<= 1) {
+      const unsigned ones = __ballot_sync(kAll, digit & b);
+      peers &= digit & b ? ones : ~ones;
+    }
+    uint16_t *mine = counts + (threadIdx.x >> 5) * bins + digit;
+    const uint32_t before = live ? *mine : 0;
+    __syncwarp();
+    const unsigned lower = peers & ((1u << lane) - 1);
+    if (live && lower == 0)
+      *mine = (uint16_t)(before + __popc(peers));
+    __syncwarp();
+    return before + __popc(lower);
+  }
+};
+
+// ---- one block ------------------------------------------------------------------
+template <int PER>
+__global__ void __launch_bounds__(kThreads)
+    nmb_sort_one(const Ids ids, int n, int bits, int passes, const Results res, const Clear clear) {
+  extern __shared__ uint32_t smem[];
+  uint32_t *keys = smem, *entries = smem + kThreads * PER;
+  Digits dg{reinterpret_cast<uint16_t *>(entries + kThreads * PER), nullptr, nullptr, 0, 0};
+  dg.local = reinterpret_cast<uint32_t *>(dg.counts + kWarps * kBins);
+  dg.sums = dg.local + kBins;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  const int digit_bits = (bits + passes - 1) / passes;
+  dg.bins = 1 << digit_bits;
+  const int begin = warp * PER * 32 + lane; // a warp owns PER * 32 consecutive entries
+  clear.run();
+  uint32_t key[PER], entry[PER], rank[PER];
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    entry[u] = begin + u * 32;
+    key[u] = begin + u * 32 < n ? ids.key(begin + u * 32) : 0;
   }
   for (int pass = 0; pass < passes; ++pass) {
-    const int shift = pass * digit_bits;
-    for (int i = tid; i < warps * bins; i += blockDim.x)
-      counts[i] = 0;
+    dg.shift = pass * digit_bits;
+    dg.clear();
     __syncthreads();
-    uint32_t key[kOnePerThread], entry[kOnePerThread], rank[kOnePerThread];
 #pragma unroll
-    for (int u = 0; u < kOnePerThread; ++u) {
-      const int i = begin + u * 32 + lane;
-      if (u * 32 < span) { // the same for all lanes
-        const bool live = i < n;
-        key[u] = live ? keys[i] : 0;
-        entry[u] = live ? entries[i] : 0;
-        rank[u] = warp_rank((key[u] >> shift) & (bins - 1), live, counts + warp * bins);
-        __syncwarp();
+    for (int u = 0; u < PER; ++u) {
+      const int i = begin + u * 32;
+      if (pass > 0 && i < n) {
+        key[u] = keys[i];
+        entry[u] = entries[i];
       }
+      rank[u] = dg.rank(dg.of(key[u]), i < n);
     }
     __syncthreads();
-    // counts[w][d] <- entries of digit d in the warps before w; the digits'
-    // totals go through a prefix over the block, up to `per` digits a thread
-    const int per = (bins + blockDim.x - 1) / blockDim.x;
+    // a thread (or a few, when there are fewer threads than digits) per digit
+    const int each = (dg.bins + blockDim.x - 1) / blockDim.x;
+    const int d0 = min(tid * each, dg.bins), d1 = min(d0 + each, dg.bins);
     uint32_t total = 0;
-    for (int b = tid * per; b < min((tid + 1) * per, bins); ++b) {
+    for (int d = d0; d < d1; ++d) {
+      dg.local[d] = total;
       for (int w = 0; w < warps; ++w) {
-        const uint32_t c = counts[w * bins + b];
-        counts[w * bins + b] = total;
+        const uint32_t c = dg.counts[w * dg.bins + d];
+        dg.counts[w * dg.bins + d] = (uint16_t)(total - dg.local[d]);
         total += c;
       }
     }
-    const uint32_t before = block_prefix(total, sums);
-    for (int b = tid * per; b < min((tid + 1) * per, bins); ++b) {
-      for (int w = 0; w < warps; ++w)
-        counts[w * bins + b] += before;
-      if (passes == 1 && res.offsets && b <= (int)ids.groups)
-        res.offsets[b] = (int32_t)counts[b];
+    const uint32_t before = block_prefix(total, dg.sums);
+    for (int d = d0; d < d1; ++d) {
+      dg.local[d] += before;
+      if (passes == 1 && res.offsets && d <= (int)ids.groups)
+        res.offsets[d] = (int32_t)dg.local[d];
     }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kOnePerThread; ++u) {
-      const int i = begin + u * 32 + lane;
-      if (u * 32 < span && i < n) {
-        const uint32_t at = counts[warp * bins + ((key[u] >> shift) & (bins - 1))] + rank[u];
-        keys[at] = key[u];
-        entries[at] = entry[u];
+    for (int u = 0; u < PER; ++u) {
+      if (begin + u * 32 < n) {
+        const uint32_t d = dg.of(key[u]), at = dg.local[d] + dg.counts[warp * dg.bins + d] + rank[u];
+        if (pass + 1 == passes) {
+          if (res.order)
+            res.order[at] = (int32_t)entry[u];
+          if (res.keys)
+            res.keys[at] = key[u];
+          if (res.place)
+            res.place[entry[u]] = (int32_t)at;
+        } else {
+          keys[at] = key[u];
+          entries[at] = entry[u];
+        }
       }
     }
     __syncthreads();
   }
-  for (int i = tid; i < n; i += blockDim.x) {
-    const uint32_t e = entries[i];
-    if (res.order)
-      res.order[i] = (int32_t)e;
-    if (res.keys)
-      res.keys[i] = keys[i];
-    if (res.place)
-      res.place[e] = i;
-  }
+}
+template <int PER> constexpr int oneBytes() {
+  return 2 * kThreads * PER * 4 + kWarps * kBins * 2 + kBins * 4 + 32 * 4;
 }
 
-// ---- many blocks --------------------------------------------------------------
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kPerThread = 16;
-constexpr int kTile = kThreads * kPerThread;
-
+// ---- many blocks ----------------------------------------------------------------
 struct Pass {
   Ids ids;                 // the first pass reads its keys here (keysIn == nullptr)
   const uint32_t *keysIn;
   const int32_t *entriesIn;
-  uint32_t *counts;        // [bins][blocks]
-  uint32_t *totals;        // [bins]
+  uint32_t *counts;        // [blocks][bins]: of each block; with `added`, of the blocks before it
+  uint32_t *totals;        // [bins], with `added`
   int64_t n;
-  int blocks, shift, bins;
+  int blocks, shift, bins, added;
   __device__ __forceinline__ uint32_t key(int64_t i) const { return keysIn ? keysIn[i] : ids.key(i); }
   __device__ __forceinline__ uint32_t digit(uint32_t k) const { return (k >> shift) & (uint32_t)(bins - 1); }
 };
 
-__global__ void __launch_bounds__(kThreads) nmb_sort_count(const Pass p, const Clear clear) {
-  clear.run();
+template <int PER> __global__ void __launch_bounds__(kThreads) nmb_sort_count(const Pass p, const Clear clear) {
   __shared__ uint32_t count[kBins];
+  const int64_t base = (int64_t)blockIdx.x * kThreads * PER + threadIdx.x;
+  uint32_t key[PER];
+#pragma unroll
+  for (int u = 0; u < PER; ++u)
+    key[u] = base + u * kThreads < p.n ? p.key(base + u * kThreads) : 0;
+  clear.run();
   for (int b = threadIdx.x; b < p.bins; b += kThreads)
     count[b] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kTile;
-#pragma unroll 4
-  for (int u = 0; u < kPerThread; ++u) {
-    const int64_t i = base + u * kThreads + threadIdx.x;
-    if (i < p.n)
-      atomicAdd(&count[p.digit(p.key(i))], 1u);
-  }
+#pragma unroll
+  for (int u = 0; u < PER; ++u)
+    if (base + u * kThreads < p.n)
+      atomicAdd(&count[p.digit(key[u])], 1u);
   __syncthreads();
   for (int b = threadIdx.x; b < p.bins; b += kThreads)
-    p.counts[(int64_t)b * p.blocks + blockIdx.x] = count[b];
+    p.counts[(int64_t)blockIdx.x * p.bins + b] = count[b];
 }
 
-// A warp per digit: counts[d][b] <- sum of counts[d][0..b), totals[d] <- the sum.
-__global__ void __launch_bounds__(kThreads) nmb_sort_prefix(uint32_t *counts, uint32_t *totals, int blocks, int bins) {
-  const int lane = threadIdx.x & 31;
-  const int d = blockIdx.x * kWarps + (threadIdx.x >> 5);
+// A warp per digit: counts[b][d] <- sum of counts[0..b)[d], totals[d] <- the sum.
+constexpr int kAddThreads = 256;
+__global__ void __launch_bounds__(kAddThreads) nmb_sort_add(uint32_t *counts, uint32_t *totals, int blocks, int bins) {
+  const int lane = threadIdx.x & 31, d = blockIdx.x * (kAddThreads / 32) + (threadIdx.x >> 5);
   if (d >= bins)
     return;
-  uint32_t *row = counts + (int64_t)d * blocks;
   uint32_t carry = 0;
   for (int b0 = 0; b0 < blocks; b0 += 32) {
-    const int b = b0 + lane;
-    const uint32_t v = b < blocks ? row[b] : 0;
+    uint32_t *at = counts + (int64_t)(b0 + lane) * bins + d;
+    const uint32_t v = b0 + lane < blocks ? *at : 0;
     uint32_t inc = v;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
@@ -237,85 +257,118 @@ __global__ void __launch_bounds__(kThreads) nmb_sort_prefix(uint32_t *counts, ui
       if (lane >= s)
         inc += t;
     }
-    if (b < blocks)
-      row[b] = carry + inc - v;
+    if (b0 + lane < blocks)
+      *at = carry + inc - v;
     carry += __shfl_sync(kAll, inc, 31);
   }
   if (lane == 0)
     totals[d] = carry;
 }
 
+template <int PER>
 __global__ void __launch_bounds__(kThreads)
     nmb_sort_scatter(const Pass p, uint32_t *keysOut, int32_t *entriesOut, int32_t *place, int32_t *offsets) {
-  __shared__ uint32_t counts[kWarps][kBins];
-  __shared__ uint32_t start[kBins];
-  __shared__ uint32_t sums[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < kWarps * kBins; i += kThreads)
-    (&counts[0][0])[i] = 0;
-  // where each digit's entries begin in the output: prefix of the totals
-  {
-    constexpr int kPer = kBins / kThreads;
-    uint32_t mine[kPer], sum = 0;
+  extern __shared__ uint32_t smem[];
+  uint32_t *before = smem;                // [threads]: a thread's blocks before this one, all its blocks
+  uint32_t *all = smem + kThreads;        // [threads]
+  Digits dg{reinterpret_cast<uint16_t *>(all + kThreads), nullptr, nullptr, p.bins, p.shift};
+  dg.local = reinterpret_cast<uint32_t *>(dg.counts + kWarps * kBins);
+  dg.sums = dg.local + kBins;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t begin = ((int64_t)blockIdx.x * kWarps + warp) * PER * 32 + lane;
+  uint32_t key[PER], rank[PER];
+  int32_t entry[PER];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int d = threadIdx.x * kPer + j;
-      mine[j] = sum;
-      sum += d < p.bins ? p.totals[d] : 0;
-    }
-    const uint32_t before = block_prefix(sum, sums);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      start[threadIdx.x * kPer + j] = before + mine[j];
-  }
-  __syncthreads();
-  if (offsets && blockIdx.x == 0)
-    for (int d = threadIdx.x; d <= (int)p.ids.groups; d += kThreads)
-      offsets[d] = (int32_t)start[d];
-  // a warp owns 512 consecutive entries of the tile, 32 at a time
-  const int64_t base = (int64_t)blockIdx.x * kTile + warp * (kTile / kWarps);
-  uint32_t key[kPerThread], rank[kPerThread];
-#pragma unroll
-  for (int u = 0; u < kPerThread; ++u) {
-    const int64_t i = base + u * 32 + lane;
+  for (int u = 0; u < PER; ++u) {
+    const int64_t i = begin + u * 32;
     key[u] = i < p.n ? p.key(i) : 0;
+    entry[u] = i < p.n && p.entriesIn ? p.entriesIn[i] : (int32_t)i;
   }
+  dg.clear();
+  // counts of the blocks: thread t adds up blocks t / bins, + share, ... of digit t % bins
+  const int share = kThreads / p.bins, d = tid & (p.bins - 1), part = tid / p.bins;
+  uint32_t mine = 0, sum = 0;
+  if (p.added) {
+    if (part == 0) {
+      mine = p.counts[(int64_t)blockIdx.x * p.bins + d];
+      sum = p.totals[d];
+    }
+  } else {
+    // sixteen loads in flight: one by one they took 15 of the kernel's 19 us at
+    // 131072 entries (an L2 access costs about 700 cycles)
+    for (int b0 = part; b0 < p.blocks; b0 += 16 * share) {
+      uint32_t c[16];
 #pragma unroll
-  for (int u = 0; u < kPerThread; ++u) {
-    rank[u] = warp_rank(p.digit(key[u]), base + u * 32 + lane < p.n, counts[warp]);
-    __syncwarp();
-  }
-  __syncthreads();
-  for (int d = threadIdx.x; d < p.bins; d += kThreads) {
-    uint32_t at = start[d] + p.counts[(int64_t)d * p.blocks + blockIdx.x];
+      for (int u = 0; u < 16; ++u)
+        c[u] = b0 + u * share < p.blocks ? __ldg(p.counts + (int64_t)(b0 + u * share) * p.bins + d) : 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const uint32_t c = counts[w][d];
-      counts[w][d] = at;
-      at += c;
+      for (int u = 0; u < 16; ++u) {
+        mine += b0 + u * share < (int)blockIdx.x ? c[u] : 0;
+        sum += c[u];
+      }
     }
   }
+  before[tid] = mine;
+  all[tid] = sum;
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < kPerThread; ++u) {
-    const int64_t i = base + u * 32 + lane;
-    if (i < p.n) {
-      const uint32_t at = counts[warp][p.digit(key[u])] + rank[u];
-      const int32_t e = p.entriesIn ? p.entriesIn[i] : (int32_t)i;
+  for (int u = 0; u < PER; ++u)
+    rank[u] = dg.rank(dg.of(key[u]), begin + u * 32 < p.n);
+  if (tid < p.bins) {
+    for (int s = 1; s < share; ++s) {
+      mine += before[s * p.bins + d];
+      sum += all[s * p.bins + d];
+    }
+  } else {
+    mine = sum = 0;
+  }
+  const uint32_t start = block_prefix(sum, dg.sums); // the digits begin there; every warp's counts are done
+  if (tid < p.bins) {
+    if (offsets && blockIdx.x == 0 && d <= (int)p.ids.groups)
+      offsets[d] = (int32_t)start;
+    dg.local[d] = start + mine;
+  }
+  // warps before each warp: this thread's share of the warps, then the shares
+  const int rows = kWarps / (share < kWarps ? share : kWarps);
+  uint32_t count = 0;
+  if (part * rows < kWarps)
+    for (int w = part * rows; w < (part + 1) * rows; ++w) {
+      const uint32_t c = dg.counts[w * p.bins + d];
+      dg.counts[w * p.bins + d] = (uint16_t)count;
+      count += c;
+    }
+  __syncthreads();
+  before[tid] = count;
+  __syncthreads();
+  if (part * rows < kWarps) {
+    uint32_t shift = 0;
+    for (int s = 0; s < part; ++s)
+      shift += before[s * p.bins + d];
+    for (int w = part * rows; w < (part + 1) * rows; ++w)
+      dg.counts[w * p.bins + d] += (uint16_t)shift;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    if (begin + u * 32 < p.n) {
+      const uint32_t digit = dg.of(key[u]);
+      const uint32_t at = dg.local[digit] + dg.counts[warp * p.bins + digit] + rank[u];
       if (keysOut)
         keysOut[at] = key[u];
       if (entriesOut)
-        entriesOut[at] = e;
+        entriesOut[at] = entry[u];
       if (place)
-        place[e] = (int32_t)at;
+        place[entry[u]] = (int32_t)at;
     }
   }
 }
+constexpr int kScatterBytes = 2 * kThreads * 4 + kWarps * kBins * 2 + kBins * 4 + 32 * 4;
 
 // offsets[g] = position of the first key >= g, for the sorts of several passes.
-__global__ void __launch_bounds__(kThreads)
+constexpr int kOffsetThreads = 256;
+__global__ void __launch_bounds__(kOffsetThreads)
     nmb_sort_offsets(const uint32_t *keys, int64_t n, int64_t groups, int32_t *offsets) {
-  const int64_t g = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t g = (int64_t)blockIdx.x * kOffsetThreads + threadIdx.x;
   if (g > groups)
     return;
   int64_t lo = 0, hi = n;
@@ -329,8 +382,8 @@ __global__ void __launch_bounds__(kThreads)
   offsets[g] = (int32_t)lo;
 }
 
-__global__ void __launch_bounds__(kThreads) nmb_sort_nothing(int64_t groups, int32_t *offsets) {
-  const int64_t g = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+__global__ void __launch_bounds__(kOffsetThreads) nmb_sort_nothing(int64_t groups, int32_t *offsets) {
+  const int64_t g = (int64_t)blockIdx.x * kOffsetThreads + threadIdx.x;
   if (g <= groups)
     offsets[g] = 0;
 }
@@ -344,9 +397,47 @@ int bitsOf(int64_t groups) {
 
 size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-int64_t tiles(int64_t n) { return (n + kTile - 1) / kTile; }
+constexpr int64_t kOneMost = 4096;
+bool fitsOneBlock(int64_t n) { return n <= kOneMost; }
 
-bool fitsOneBlock(int64_t n) { return n <= kOneMax; }
+// Entries per thread of the many blocks: the fewest that keep them at 148 at
+// most, and never more than 8.
+int perThread(int64_t n) {
+  int per = 1;
+  while (per < kMostPerThread && n > (int64_t)per * kThreads * kMostBlocks)
+    per *= 2;
+  return per;
+}
+int64_t manyBlocks(int64_t n) {
+  const int64_t tile = (int64_t)perThread(n) * kThreads;
+  return (n + tile - 1) / tile;
+}
+
+// Calls f(constant) for 1, 2, 4 or 8.
+template <typename F> bool withPer(int per, F &&f) {
+  if (per == 1)
+    return f(std::integral_constant<int, 1>());
+  if (per == 2)
+    return f(std::integral_constant<int, 2>());
+  if (per == 4)
+    return f(std::integral_constant<int, 4>());
+  return f(std::integral_constant<int, 8>());
+}
+
+// Lets a kernel use more than 48 KB of shared memory; once per kernel and device.
+template <typename K> bool allowShared(const char *who, K kernel, int bytes, std::atomic<bool> *ready, int device) {
+  if (device >= 0 && device < 64 && ready[device])
+    return true;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) {
+    nmb::setError("%s: cudaFuncSetAttribute failed: %s", who, cudaGetErrorString(e));
+    (void)cudaGetLastError();
+    return false;
+  }
+  if (device >= 0 && device < 64)
+    ready[device] = true;
+  return true;
+}
 
 } // namespace
 
@@ -360,7 +451,7 @@ size_t sortBytes(int64_t count, int64_t groups) {
   const size_t pairs = padded((size_t)count * 4);
   if (fitsOneBlock(count))
     return bitsOf(groups) > kMaxDigitBits ? pairs : 0; // the sorted keys, for the offsets
-  return 4 * pairs + padded((size_t)kBins * (size_t)tiles(count) * 4) + padded(kBins * 4);
+  return 4 * pairs + padded((size_t)kBins * (size_t)manyBlocks(count) * 4) + padded(kBins * 4);
 }
 
 bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t groups, int32_t *order,
@@ -369,11 +460,11 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
   const int64_t n = ids.count;
   const Ids in{ids.data, ids.bytes, (uint32_t)groups};
   const int bits = bitsOf(groups), passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
-  const unsigned offsetBlocks = (unsigned)((groups + kThreads) / kThreads);
+  const unsigned offsetBlocks = (unsigned)((groups + kOffsetThreads) / kOffsetThreads);
   if (n == 0) {
     if (!offsets)
       return true;
-    nmb_sort_nothing<<<offsetBlocks, kThreads, 0, s.stream>>>(groups, offsets);
+    nmb_sort_nothing<<<offsetBlocks, kOffsetThreads, 0, s.stream>>>(groups, offsets);
     return launched(who);
   }
   unsigned char *ws = static_cast<unsigned char *>(workspace);
@@ -381,58 +472,61 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
   if (passes > 1 && offsets && !keys)
     keys = reinterpret_cast<uint32_t *>(ws); // the sorted keys, wanted for the offsets below
   if (fitsOneBlock(n)) {
-    static std::atomic<bool> ready[64]; // per device; setting it twice is harmless
-    if (s.device < 0 || s.device >= 64 || !ready[s.device]) {
-      const cudaError_t e =
-          cudaFuncSetAttribute(nmb_sort_one, cudaFuncAttributeMaxDynamicSharedMemorySize, kOneSmem);
-      if (e != cudaSuccess) {
-        setError("%s: cudaFuncSetAttribute failed: %s", who, cudaGetErrorString(e));
-        (void)cudaGetLastError();
+    const int per = n <= kThreads ? 1 : n <= 2 * kThreads ? 2 : 4;
+    const bool ok = withPer(per, [&](auto P) {
+      constexpr int kPer = P.value < 4 ? P.value : 4;
+      static std::atomic<bool> ready[64];
+      if (!allowShared(who, nmb_sort_one<kPer>, oneBytes<kPer>(), ready, s.device))
         return false;
-      }
-      if (s.device >= 0 && s.device < 64)
-        ready[s.device] = true;
-    }
-    // as many warps as there are rows of 32 entries
-    const int warps = (int)(n + 31) / 32 < 32 ? (int)(n + 31) / 32 : 32;
-    nmb_sort_one<<<1, warps * 32, kOneSmem, s.stream>>>(in, (int)n, bits, passes,
-                                                        Results{order, keys, place, passes == 1 ? offsets : nullptr},
-                                                        Clear{clear, clearWords});
-    if (!launched(who))
+      // as many warps as the entries fill
+      const int warps = (int)((n + 32 * kPer - 1) / (32 * kPer));
+      nmb_sort_one<kPer><<<1, warps * 32, oneBytes<kPer>(), s.stream>>>(
+          in, (int)n, bits, passes, Results{order, keys, place, passes == 1 ? offsets : nullptr},
+          Clear{clear, clearWords});
+      return launched(who);
+    });
+    if (!ok)
       return false;
   } else {
-    const int64_t blocks = tiles(n);
+    const int64_t blocks = manyBlocks(n);
     uint32_t *keyBuf[2] = {reinterpret_cast<uint32_t *>(ws), reinterpret_cast<uint32_t *>(ws + pairs)};
     int32_t *entryBuf[2] = {reinterpret_cast<int32_t *>(ws + 2 * pairs), reinterpret_cast<int32_t *>(ws + 3 * pairs)};
     uint32_t *counts = reinterpret_cast<uint32_t *>(ws + 4 * pairs);
     uint32_t *totals =
         reinterpret_cast<uint32_t *>(ws + 4 * pairs + padded((size_t)kBins * (size_t)blocks * 4));
     const int digitBits = (bits + passes - 1) / passes;
-    Pass p{in, nullptr, nullptr, counts, totals, n, (int)blocks, 0, 1 << digitBits};
+    Pass p{in, nullptr, nullptr, counts, totals, n, (int)blocks, 0, 1 << digitBits, blocks > kMostBlocks};
     for (int pass = 0; pass < passes; ++pass) {
       const bool last = pass + 1 == passes;
       // the passes alternate between the buffers so that the last one may write
       // sorted keys into buffer 0 (see above)
       const int to = (passes - 1 - pass) & 1;
       p.shift = pass * digitBits;
-      nmb_sort_count<<<(unsigned)blocks, kThreads, 0, s.stream>>>(p, Clear{clear, pass == 0 ? clearWords : 0});
-      if (!launched(who))
-        return false;
-      nmb_sort_prefix<<<(unsigned)((p.bins + kWarps - 1) / kWarps), kThreads, 0, s.stream>>>(counts, totals,
-                                                                                             (int)blocks, p.bins);
-      if (!launched(who))
-        return false;
-      nmb_sort_scatter<<<(unsigned)blocks, kThreads, 0, s.stream>>>(
-          p, last ? keys : keyBuf[to], last ? order : entryBuf[to], last ? place : nullptr,
-          passes == 1 ? offsets : nullptr);
-      if (!launched(who))
+      const bool ok = withPer(perThread(n), [&](auto P) {
+        static std::atomic<bool> ready[64];
+        if (!allowShared(who, nmb_sort_scatter<P.value>, kScatterBytes, ready, s.device))
+          return false;
+        nmb_sort_count<P.value><<<(unsigned)blocks, kThreads, 0, s.stream>>>(p, Clear{clear, pass == 0 ? clearWords : 0});
+        if (!launched(who))
+          return false;
+        if (p.added) {
+          nmb_sort_add<<<(unsigned)((p.bins + kAddThreads / 32 - 1) / (kAddThreads / 32)), kAddThreads, 0, s.stream>>>(counts, totals, (int)blocks, p.bins);
+          if (!launched(who))
+            return false;
+        }
+        nmb_sort_scatter<P.value><<<(unsigned)blocks, kThreads, kScatterBytes, s.stream>>>(
+            p, last ? keys : keyBuf[to], last ? order : entryBuf[to], last ? place : nullptr,
+            passes == 1 ? offsets : nullptr);
+        return launched(who);
+      });
+      if (!ok)
         return false;
       p.keysIn = keyBuf[to];
       p.entriesIn = entryBuf[to];
     }
   }
   if (offsets && passes > 1) {
-    nmb_sort_offsets<<<offsetBlocks, kThreads, 0, s.stream>>>(keys, n, groups, offsets);
+    nmb_sort_offsets<<<offsetBlocks, kOffsetThreads, 0, s.stream>>>(keys, n, groups, offsets);
     return launched(who);
   }
   return true;
