@@ -13,6 +13,7 @@
 // moves `V` neighbouring elements per access (16 bytes where alignment and
 // width allow), and blocks take several short rows or one long one.  Arithmetic
 // is float32 (float64 for float64 rows) and rounds once, on the way out.
+#include "kernels/bulk_pipe.cuh"
 #include "rows_host.h"
 
 #include <type_traits>
@@ -92,13 +93,16 @@ template <typename A> __device__ __forceinline__ void set_scalar(void *p, int ty
 }
 
 // ------------------------------------------------------------------- take ---
+// A thread has up to four accesses of a row in flight.
+constexpr int kTakeBatch = 4;
+
 template <typename I, typename O, int V>
 __global__ void __launch_bounds__(kThreads)
     nmb_take_rows(const I *__restrict__ table, int64_t rows, int64_t stride, const void *__restrict__ ids, int id_bytes,
                   int64_t n, typename Acc<I>::type scale, O *__restrict__ out, int64_t out_stride, int64_t vecs,
                   int lane_bits) {
   using A = typename Acc<I>::type;
-  const int lane = threadIdx.x & ((1 << lane_bits) - 1);
+  const int lanes = 1 << lane_bits, lane = threadIdx.x & (lanes - 1);
   const int64_t i = (int64_t)blockIdx.x * (kThreads >> lane_bits) + (threadIdx.x >> lane_bits);
   if (i >= n)
     return;
@@ -106,28 +110,38 @@ __global__ void __launch_bounds__(kThreads)
   const bool inside = id >= 0 && id < rows;
   const I *src = table + (inside ? id : 0) * stride;
   O *dst = out + i * out_stride;
-#pragma unroll 4
-  for (int64_t c = lane; c < vecs; c += 1 << lane_bits) {
-    Pack<O, V> y;
-    if (inside) {
-      const Pack<I, V> x = load<I, V>(src + c * V);
+  for (int64_t c0 = lane; c0 < vecs; c0 += (int64_t)kTakeBatch * lanes) {
+    Pack<I, V> x[kTakeBatch];
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        y.v[e] = down<O, A>(up(x.v[e]) * scale);
-    } else {
+    for (int u = 0; u < kTakeBatch; ++u)
+      if (inside && c0 + u * lanes < vecs)
+        x[u] = load<I, V>(src + (c0 + u * lanes) * V);
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        y.v[e] = down<O, A>(A(0));
-    }
-    store<O, V>(dst + c * V, y);
+    for (int u = 0; u < kTakeBatch; ++u)
+      if (c0 + u * lanes < vecs) {
+        Pack<O, V> y;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          y.v[e] = down<O, A>(inside ? up(x[u].v[e]) * scale : A(0));
+        store<O, V>(dst + (c0 + u * lanes) * V, y);
+      }
   }
+}
+
+// Threads per row: enough for four accesses each where there are rows enough to
+// fill the multiprocessors that way, one access each otherwise.
+int takeLaneBits(int64_t n, int64_t vecs) {
+  const int wide = laneBits(vecs, kThreadBits);
+  const int narrow = laneBits((vecs + kTakeBatch - 1) / kTakeBatch, kThreadBits);
+  return n * (vecs / kTakeBatch) >= 148 * 2048 ? narrow : wide;
 }
 
 // -------------------------------------------------------------- take_grad ---
 // The entries arrive sorted by row (keys, order), so a row's entries are a run
 // of neighbours.  The sorted list is cut into chunks of `span` entries; a group
 // of `lanes` threads takes a chunk, a thread one access's width of columns, and
-// adds up the runs that begin in the chunk, eight incoming rows in flight.
+// adds up the runs that begin in the chunk, two incoming rows in flight
+// and four blocks a multiprocessor.
 // Every incoming row is read once, every row of the result written once.
 //
 // A run that goes on past its chunk is finished by the group it began in, up
@@ -135,7 +149,8 @@ __global__ void __launch_bounds__(kThreads)
 // add up their own entries, so a frequent token (padding, the end of a line)
 // does not keep one group busy: all of the run's groups leave partial sums in
 // the workspace, and the one that draws the last ticket adds them up in the
-// order of the chunks.  The order of additions is a function of the ids alone.
+// order of the chunks (of 32 chunks at a time, then of those).  The order of
+// additions is a function of the ids alone.
 //
 // Rows without entries are set to zero by blocks of their own, which look their
 // rows up in the sorted keys, one row a lane.
@@ -161,8 +176,20 @@ __device__ __forceinline__ void group_sync(int lane_bits, int group) {
     asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(1 << lane_bits) : "memory");
 }
 
-constexpr int kGradBatch = 8;   // incoming rows in flight per thread
+constexpr int kGradBatch = 2;   // incoming rows in flight per thread
 constexpr int kZeroRows = 32;   // rows looked up by a block that clears
+constexpr int kBundle = 32;     // partial sums added up by one group
+
+// A run's row: scale * sum, or that added to what the row holds.
+template <typename O, int V, bool ADD, typename A>
+__device__ __forceinline__ void write_sum(O *to, A scale, const A (&sum)[V], const Pack<O, V> &old, bool active) {
+  Pack<O, V> y;
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    y.v[e] = down<O, A>(ADD ? madd(scale, sum[e], up(old.v[e])) : scale * sum[e]);
+  if (active)
+    store<O, V>(to, y);
+}
 
 struct GradPlan {
   const int32_t *order;
@@ -170,38 +197,59 @@ struct GradPlan {
   int64_t n;
   int span;
   unsigned slabs;          // groups side by side over the columns
-  unsigned chunk_blocks;   // blocks over chunks (times slabs), the rest clears
+  unsigned chunk_blocks;   // blocks over chunks, times slabs
+  unsigned zero_blocks;    // blocks that clear
   void *partials;          // [chunks][cols]
-  uint32_t *tickets;       // [chunks][slabs], zero
+  uint32_t *tickets;       // [2][chunks][slabs], zero
+  int64_t chunks;
   int lane_bits;
-  int accumulate;
 };
 
-// The threads of a group walk over entries [j, end) of one or several runs;
-// `flush` gets each run's row and sum when the next begins.
-template <typename I, int V, typename A, typename F>
-__device__ __forceinline__ void walk_runs(const I *__restrict__ dout, int64_t stride, const GradPlan &p, int64_t j,
-                                          int64_t end, uint32_t &row, A (&sum)[V], F &&flush) {
+// A group walks over the entries [j, end) of one or several runs and writes a
+// run's row when the next begins; the row and the sum of the last stay behind.
+// The indices of the next batch are read along with the rows of this one, and
+// where the results are added to, the rows to be written with them.
+template <typename I, typename O, int V, bool ADD, typename A>
+__device__ __forceinline__ void walk_runs(const I *__restrict__ src, int64_t stride, const GradPlan &p, int64_t j,
+                                          int64_t end, A scale, O *dst, int64_t out_stride, bool active, uint32_t &row,
+                                          A (&sum)[V]) {
+  int32_t at[kGradBatch];
+  uint32_t key[kGradBatch];
+#pragma unroll
+  for (int u = 0; u < kGradBatch; ++u)
+    if (j + u < end) {
+      at[u] = __ldg(p.order + j + u);
+      key[u] = __ldg(p.keys + j + u);
+    }
   while (j < end) {
-    int32_t at[kGradBatch];
-    uint32_t key[kGradBatch];
     Pack<I, V> x[kGradBatch];
+    Pack<O, V> old[ADD ? kGradBatch : 1];
 #pragma unroll
     for (int u = 0; u < kGradBatch; ++u)
       if (j + u < end) {
-        at[u] = __ldg(p.order + j + u);
-        key[u] = __ldg(p.keys + j + u);
+        x[u] = load<I, V>(src + (int64_t)at[u] * stride);
+        if constexpr (ADD) {
+          const uint32_t before = u > 0 ? key[u > 0 ? u - 1 : 0] : row;
+          if (key[u] != before)
+            old[u] = load<O, V>(dst + (int64_t)before * out_stride);
+        }
       }
+    const int64_t next = j + kGradBatch;
+    uint32_t now[kGradBatch];
 #pragma unroll
-    for (int u = 0; u < kGradBatch; ++u)
-      if (j + u < end)
-        x[u] = load<I, V>(dout + (int64_t)at[u] * stride);
+    for (int u = 0; u < kGradBatch; ++u) {
+      now[u] = key[u];
+      if (next + u < end) {
+        at[u] = __ldg(p.order + next + u);
+        key[u] = __ldg(p.keys + next + u);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < kGradBatch; ++u)
       if (j + u < end) {
-        if (key[u] != row) {
-          flush(row, sum);
-          row = key[u];
+        if (now[u] != row) {
+          write_sum<O, V, ADD>(dst + (int64_t)row * out_stride, scale, sum, old[ADD ? u : 0], active);
+          row = now[u];
 #pragma unroll
           for (int e = 0; e < V; ++e)
             sum[e] = A(0);
@@ -210,21 +258,45 @@ __device__ __forceinline__ void walk_runs(const I *__restrict__ dout, int64_t st
         for (int e = 0; e < V; ++e)
           sum[e] += up(x[u].v[e]);
       }
-    j += kGradBatch;
+    j = next;
   }
 }
 
-template <typename I, typename O, int V>
-__global__ void __launch_bounds__(kThreads)
+// Sum of the partial sums of chunks first, first + step, ... up to last.
+template <int V, typename A>
+__device__ __forceinline__ void add_partials(const A *partials, int64_t width, int64_t first, int64_t count,
+                                             int64_t second, int64_t step, A (&sum)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    sum[e] = A(0);
+#pragma unroll 4
+  for (int64_t i = 0; i < count; ++i) {
+    const A *from = partials + (i == 0 ? first : second + (i - 1) * step) * width;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      sum[e] += __ldcg(from + e);
+  }
+}
+
+template <typename I, typename O, int V, bool ADD>
+__global__ void __launch_bounds__(kThreads, 4)
     nmb_take_rows_grad(const I *__restrict__ dout, int64_t stride, const GradPlan p, typename Acc<I>::type scale, O *out,
                        int64_t rows, int64_t out_stride, int64_t vecs) {
   using A = typename Acc<I>::type;
   __shared__ uint32_t shared_word[kThreads / 64 + 1];
   const int lanes = 1 << p.lane_bits, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> p.lane_bits;
   const int groups = kThreads >> p.lane_bits;
+  Pack<O, V> zero;
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    zero.v[e] = down<O, A>(A(0));
 
-  if (blockIdx.x >= p.chunk_blocks * p.slabs) { // rows without entries
-    const int64_t first = (int64_t)(blockIdx.x - p.chunk_blocks * p.slabs) * kZeroRows;
+  // blocks that clear are spread evenly among the others: theirs are writes
+  // alone, the others mostly wait for reads
+  const uint64_t all_chunks = (uint64_t)p.chunk_blocks * p.slabs, all = all_chunks + p.zero_blocks;
+  const uint64_t chunks_before = (uint64_t)blockIdx.x * all_chunks / all;
+  if (((uint64_t)blockIdx.x + 1) * all_chunks / all == chunks_before) { // rows without entries
+    const int64_t first = (int64_t)(blockIdx.x - chunks_before) * kZeroRows;
     if (threadIdx.x < 32) {
       const int64_t v = first + threadIdx.x;
       bool absent = v < rows;
@@ -238,10 +310,6 @@ __global__ void __launch_bounds__(kThreads)
     }
     __syncthreads();
     const uint32_t mask = shared_word[0];
-    Pack<O, V> zero;
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      zero.v[e] = down<O, A>(A(0));
     for (int r = group; r < kZeroRows; r += groups)
       if (mask >> r & 1)
         for (int64_t c = lane; c < vecs; c += lanes)
@@ -249,8 +317,8 @@ __global__ void __launch_bounds__(kThreads)
     return;
   }
 
-  const unsigned slab = blockIdx.x % p.slabs;
-  const int64_t chunk = (int64_t)(blockIdx.x / p.slabs) * groups + group;
+  const unsigned slab = (unsigned)(chunks_before % p.slabs);
+  const int64_t chunk = (int64_t)(chunks_before / p.slabs) * groups + group;
   const int64_t column = (int64_t)slab * lanes + lane; // of accesses; a group's spare lanes idle through the barriers
   const bool active = column < vecs;
   const int64_t begin = chunk * p.span;
@@ -263,21 +331,11 @@ __global__ void __launch_bounds__(kThreads)
     return;
   const I *src = dout + (active ? column : 0) * V;
   O *dst = out + (active ? column : 0) * V;
-  auto write = [&](uint32_t row, const A(&sum)[V]) {
-    if (!active)
-      return;
-    Pack<O, V> y;
-    if (p.accumulate) {
-      y = load<O, V>(dst + (int64_t)row * out_stride);
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        y.v[e] = down<O, A>(madd(scale, sum[e], up(y.v[e])));
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        y.v[e] = down<O, A>(scale * sum[e]);
-    }
-    store<O, V>(dst + (int64_t)row * out_stride, y);
+  auto write_last = [&](uint32_t row, const A(&sum)[V]) {
+    Pack<O, V> old = zero;
+    if (ADD)
+      old = load<O, V>(dst + (int64_t)row * out_stride);
+    write_sum<O, V, ADD>(dst + (int64_t)row * out_stride, scale, sum, old, active);
   };
 
   A sum[V];
@@ -289,7 +347,7 @@ __global__ void __launch_bounds__(kThreads)
   if (begin > 0 && prev_key == first_key && last_key == first_key && end - begin == p.span) {
     // inside a long run as a whole
     row = first_key;
-    walk_runs<I, V>(src, stride, p, begin, end, row, sum, [](uint32_t, const A(&)[V]) {});
+    walk_runs<I, O, V, ADD>(src, stride, p, begin, end, scale, dst, out_stride, active, row, sum);
     owner = lower_bound(p.keys, 0, begin, row) / p.span;
     const int64_t run_end = lower_bound(p.keys, end, p.n, row + 1);
     inner = (run_end - (owner + 1) * p.span) / p.span;
@@ -300,54 +358,59 @@ __global__ void __launch_bounds__(kThreads)
     if (j >= stop)
       return;
     row = __ldg(p.keys + j);
-    walk_runs<I, V>(src, stride, p, j, stop, row, sum, write);
+    walk_runs<I, O, V, ADD>(src, stride, p, j, stop, scale, dst, out_stride, active, row, sum);
     if (stop == end && end < p.n && __ldg(p.keys + end) == row) {
       const int64_t run_end = lower_bound(p.keys, end, p.n, row + 1);
       inner = (run_end - end) / p.span;
-      walk_runs<I, V>(src, stride, p, end + inner * p.span, run_end, row, sum, write);
+      walk_runs<I, O, V, ADD>(src, stride, p, end + inner * p.span, run_end, scale, dst, out_stride, active, row, sum);
     }
     if (inner == 0) {
-      write(row, sum);
+      write_last(row, sum);
       return;
     }
   }
 
-  // a long run: leave the partial sum, the last of its groups adds them up
+  // A long run: leave the partial sum.  The last group of a bundle of chunks
+  // adds its bundle's up, the last of those groups the bundles'.
   A *partials = static_cast<A *>(p.partials) + column * V;
   const int64_t width = vecs * V;
-  if (active) {
+  auto leave_and_draw = [&](int64_t slot, uint32_t *ticket) {
+    if (active) {
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-      __stcg(partials + chunk * width + e, sum[e]);
-  }
-  __threadfence();
-  group_sync(p.lane_bits, group);
-  uint32_t drawn = 0;
-  if (lane == 0)
-    drawn = atomicAdd(p.tickets + owner * p.slabs + slab, 1u);
-  if (p.lane_bits <= 5) {
-    const int base = (threadIdx.x & 31) & ~(lanes - 1);
-    const uint32_t mask = p.lane_bits == 5 ? kAll : ((1u << lanes) - 1) << base;
-    drawn = __shfl_sync(mask, drawn, base);
-  } else {
-    if (lane == 0)
-      shared_word[group] = drawn;
+      for (int e = 0; e < V; ++e)
+        __stcg(partials + slot * width + e, sum[e]);
+    }
+    __threadfence();
     group_sync(p.lane_bits, group);
-    drawn = shared_word[group];
-  }
-  if (drawn != (uint32_t)inner || !active)
+    uint32_t drawn = 0;
+    if (lane == 0)
+      drawn = atomicAdd(ticket + slab, 1u);
+    if (p.lane_bits <= 5) {
+      const int base = (threadIdx.x & 31) & ~(lanes - 1);
+      drawn = __shfl_sync(p.lane_bits == 5 ? kAll : ((1u << lanes) - 1) << base, drawn, base);
+    } else {
+      if (lane == 0)
+        shared_word[group] = drawn;
+      group_sync(p.lane_bits, group);
+      drawn = shared_word[group];
+    }
+    __threadfence();
+    return drawn;
+  };
+  const int64_t last = owner + inner, bundle = chunk / kBundle;
+  const int64_t first = max(owner, bundle * kBundle), count = min(last, bundle * kBundle + kBundle - 1) - first + 1;
+  const int64_t bundles = last / kBundle - owner / kBundle + 1;
+  if (leave_and_draw(chunk, p.tickets + first * p.slabs) != (uint32_t)(count - 1))
     return;
-  __threadfence();
-#pragma unroll
-  for (int e = 0; e < V; ++e)
-    sum[e] = A(0);
-#pragma unroll 8
-  for (int64_t c = owner; c <= owner + inner; ++c) {
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      sum[e] += __ldcg(partials + c * width + e);
+  add_partials<V>(active ? partials : partials - lane * V, width, first, count, first + 1, 1, sum);
+  if (bundles > 1) {
+    group_sync(p.lane_bits, group);
+    if (leave_and_draw(first, p.tickets + (p.chunks + owner) * p.slabs) != (uint32_t)(bundles - 1))
+      return;
+    add_partials<V>(active ? partials : partials - lane * V, width, owner, bundles, (owner / kBundle + 1) * kBundle,
+                    kBundle, sum);
   }
-  write(row, sum);
+  write_last(row, sum);
 }
 
 // Entries per chunk: 32, or fewer (down to 4) where that leaves less than four
@@ -420,57 +483,290 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// The same with the rows fetched by bulk copies: a block takes a token (or a
+// slab of its columns), brings the rows of all its choices into shared memory
+// at once and adds them up from there.  Copies in flight cost no registers: with
+// the rows in registers eight choices left room for one block a multiprocessor,
+// and batches of four reached 4.5 of the 6.5 TB/s that a copy reaches.
+constexpr int kBulkThreads = 128;
+constexpr int kBulkChoices = 32;        // most choices of a token
+constexpr int kBulkBytes = 32768;       // most bytes in flight per block
+constexpr int kBulkLeast = 1024;        // narrower rows are left to the kernels above
+
+// What the threads of a block share about a token's choices.
+template <typename A> struct BulkChoices {
+  uint64_t bar;
+  int32_t at[kBulkChoices]; // -1: left out
+  A weight[kBulkChoices];
+};
+
+// Waits for the block's copies.  A wait that runs out is reported in the queue's
+// status word; nothing is then written, and the block stays for its copies.
+__device__ __forceinline__ bool bulk_arrived(uint64_t *bar, uint32_t phase, uint32_t *status) {
+  if (nmb::mbar_wait(bar, phase))
+    return true;
+  if (status)
+    atomicExch(status, (uint32_t)nmb::kStatusWaitTimeout);
+  (void)nmb::mbar_wait(bar, phase);
+  return false;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kBulkThreads)
+    nmb_combine_rows_bulk(const T *__restrict__ ys, int64_t y_rows, int64_t stride, int k,
+                          const int32_t *__restrict__ place, const int32_t *__restrict__ kept,
+                          const void *__restrict__ weights, int weight_type, T *__restrict__ out, int64_t out_stride,
+                          int64_t vecs, int slab_vecs, uint32_t *status) {
+  using A = typename Acc<T>::type;
+  constexpr int V = 16 / (int)sizeof(T);
+  extern __shared__ __align__(128) unsigned char rows[]; // [k][slab_vecs] accesses
+  __shared__ BulkChoices<A> c;
+  const int64_t t = blockIdx.x, first = (int64_t)blockIdx.y * slab_vecs;
+  const int here = (int)min((int64_t)slab_vecs, vecs - first);
+  const int j = threadIdx.x;
+  int32_t at = -1;
+  if (j < k) {
+    at = __ldg(place + t * k + j);
+    at = at < min((int64_t)__ldg(kept), y_rows) ? at : -1;
+    c.at[j] = at;
+    c.weight[j] = weights ? scalar_at<A>(weights, weight_type, t * k + j) : A(1);
+  }
+  if (j == 0) {
+    nmb::mbar_init(&c.bar, (uint32_t)k);
+    nmb::mbar_init_fence();
+  }
+  __syncthreads();
+  if (j < k) {
+    if (at >= 0) {
+      nmb::mbar_expect_tx(&c.bar, (uint32_t)here * 16);
+      nmb::bulk_load(rows + (int64_t)j * slab_vecs * 16, ys + at * stride + first * V, (uint32_t)here * 16, &c.bar);
+    } else {
+      nmb::mbar_arrive(&c.bar);
+    }
+  }
+  if (!bulk_arrived(&c.bar, 0, status))
+    return;
+  for (int col = threadIdx.x; col < here; col += kBulkThreads) {
+    A sum[V] = {};
+#pragma unroll 4
+    for (int i = 0; i < k; ++i)
+      if (c.at[i] >= 0) {
+        const Pack<T, V> y = load<T, V>(reinterpret_cast<const T *>(rows) + ((int64_t)i * slab_vecs + col) * V);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          sum[e] = madd(c.weight[i], up(y.v[e]), sum[e]);
+      }
+    Pack<T, V> r;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      r.v[e] = down<T, A>(sum[e]);
+    store<T, V>(out + t * out_stride + (first + col) * V, r);
+  }
+}
+
+// Accesses of a slab where `rows` rows share a block's bytes; 0: not by bulk
+// copies (rows that are narrow or not aligned, too many choices).
+int bulkSlab(int64_t cols, int type, int v, int64_t choices, int rows) {
+  const int64_t bytes = cols * elemBytes(type);
+  if (v * elemBytes(type) != 16 || choices < 1 || choices > kBulkChoices || bytes < kBulkLeast)
+    return 0;
+  int64_t slab = kBulkBytes / rows / 16 / 32 * 32; // at least 32: 33 rows of 512 bytes
+  slab = slab < bytes / 16 ? slab : bytes / 16;
+  return (bytes / 16 + slab - 1) / slab <= 65535 ? (int)slab : 0;
+}
+
 // ----------------------------------------------------------- combine_grad ---
-// The threads of a token go over its choices one by one; the products of a
-// choice meet in a fixed tree (shuffles, then the warps in order).
+// The threads of a token read dout once for up to four choices, whose rows are
+// in flight together; each keeps its share of their dot products, which meet at
+// the end in a fixed tree: shuffles that halve the values along with the lanes,
+// then the token's warps in order.
+constexpr int kChoices = 4;
+constexpr int kChoiceBits = 2;
+
+template <typename A> struct Choices {
+  int32_t at[kChoices];
+  A weight[kChoices];
+  __device__ __forceinline__ void read(const int32_t *__restrict__ place, const void *__restrict__ weights,
+                                       int weight_type, int64_t entry, int64_t left) {
+#pragma unroll
+    for (int j = 0; j < kChoices; ++j) {
+      at[j] = j < left ? __ldg(place + entry + j) : -1;
+      weight[j] = weights && j < left ? scalar_at<A>(weights, weight_type, entry + j) : A(1);
+    }
+  }
+};
+
+// Adds the values up over the lanes of a token (up to a warp).  The first
+// kChoiceBits steps also halve the values a lane is left with: lane bit b picks
+// bit kChoiceBits - 1 - b of the value.
+template <typename A> __device__ __forceinline__ void meet(A (&v)[kChoices], int lanes) {
+  const int lane = threadIdx.x & 31;
+  int held = kChoices;
+#pragma unroll
+  for (int step = 1; step <= 16; step <<= 1) {
+    if (step >= lanes)
+      break;
+    if (held > 1) {
+      held /= 2;
+      const bool high = lane & step;
+#pragma unroll
+      for (int i = 0; i < kChoices / 2; ++i)
+        if (i < held) {
+          const A give = high ? v[i] : v[i + held], keep = high ? v[i + held] : v[i];
+          v[i] = keep + __shfl_xor_sync(kAll, give, step);
+        }
+    } else {
+      v[0] += __shfl_xor_sync(kAll, v[0], step);
+    }
+  }
+}
+
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
     nmb_combine_rows_grad(const T *__restrict__ dout, int64_t tokens, int64_t stride, const T *__restrict__ ys,
                           int64_t y_rows, int64_t y_stride, int64_t k, const int32_t *__restrict__ place,
-                          const int32_t *__restrict__ kept, const void *weights, int weight_type, T *__restrict__ dys,
-                          int64_t dy_rows, int64_t dy_stride, void *dweights, int64_t vecs, int lane_bits) {
+                          const int32_t *__restrict__ kept, const void *__restrict__ weights, int weight_type,
+                          T *__restrict__ dys, int64_t dy_rows, int64_t dy_stride, void *dweights, int64_t vecs,
+                          int lane_bits) {
   using A = typename Acc<T>::type;
-  __shared__ A parts[kThreads / 32];
+  __shared__ A parts[kThreads / 32][kChoices];
   const int lanes = 1 << lane_bits;
   const int lane = threadIdx.x & (lanes - 1);
   const int64_t t = (int64_t)blockIdx.x * (kThreads >> lane_bits) + (threadIdx.x >> lane_bits);
-  const bool token = t < tokens; // every thread stays for the barriers
-  const int64_t live = min((int64_t)*kept, y_rows);
-  for (int64_t j = 0; j < k; ++j) {
-    const int64_t at = token ? place[t * k + j] : -1;
-    const bool inside = at >= 0 && at < live;
-    const A w = inside ? (weights ? scalar_at<A>(weights, weight_type, t * k + j) : A(1)) : A(0);
-    A dot = A(0);
-    if (at >= 0 && at < dy_rows) {
-      for (int64_t c = lane; c < vecs; c += lanes) {
+  const bool token = t < tokens; // every thread stays for the shuffles and barriers
+  const int64_t live = min((int64_t)__ldg(kept), y_rows);
+  Choices<A> c;
+  for (int64_t j0 = 0; j0 < k; j0 += kChoices) {
+    c.read(place, weights, weight_type, t * k + j0, token ? k - j0 : 0);
+    A dot[kChoices] = {};
+    for (int64_t col = token ? lane : vecs; col < vecs; col += lanes) {
+      const Pack<T, V> d = load<T, V>(dout + t * stride + col * V);
+      Pack<T, V> y[kChoices];
+#pragma unroll
+      for (int j = 0; j < kChoices; ++j)
+        if (c.at[j] >= 0 && c.at[j] < live)
+          y[j] = load<T, V>(ys + c.at[j] * y_stride + col * V);
+#pragma unroll
+      for (int j = 0; j < kChoices; ++j)
+        if (c.at[j] >= 0 && c.at[j] < dy_rows) {
+          Pack<T, V> r{};
+          if (c.at[j] < live) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              dot[j] = madd(up(d.v[e]), up(y[j].v[e]), dot[j]);
+              r.v[e] = down<T, A>(c.weight[j] * up(d.v[e]));
+            }
+          }
+          store<T, V>(dys + c.at[j] * dy_stride + col * V, r);
+        }
+    }
+    meet(dot, lanes);
+    const int halvings = lane_bits < kChoiceBits ? lane_bits : kChoiceBits;
+    int mine = 0; // the first of the values that this lane ends up with
+    for (int b = 0; b < halvings; ++b)
+      mine |= (lane >> b & 1) << (kChoiceBits - 1 - b);
+    const int held = kChoices >> halvings;
+    if (lanes > 32) {
+      const int warp = threadIdx.x >> 5;
+      if ((threadIdx.x & 31) < kChoices)
+        parts[warp][mine] = dot[0];
+      __syncthreads();
+      if (lane < kChoices) {
+        A sum = A(0);
+        for (int w = 0; w < lanes / 32; ++w)
+          sum += parts[warp + w][lane];
+        if (token && j0 + lane < k && dweights)
+          set_scalar<A>(dweights, weight_type, t * k + j0 + lane, sum);
+      }
+      __syncthreads();
+    } else if (token && lane < (1 << halvings) && dweights) {
+#pragma unroll
+      for (int i = 0; i < kChoices; ++i)
+        if (i < held && j0 + mine + i < k)
+          set_scalar<A>(dweights, weight_type, t * k + j0 + mine + i, dot[i]);
+    }
+  }
+}
+
+// The same with the rows fetched by bulk copies, dout's first.  A block takes a
+// whole token; columns beyond a slab come in turns through the same memory.
+template <typename T>
+__global__ void __launch_bounds__(kBulkThreads)
+    nmb_combine_rows_grad_bulk(const T *__restrict__ dout, int64_t stride, const T *__restrict__ ys, int64_t y_rows,
+                               int64_t y_stride, int k, const int32_t *__restrict__ place,
+                               const int32_t *__restrict__ kept, const void *__restrict__ weights, int weight_type,
+                               T *__restrict__ dys, int64_t dy_rows, int64_t dy_stride, void *dweights, int64_t vecs,
+                               int slab_vecs, uint32_t *status) {
+  using A = typename Acc<T>::type;
+  constexpr int V = 16 / (int)sizeof(T), kWarps = kBulkThreads / 32;
+  extern __shared__ __align__(128) unsigned char rows[]; // [1 + k][slab_vecs] accesses
+  __shared__ BulkChoices<A> c;
+  __shared__ A parts[kWarps][kBulkChoices];
+  const int64_t t = blockIdx.x;
+  const int j = threadIdx.x, lane = j & 31, warp = j >> 5;
+  const int64_t live = min((int64_t)__ldg(kept), y_rows);
+  int32_t at = -1;
+  if (j < k) {
+    at = __ldg(place + t * k + j);
+    c.at[j] = at < dy_rows ? at : -1;
+    c.weight[j] = weights ? scalar_at<A>(weights, weight_type, t * k + j) : A(1);
+  }
+  if (j == 0) {
+    nmb::mbar_init(&c.bar, (uint32_t)k + 1);
+    nmb::mbar_init_fence();
+  }
+  for (int i = j; i < kWarps * kBulkChoices; i += kBulkThreads)
+    (&parts[0][0])[i] = A(0);
+  __syncthreads();
+  uint32_t phase = 0;
+  for (int64_t first = 0; first < vecs; first += slab_vecs, phase ^= 1) {
+    const int here = (int)min((int64_t)slab_vecs, vecs - first);
+    if (j <= k) { // thread k fetches dout
+      const int64_t row = j < k ? at : t;
+      if (j == k || (at >= 0 && at < live)) {
+        nmb::mbar_expect_tx(&c.bar, (uint32_t)here * 16);
+        nmb::bulk_load(rows + (int64_t)(j < k ? j + 1 : 0) * slab_vecs * 16,
+                       (j < k ? ys + row * y_stride : dout + row * stride) + first * V, (uint32_t)here * 16, &c.bar);
+      } else {
+        nmb::mbar_arrive(&c.bar);
+      }
+    }
+    if (!bulk_arrived(&c.bar, phase, status))
+      return; // every thread gives up by itself: no barrier is left waiting
+    const T *mem = reinterpret_cast<const T *>(rows);
+    for (int i = 0; i < k; ++i) {
+      const int32_t to = c.at[i];
+      if (to < 0)
+        continue;
+      A dot = A(0);
+      for (int col = j; col < here; col += kBulkThreads) {
         Pack<T, V> r{};
-        if (inside) {
-          const Pack<T, V> d = load<T, V>(dout + t * stride + c * V);
-          const Pack<T, V> y = load<T, V>(ys + at * y_stride + c * V);
+        if (to < live) {
+          const Pack<T, V> d = load<T, V>(mem + (int64_t)col * V);
+          const Pack<T, V> y = load<T, V>(mem + ((int64_t)(i + 1) * slab_vecs + col) * V);
+          const A w = c.weight[i];
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             dot = madd(up(d.v[e]), up(y.v[e]), dot);
             r.v[e] = down<T, A>(w * up(d.v[e]));
           }
         }
-        store<T, V>(dys + at * dy_stride + c * V, r);
+        store<T, V>(dys + to * dy_stride + (first + col) * V, r);
       }
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1)
+        dot += __shfl_xor_sync(kAll, dot, s);
+      if (lane == 0)
+        parts[warp][i] += dot;
     }
-    for (int s = min(lanes, 32) / 2; s > 0; s >>= 1)
-      dot += __shfl_xor_sync(kAll, dot, s);
-    if (lanes > 32) {
-      if ((threadIdx.x & 31) == 0)
-        parts[threadIdx.x >> 5] = dot;
-      __syncthreads();
-      if (lane == 0) {
-        dot = A(0);
-        for (int i = 0; i < lanes / 32; ++i)
-          dot += parts[(threadIdx.x >> 5) + i];
-      }
-      __syncthreads();
-    }
-    if (token && lane == 0 && dweights)
-      set_scalar<A>(dweights, weight_type, t * k + j, dot);
+    __syncthreads(); // the slab's memory is free again, the sums are in place
+  }
+  if (j < k && dweights) {
+    A sum = A(0);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      sum += parts[w][j];
+    set_scalar<A>(dweights, weight_type, t * k + j, sum);
   }
 }
 
@@ -597,7 +893,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_device(void *queue, const GPUXRows *t
     constexpr int most = mostElems<I>() > mostElems<O>() ? mostElems<I>() : mostElems<O>();
     const int v = accessElems(out->cols, most, {table, out});
     const int64_t vecs = out->cols / v;
-    const int bits = laneBits(vecs, kThreadBits);
+    const int bits = takeLaneBits(out->rows, vecs);
     withElems<most>(v, [&](auto V) {
       nmb_take_rows<I, O, V.value><<<blocksFor(out->rows, bits), kThreads, 0, s.stream>>>(
           static_cast<const I *>(table->data), table->rows, table->stride, ids->data, ids->bytes, ids->count,
@@ -617,7 +913,7 @@ struct GradMemory {
     const int span = gradSpan(n, (cols + 7) / 8);
     const int64_t chunks = (n + span - 1) / span;
     entries = padded((size_t)n * 4);
-    tickets = padded((size_t)chunks * (size_t)((cols + kThreads - 1) / kThreads) * 4);
+    tickets = padded((size_t)chunks * 2 * (size_t)((cols + kThreads - 1) / kThreads) * 4);
     partials = padded((size_t)chunks * (size_t)cols * (type == GPUX_ELEM_F64 ? 8 : 4));
     sort = nmb::rows::sortBytes(n, rows);
   }
@@ -667,8 +963,8 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
     const int64_t chunks = (ids->count + span - 1) / span;
     const unsigned slabs = (unsigned)((vecs + (int64_t(1) << bits) - 1) >> bits);
     const unsigned zeros = accumulate ? 0 : (unsigned)((out->rows + kZeroRows - 1) / kZeroRows);
-    const GradPlan plan{order, keys,    ids->count, span, slabs, blocksFor(chunks, bits), partials,
-                        tickets, bits, accumulate};
+    const GradPlan plan{order, keys,     ids->count, span,   slabs, blocksFor(chunks, bits),
+                        zeros, partials, tickets,    chunks, bits};
     const int64_t blocks = (int64_t)plan.chunk_blocks * slabs + zeros;
     if (blocks >= (int64_t(1) << 31)) {
       nmb::setError("%s: too many indices for their width", who);
@@ -676,13 +972,15 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
       return;
     }
     ok = nmb::rows::sortByKey(s, who, *ids, out->rows, order, keys, nullptr, nullptr,
-                              ws + 2 * need.entries + need.tickets + need.partials, tickets, chunks * slabs);
+                              ws + 2 * need.entries + need.tickets + need.partials, tickets, 2 * chunks * slabs);
     if (!ok)
       return;
     withElems<most>(v, [&](auto V) {
-      nmb_take_rows_grad<I, O, V.value><<<(unsigned)blocks, kThreads, 0, s.stream>>>(
-          static_cast<const I *>(dout->data), dout->stride, plan, (typename Acc<I>::type)scale,
-          static_cast<O *>(out->data), out->rows, out->stride, vecs);
+      const auto kernel =
+          accumulate ? nmb_take_rows_grad<I, O, V.value, true> : nmb_take_rows_grad<I, O, V.value, false>;
+      kernel<<<(unsigned)blocks, kThreads, 0, s.stream>>>(static_cast<const I *>(dout->data), dout->stride, plan,
+                                                          (typename Acc<I>::type)scale, static_cast<O *>(out->data),
+                                                          out->rows, out->stride, vecs);
     });
   });
   return ok && launched(who) ? 0 : 1;
@@ -732,11 +1030,19 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows
   Stream s(queue);
   if (!s.ok)
     return 1;
+  uint32_t *status = nmb::statusWordOrNull(queue);
   withType(ys->type, [&](auto e) {
     using T = decltype(e);
     const int v = accessElems(out->cols, mostElems<T>(), {ys, out});
     const int64_t vecs = out->cols / v;
     const int bits = laneBits(vecs, kThreadBits);
+    if (const int slab = bulkSlab(out->cols, out->type, v, k, (int)k)) {
+      nmb_combine_rows_bulk<T><<<dim3((unsigned)out->rows, (unsigned)((vecs + slab - 1) / slab)), kBulkThreads,
+                                 (size_t)k * slab * 16, s.stream>>>(
+          static_cast<const T *>(ys->data), ys->rows, ys->stride, (int)k, place, kept, weights, weightType,
+          static_cast<T *>(out->data), out->stride, vecs, slab, status);
+      return;
+    }
     withElems<mostElems<T>()>(v, [&](auto V) {
       nmb_combine_rows<T, V.value><<<blocksFor(out->rows, bits), kThreads, 0, s.stream>>>(
           static_cast<const T *>(ys->data), ys->rows, ys->stride, k, place, kept, weights, weightType,
@@ -762,11 +1068,19 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_grad_device(void *queue, const GPU
   Stream s(queue);
   if (!s.ok)
     return 1;
+  uint32_t *status = nmb::statusWordOrNull(queue);
   withType(ys->type, [&](auto e) {
     using T = decltype(e);
     const int v = dout->cols ? accessElems(dout->cols, mostElems<T>(), {dout, ys, dys}) : 1;
     const int64_t vecs = dout->cols / v;
     const int bits = laneBits(vecs, kThreadBits);
+    if (const int slab = bulkSlab(dout->cols, dout->type, v, k, (int)k + 1)) {
+      nmb_combine_rows_grad_bulk<T><<<(unsigned)dout->rows, kBulkThreads, (size_t)(k + 1) * slab * 16, s.stream>>>(
+          static_cast<const T *>(dout->data), dout->stride, static_cast<const T *>(ys->data), ys->rows, ys->stride,
+          (int)k, place, kept, weights, weightType, static_cast<T *>(dys->data), dys->rows, dys->stride, dweights,
+          vecs, slab, status);
+      return;
+    }
     withElems<mostElems<T>()>(v, [&](auto V) {
       nmb_combine_rows_grad<T, V.value><<<blocksFor(dout->rows, bits), kThreads, 0, s.stream>>>(
           static_cast<const T *>(dout->data), dout->rows, dout->stride, static_cast<const T *>(ys->data), ys->rows,

@@ -659,6 +659,20 @@ uint32_t *statusWord(void *queue) {
   return q->status;
 }
 
+// For launches that may be the queue's first and recorded into a graph: memory
+// allocated while recording belongs to the graph, so the word is not made then.
+uint32_t *statusWordOrNull(void *queue) {
+  Queue *q = toQueue(queue);
+  if (!q->status) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(q->stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+      (void)cudaGetLastError();
+      return nullptr;
+    }
+  }
+  return statusWord(queue);
+}
+
 } // namespace nmb
 
 // ---------------------------------------------------------------- exports ---
