@@ -55,6 +55,47 @@ template <> __device__ __forceinline__ __nv_bfloat16 down<__nv_bfloat16, float>(
 __device__ __forceinline__ float madd(float a, float b, float c) { return __fmaf_rn(a, b, c); }
 __device__ __forceinline__ double madd(double a, double b, double c) { return __fma_rn(a, b, c); }
 
+// Two neighbouring elements at a time: one instruction multiplies (and adds) a
+// pair of float32, one rounds it to 16 bits.
+__device__ __forceinline__ float2 up2(const float *p) { return make_float2(p[0], p[1]); }
+__device__ __forceinline__ double2 up2(const double *p) { return make_double2(p[0], p[1]); }
+__device__ __forceinline__ float2 up2(const __half *p) { return __half22float2(*reinterpret_cast<const __half2 *>(p)); }
+__device__ __forceinline__ float2 up2(const __nv_bfloat16 *p) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(p));
+}
+__device__ __forceinline__ void down2(float *p, float2 v) { p[0] = v.x, p[1] = v.y; }
+__device__ __forceinline__ void down2(double *p, double2 v) { p[0] = v.x, p[1] = v.y; }
+__device__ __forceinline__ void down2(__half *p, float2 v) {
+  *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(v.x, v.y);
+}
+__device__ __forceinline__ void down2(__nv_bfloat16 *p, float2 v) {
+  *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(v.x, v.y);
+}
+__device__ __forceinline__ uint64_t bits2(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 pair2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ float2 madd2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return pair2(r);
+}
+__device__ __forceinline__ double2 madd2(double2 a, double2 b, double2 c) {
+  return make_double2(madd(a.x, b.x, c.x), madd(a.y, b.y, c.y));
+}
+__device__ __forceinline__ float2 mul2(float a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(make_float2(a, a))), "l"(bits2(b)));
+  return pair2(r);
+}
+__device__ __forceinline__ double2 mul2(double a, double2 b) { return make_double2(a * b.x, a * b.y); }
+
 // V neighbouring elements, moved with 16-byte accesses where they fill one.
 template <typename T, int V> struct alignas(sizeof(T) * V <= 16 ? sizeof(T) * V : 16) Pack {
   T v[V];
@@ -596,12 +637,12 @@ template <typename A> struct Choices {
   }
 };
 
-// Adds the values up over the lanes of a token (up to a warp).  The first
-// kChoiceBits steps also halve the values a lane is left with: lane bit b picks
-// bit kChoiceBits - 1 - b of the value.
-template <typename A> __device__ __forceinline__ void meet(A (&v)[kChoices], int lanes) {
+// Adds N values up over the lanes of a token (up to a warp).  The first log2(N)
+// steps also halve the values a lane is left with: lane bit b picks bit
+// log2(N) - 1 - b of the value.
+template <int N, typename A> __device__ __forceinline__ void meet(A (&v)[N], int lanes) {
   const int lane = threadIdx.x & 31;
-  int held = kChoices;
+  int held = N;
 #pragma unroll
   for (int step = 1; step <= 16; step <<= 1) {
     if (step >= lanes)
@@ -610,7 +651,7 @@ template <typename A> __device__ __forceinline__ void meet(A (&v)[kChoices], int
       held /= 2;
       const bool high = lane & step;
 #pragma unroll
-      for (int i = 0; i < kChoices / 2; ++i)
+      for (int i = 0; i < N / 2; ++i)
         if (i < held) {
           const A give = high ? v[i] : v[i + held], keep = high ? v[i + held] : v[i];
           v[i] = keep + __shfl_xor_sync(kAll, give, step);
@@ -688,6 +729,9 @@ __global__ void __launch_bounds__(kThreads, 4)
   }
 }
 
+template <typename A> struct Two { using type = float2; };
+template <> struct Two<double> { using type = double2; };
+
 // The same with the rows fetched by bulk copies, dout's first.  A block takes a
 // whole token; columns beyond a slab come in turns through the same memory.
 template <typename T>
@@ -698,7 +742,7 @@ __global__ void __launch_bounds__(kBulkThreads)
                                T *__restrict__ dys, int64_t dy_rows, int64_t dy_stride, void *dweights, int64_t vecs,
                                int slab_vecs, uint32_t *status) {
   using A = typename Acc<T>::type;
-  constexpr int V = 16 / (int)sizeof(T), kWarps = kBulkThreads / 32;
+  constexpr int V = 16 / (int)sizeof(T), kWarps = kBulkThreads / 32, kGradChoices = 8;
   extern __shared__ __align__(128) unsigned char rows[]; // [1 + k][slab_vecs] accesses
   __shared__ BulkChoices<A> c;
   __shared__ A parts[kWarps][kBulkChoices];
@@ -734,30 +778,44 @@ __global__ void __launch_bounds__(kBulkThreads)
     if (!bulk_arrived(&c.bar, phase, status))
       return; // every thread gives up by itself: no barrier is left waiting
     const T *mem = reinterpret_cast<const T *>(rows);
-    for (int i = 0; i < k; ++i) {
-      const int32_t to = c.at[i];
-      if (to < 0)
-        continue;
-      A dot = A(0);
-      for (int col = j; col < here; col += kBulkThreads) {
-        Pack<T, V> r{};
-        if (to < live) {
-          const Pack<T, V> d = load<T, V>(mem + (int64_t)col * V);
-          const Pack<T, V> y = load<T, V>(mem + ((int64_t)(i + 1) * slab_vecs + col) * V);
-          const A w = c.weight[i];
+    for (int j0 = 0; j0 < k; j0 += kGradChoices) {
+      int32_t to[kGradChoices];
+      A w[kGradChoices];
+      typename Two<A>::type dots[kGradChoices] = {};
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            dot = madd(up(d.v[e]), up(y.v[e]), dot);
-            r.v[e] = down<T, A>(w * up(d.v[e]));
-          }
-        }
-        store<T, V>(dys + to * dy_stride + (first + col) * V, r);
+      for (int i = 0; i < kGradChoices; ++i) {
+        to[i] = j0 + i < k ? c.at[j0 + i] : -1;
+        w[i] = j0 + i < k ? c.weight[j0 + i] : A(0);
       }
+      for (int col = j; col < here; col += kBulkThreads) {
+        const Pack<T, V> x = load<T, V>(mem + (int64_t)col * V);
+        typename Two<A>::type d[V / 2];
 #pragma unroll
-      for (int s = 16; s > 0; s >>= 1)
-        dot += __shfl_xor_sync(kAll, dot, s);
-      if (lane == 0)
-        parts[warp][i] += dot;
+        for (int e = 0; e < V / 2; ++e)
+          d[e] = up2(x.v + 2 * e);
+#pragma unroll
+        for (int i = 0; i < kGradChoices; ++i)
+          if (to[i] >= 0) {
+            Pack<T, V> r{};
+            if (to[i] < live) {
+              const Pack<T, V> y = load<T, V>(mem + ((int64_t)(j0 + i + 1) * slab_vecs + col) * V);
+#pragma unroll
+              for (int e = 0; e < V / 2; ++e) {
+                dots[i] = madd2(d[e], up2(y.v + 2 * e), dots[i]);
+                down2(r.v + 2 * e, mul2(w[i], d[e]));
+              }
+            }
+            store<T, V>(dys + to[i] * dy_stride + (first + col) * V, r);
+          }
+      }
+      A dot[kGradChoices];
+#pragma unroll
+      for (int i = 0; i < kGradChoices; ++i)
+        dot[i] = dots[i].x + dots[i].y;
+      meet(dot, 32);
+      const int mine = (lane & 1) << 2 | (lane & 2) | (lane & 4) >> 2;
+      if (lane < kGradChoices && j0 + mine < k)
+        parts[warp][j0 + mine] += dot[0];
     }
     __syncthreads(); // the slab's memory is free again, the sums are in place
   }
