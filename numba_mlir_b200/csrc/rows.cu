@@ -531,7 +531,10 @@ __global__ void __launch_bounds__(kThreads)
 // and batches of four reached 4.5 of the 6.5 TB/s that a copy reaches.
 constexpr int kBulkThreads = 128;
 constexpr int kBulkChoices = 32;        // most choices of a token
-constexpr int kBulkBytes = 32768;       // most bytes in flight per block
+// Most bytes in flight per block.  combine: 16384 tokens with eight rows of 4 KB
+// took 94.5 us at 16 KB (two slabs a token), 98.1 us at 32 KB.  combine_grad: a
+// token with eight such rows 175.7 us in one turn of 36 KB, 203 us in two.
+constexpr int kBulkBytes = 16384, kBulkGradBytes = 46080;
 constexpr int kBulkLeast = 1024;        // narrower rows are left to the kernels above
 
 // What the threads of a block share about a token's choices.
@@ -605,15 +608,15 @@ __global__ void __launch_bounds__(kBulkThreads)
   }
 }
 
-// Accesses of a slab where `rows` rows share a block's bytes; 0: not by bulk
-// copies (rows that are narrow or not aligned, too many choices).
-int bulkSlab(int64_t cols, int type, int v, int64_t choices, int rows) {
-  const int64_t bytes = cols * elemBytes(type);
+// Accesses of a slab where `rows` rows share `most` bytes: equal shares of the
+// row in as few slabs as that allows.  0: not by bulk copies (rows that are
+// narrow or not aligned, too many choices).
+int bulkSlab(int64_t cols, int type, int v, int64_t choices, int rows, int most) {
+  const int64_t bytes = cols * elemBytes(type), vecs = bytes / 16;
   if (v * elemBytes(type) != 16 || choices < 1 || choices > kBulkChoices || bytes < kBulkLeast)
     return 0;
-  int64_t slab = kBulkBytes / rows / 16 / 32 * 32; // at least 32: 33 rows of 512 bytes
-  slab = slab < bytes / 16 ? slab : bytes / 16;
-  return (bytes / 16 + slab - 1) / slab <= 65535 ? (int)slab : 0;
+  const int64_t slabs = (vecs * rows * 16 + most - 1) / most;
+  return slabs <= 65535 ? (int)((vecs + slabs - 1) / slabs) : 0;
 }
 
 // ----------------------------------------------------------- combine_grad ---
@@ -1094,7 +1097,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows
     const int v = accessElems(out->cols, mostElems<T>(), {ys, out});
     const int64_t vecs = out->cols / v;
     const int bits = laneBits(vecs, kThreadBits);
-    if (const int slab = bulkSlab(out->cols, out->type, v, k, (int)k)) {
+    if (const int slab = bulkSlab(out->cols, out->type, v, k, (int)k, kBulkBytes)) {
       nmb_combine_rows_bulk<T><<<dim3((unsigned)out->rows, (unsigned)((vecs + slab - 1) / slab)), kBulkThreads,
                                  (size_t)k * slab * 16, s.stream>>>(
           static_cast<const T *>(ys->data), ys->rows, ys->stride, (int)k, place, kept, weights, weightType,
@@ -1132,7 +1135,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_grad_device(void *queue, const GPU
     const int v = dout->cols ? accessElems(dout->cols, mostElems<T>(), {dout, ys, dys}) : 1;
     const int64_t vecs = dout->cols / v;
     const int bits = laneBits(vecs, kThreadBits);
-    if (const int slab = bulkSlab(dout->cols, dout->type, v, k, (int)k + 1)) {
+    if (const int slab = bulkSlab(dout->cols, dout->type, v, k, (int)k + 1, kBulkGradBytes)) {
       nmb_combine_rows_grad_bulk<T><<<(unsigned)dout->rows, kBulkThreads, (size_t)(k + 1) * slab * 16, s.stream>>>(
           static_cast<const T *>(dout->data), dout->stride, static_cast<const T *>(ys->data), ys->rows, ys->stride,
           (int)k, place, kept, weights, weightType, static_cast<T *>(dys->data), dys->rows, dys->stride, dweights,

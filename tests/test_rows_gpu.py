@@ -314,7 +314,7 @@ def test_dispatch_rows(queue, name, tokens, k, groups, dim, pad):
 
 # ---------------------------------------------------------------- combine ---
 @pytest.mark.parametrize("name", TYPES)
-@pytest.mark.parametrize("tokens,k,groups,dim,pad", ROUTES)
+@pytest.mark.parametrize("tokens,k,groups,dim,pad", ROUTES + [(6, 32, 40, 1024, 0), (3, 33, 40, 1024, 0), (9, 5, 7, 8192, 8)])
 def test_combine_rows(queue, name, tokens, k, groups, dim, pad):
     import numba_mlir_b200 as nm
 
@@ -339,7 +339,7 @@ def test_combine_rows(queue, name, tokens, k, groups, dim, pad):
 
 
 @pytest.mark.parametrize("name", TYPES)
-@pytest.mark.parametrize("tokens,k,groups,dim,pad", ROUTES + [(5, 40, 50, 96, 0)])
+@pytest.mark.parametrize("tokens,k,groups,dim,pad", ROUTES + [(5, 40, 50, 96, 0), (6, 32, 40, 1024, 0), (3, 33, 40, 1024, 0), (9, 5, 7, 8192, 8)])
 def test_combine_rows_grad(queue, name, tokens, k, groups, dim, pad):
     import numba_mlir_b200 as nm
 
