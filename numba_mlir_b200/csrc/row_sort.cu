@@ -424,21 +424,6 @@ template <typename F> bool withPer(int per, F &&f) {
   return f(std::integral_constant<int, 8>());
 }
 
-// Lets a kernel use more than 48 KB of shared memory; once per kernel and device.
-template <typename K> bool allowShared(const char *who, K kernel, int bytes, std::atomic<bool> *ready, int device) {
-  if (device >= 0 && device < 64 && ready[device])
-    return true;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) {
-    nmb::setError("%s: cudaFuncSetAttribute failed: %s", who, cudaGetErrorString(e));
-    (void)cudaGetLastError();
-    return false;
-  }
-  if (device >= 0 && device < 64)
-    ready[device] = true;
-  return true;
-}
-
 } // namespace
 
 namespace nmb {
@@ -476,7 +461,7 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
     const bool ok = withPer(per, [&](auto P) {
       constexpr int kPer = P.value < 4 ? P.value : 4;
       static std::atomic<bool> ready[64];
-      if (!allowShared(who, nmb_sort_one<kPer>, oneBytes<kPer>(), ready, s.device))
+      if (!nmb::rows::allowShared(who, nmb_sort_one<kPer>, oneBytes<kPer>(), ready, s.device))
         return false;
       // as many warps as the entries fill
       const int warps = (int)((n + 32 * kPer - 1) / (32 * kPer));
@@ -504,7 +489,7 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
       p.shift = pass * digitBits;
       const bool ok = withPer(perThread(n), [&](auto P) {
         static std::atomic<bool> ready[64];
-        if (!allowShared(who, nmb_sort_scatter<P.value>, kScatterBytes, ready, s.device))
+        if (!nmb::rows::allowShared(who, nmb_sort_scatter<P.value>, kScatterBytes, ready, s.device))
           return false;
         nmb_sort_count<P.value><<<(unsigned)blocks, kThreads, 0, s.stream>>>(p, Clear{clear, pass == 0 ? clearWords : 0});
         if (!launched(who))

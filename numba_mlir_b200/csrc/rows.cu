@@ -95,6 +95,14 @@ __device__ __forceinline__ float2 mul2(float a, float2 b) {
   return pair2(r);
 }
 __device__ __forceinline__ double2 mul2(double a, double2 b) { return make_double2(a * b.x, a * b.y); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+  return pair2(r);
+}
+__device__ __forceinline__ double2 add2(double2 a, double2 b) { return make_double2(a.x + b.x, a.y + b.y); }
+template <typename A> struct Two { using type = float2; };
+template <> struct Two<double> { using type = double2; };
 
 // V neighbouring elements, moved with 16-byte accesses where they fill one.
 template <typename T, int V> struct alignas(sizeof(T) * V <= 16 ? sizeof(T) * V : 16) Pack {
@@ -105,6 +113,22 @@ template <typename T, int V> __device__ __forceinline__ Pack<T, V> load(const T 
 }
 template <typename T, int V> __device__ __forceinline__ void store(T *p, const Pack<T, V> &x) {
   *reinterpret_cast<Pack<T, V> *>(p) = x;
+}
+
+// The same past L1, for what other blocks of the launch have written.
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_l2(const T *p) {
+  Pack<T, V> x;
+  constexpr int bytes = (int)sizeof(T) * V;
+  if constexpr (bytes >= 16) {
+#pragma unroll
+    for (int i = 0; i < bytes / 16; ++i)
+      reinterpret_cast<int4 *>(&x)[i] = __ldcg(reinterpret_cast<const int4 *>(p) + i);
+  } else if constexpr (bytes == 8) {
+    *reinterpret_cast<int2 *>(&x) = __ldcg(reinterpret_cast<const int2 *>(p));
+  } else {
+    *reinterpret_cast<int *>(&x) = __ldcg(reinterpret_cast<const int *>(p));
+  }
+  return x;
 }
 
 // A signed index of 4 or 8 bytes.
@@ -131,6 +155,20 @@ template <typename A> __device__ __forceinline__ void set_scalar(void *p, int ty
     static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn((float)v);
   else
     static_cast<double *>(p)[i] = (double)v;
+}
+
+// Rows narrower than this are not fetched by bulk copies.
+constexpr int kBulkLeast = 1024;
+
+// Waits for the block's copies.  A wait that runs out is reported in the queue's
+// status word; nothing is then written, and the block stays for its copies.
+__device__ __forceinline__ bool bulk_arrived(uint64_t *bar, uint32_t phase, uint32_t *status) {
+  if (nmb::mbar_wait(bar, phase))
+    return true;
+  if (status)
+    atomicExch(status, (uint32_t)nmb::kStatusWaitTimeout);
+  (void)nmb::mbar_wait(bar, phase);
+  return false;
 }
 
 // ------------------------------------------------------------------- take ---
@@ -180,10 +218,11 @@ int takeLaneBits(int64_t n, int64_t vecs) {
 // -------------------------------------------------------------- take_grad ---
 // The entries arrive sorted by row (keys, order), so a row's entries are a run
 // of neighbours.  The sorted list is cut into chunks of `span` entries; a group
-// of `lanes` threads takes a chunk, a thread one access's width of columns, and
-// adds up the runs that begin in the chunk, two incoming rows in flight
-// and four blocks a multiprocessor.
-// Every incoming row is read once, every row of the result written once.
+// of threads takes a chunk, a thread one access's width of columns, and adds up
+// the runs that begin in the chunk.  Every incoming row is read once, every row
+// of the result written once.  Rows of 1 KB and more come by bulk copies into
+// shared memory, two turns of four rows in flight, and the group is a block;
+// others come through registers, and a block holds several groups.
 //
 // A run that goes on past its chunk is finished by the group it began in, up
 // to the first chunk that lies inside the run as a whole.  Those inner chunks
@@ -195,6 +234,27 @@ int takeLaneBits(int64_t n, int64_t vecs) {
 //
 // Rows without entries are set to zero by blocks of their own, which look their
 // rows up in the sorted keys, one row a lane.
+constexpr int kGradBatch = 2;   // incoming rows in flight per thread, through registers
+constexpr int kTurnRows = 4;    // rows of a turn, by bulk copies
+constexpr int kZeroRows = 32;   // rows looked up by a block that clears
+constexpr int kBundle = 32;     // partial sums added up by one group
+
+struct GradPlan {
+  const int32_t *order;
+  const uint32_t *keys;
+  int64_t n;
+  int span;
+  unsigned slabs;          // groups side by side over the columns
+  int slab_vecs;           // accesses of a slab
+  unsigned chunk_blocks;   // blocks over chunks
+  unsigned period;         // one block of so many takes a chunk
+  void *partials;          // [chunks][cols]
+  uint32_t *tickets;       // [2][chunks][slabs], zero
+  int64_t chunks;
+  int lane_bits;           // threads of a group, through registers
+  uint32_t *status;
+};
+
 __device__ __forceinline__ int64_t lower_bound(const uint32_t *__restrict__ keys, int64_t lo, int64_t hi,
                                                uint32_t key) {
   while (lo < hi) {
@@ -207,234 +267,386 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t *__restrict__ keys
   return lo;
 }
 
-// Barrier over the threads of a group: part of a warp, a warp, or several.
-__device__ __forceinline__ void group_sync(int lane_bits, int group) {
-  if (lane_bits < 5)
-    __syncwarp(((1u << (1 << lane_bits)) - 1) << ((threadIdx.x & 31) & ~((1 << lane_bits) - 1)));
-  else if (lane_bits == 5)
-    __syncwarp();
-  else
-    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(1 << lane_bits) : "memory");
+// The same for a warp that looks for one key: 32 places at a time, so four
+// dependent reads where halving takes fifteen (an L2 access is about 0.4 us).
+__device__ __forceinline__ int64_t warp_lower_bound(const uint32_t *__restrict__ keys, int64_t lo, int64_t hi,
+                                                    uint32_t key) {
+  const int lane = threadIdx.x & 31;
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const int below = __popc(__ballot_sync(kAll, at < hi && __ldg(keys + (at < hi ? at : lo)) < key));
+    if (below == 0)
+      return lo;
+    hi = min(hi, lo + below * step);
+    lo += (below - 1) * step + 1;
+  }
+  return lo;
 }
 
-constexpr int kGradBatch = 2;   // incoming rows in flight per thread
-constexpr int kZeroRows = 32;   // rows looked up by a block that clears
-constexpr int kBundle = 32;     // partial sums added up by one group
-
-// A run's row: scale * sum, or that added to what the row holds.
-template <typename O, int V, bool ADD, typename A>
-__device__ __forceinline__ void write_sum(O *to, A scale, const A (&sum)[V], const Pack<O, V> &old, bool active) {
-  Pack<O, V> y;
-#pragma unroll
-  for (int e = 0; e < V; ++e)
-    y.v[e] = down<O, A>(ADD ? madd(scale, sum[e], up(old.v[e])) : scale * sum[e]);
-  if (active)
-    store<O, V>(to, y);
-}
-
-struct GradPlan {
-  const int32_t *order;
-  const uint32_t *keys;
-  int64_t n;
-  int span;
-  unsigned slabs;          // groups side by side over the columns
-  unsigned chunk_blocks;   // blocks over chunks, times slabs
-  unsigned zero_blocks;    // blocks that clear
-  void *partials;          // [chunks][cols]
-  uint32_t *tickets;       // [2][chunks][slabs], zero
-  int64_t chunks;
-  int lane_bits;
+// The threads that share a chunk: a block, or 1 << bits of its threads.
+template <bool BLOCK> struct Group {
+  int bits, lanes, lane, number;
+  __device__ __forceinline__ explicit Group(int lane_bits)
+      : bits(lane_bits), lanes(BLOCK ? (int)blockDim.x : 1 << lane_bits),
+        lane(BLOCK ? (int)threadIdx.x : threadIdx.x & ((1 << lane_bits) - 1)),
+        number(BLOCK ? 0 : threadIdx.x >> lane_bits) {}
+  __device__ __forceinline__ unsigned mask() const { // of a group inside a warp
+    return bits >= 5 ? kAll : ((1u << lanes) - 1) << ((threadIdx.x & 31) & ~(lanes - 1));
+  }
+  __device__ __forceinline__ void sync() const {
+    if (BLOCK)
+      __syncthreads();
+    else if (bits <= 5)
+      __syncwarp(mask());
+    else
+      asm volatile("bar.sync %0, %1;" ::"r"(number + 1), "r"(lanes) : "memory");
+  }
+  // lane 0's value; `words` is shared, one word per group
+  __device__ __forceinline__ uint32_t first(uint32_t v, uint32_t *words) const {
+    if (!BLOCK && bits <= 5)
+      return __shfl_sync(mask(), v, (threadIdx.x & 31) & ~(lanes - 1));
+    if (lane == 0)
+      words[number] = v;
+    sync();
+    v = words[number];
+    sync();
+    return v;
+  }
+  __device__ __forceinline__ int64_t find(const uint32_t *keys, int64_t lo, int64_t hi, uint32_t key) const {
+    return BLOCK || bits >= 5 ? warp_lower_bound(keys, lo, hi, key) : lower_bound(keys, lo, hi, key);
+  }
 };
 
-// A group walks over the entries [j, end) of one or several runs and writes a
-// run's row when the next begins; the row and the sum of the last stay behind.
-// The indices of the next batch are read along with the rows of this one, and
-// where the results are added to, the rows to be written with them.
+// V sums, kept and added in pairs where there are pairs.
+template <typename A, int V> struct Sums {
+  static constexpr int kPairs = V / 2;
+  typename Two<A>::type pair[kPairs > 0 ? kPairs : 1];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int e = 0; e < (kPairs > 0 ? kPairs : 1); ++e)
+      pair[e].x = pair[e].y = A(0);
+  }
+  template <typename T> __device__ __forceinline__ void add(const Pack<T, V> &x) {
+    if constexpr (V == 1) {
+      pair[0].x += up(x.v[0]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e)
+        pair[e] = add2(pair[e], up2(x.v + 2 * e));
+    }
+  }
+  // scale * sum, or that added to `old`
+  template <bool ADD, typename O> __device__ __forceinline__ Pack<O, V> result(A scale, const Pack<O, V> &old) const {
+    Pack<O, V> y;
+    if constexpr (V == 1) {
+      y.v[0] = down<O, A>(ADD ? madd(scale, pair[0].x, up(old.v[0])) : scale * pair[0].x);
+    } else {
+      typename Two<A>::type s;
+      s.x = s.y = scale;
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e)
+        down2(y.v + 2 * e, ADD ? madd2(s, pair[e], up2(old.v + 2 * e)) : mul2(scale, pair[e]));
+    }
+    return y;
+  }
+  __device__ __forceinline__ Pack<A, V> values() const {
+    Pack<A, V> y;
+    if constexpr (V == 1) {
+      y.v[0] = pair[0].x;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e)
+        down2(y.v + 2 * e, pair[e]);
+    }
+    return y;
+  }
+};
+
+// A thread's columns of the result.
+template <typename O, int V, bool ADD, typename A> struct GradColumn {
+  O *out;          // the thread's first column of row 0
+  int64_t stride;
+  A scale;
+  bool active;     // threads without columns go along for the barriers
+  __device__ __forceinline__ Pack<O, V> old(uint32_t row) const {
+    Pack<O, V> v{};
+    if (ADD && active)
+      v = load<O, V>(out + (int64_t)row * stride);
+    return v;
+  }
+  // A run's row: scale * sum, or that added to what the row holds.
+  __device__ __forceinline__ void write(uint32_t row, const Sums<A, V> &sum, const Pack<O, V> &old) const {
+    const Pack<O, V> y = sum.template result<ADD, O>(scale, old);
+    if (active)
+      store<O, V>(out + (int64_t)row * stride, y);
+  }
+};
+
+// The entries that a group adds up: sorted positions [begin, middle), then
+// [tail, end), which go on with the last run of the first part.
+struct Walk {
+  int64_t begin, middle, tail, end;
+  __device__ __forceinline__ int64_t count() const { return middle - begin + end - tail; }
+  __device__ __forceinline__ int64_t at(int64_t i) const {
+    return i < middle - begin ? begin + i : tail + (i - (middle - begin));
+  }
+};
+
+// Adds up one after another the rows of a batch of N entries, writing a run's
+// row when the next begins.  Where the results are added to, the rows to be
+// written are read for the whole batch first.
+template <bool WHOLE, int N, typename I, typename O, int V, bool ADD, typename A>
+__device__ __forceinline__ void add_rows(const Pack<I, V> (&x)[N], const uint32_t (&key)[N], int live,
+                                         const GradColumn<O, V, ADD, A> &column, uint32_t &row, Sums<A, V> &sum) {
+  Pack<O, V> old[ADD ? N : 1] = {};
+  if constexpr (ADD) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const uint32_t before = u > 0 ? key[u > 0 ? u - 1 : 0] : row;
+      if ((WHOLE || u < live) && key[u] != before)
+        old[u] = column.old(before);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+    if (WHOLE || u < live) {
+      if (key[u] != row) {
+        column.write(row, sum, old[ADD ? u : 0]);
+        row = key[u];
+        sum.clear();
+      }
+      sum.add(x[u]);
+    }
+}
+
+// Through registers: the indices of the next batch are read along with the rows
+// of this one.  The row and the sum of the last run stay behind.
 template <typename I, typename O, int V, bool ADD, typename A>
-__device__ __forceinline__ void walk_runs(const I *__restrict__ src, int64_t stride, const GradPlan &p, int64_t j,
-                                          int64_t end, A scale, O *dst, int64_t out_stride, bool active, uint32_t &row,
-                                          A (&sum)[V]) {
-  int32_t at[kGradBatch];
-  uint32_t key[kGradBatch];
+__device__ __forceinline__ void walk_registers(const I *__restrict__ src, int64_t stride, const GradPlan &p,
+                                               const Walk &w, const GradColumn<O, V, ADD, A> &column, uint32_t &row,
+                                               Sums<A, V> &sum) {
+  const int64_t count = w.count();
+  int32_t at[kGradBatch] = {};
+  uint32_t key[kGradBatch] = {}, next[kGradBatch];
 #pragma unroll
   for (int u = 0; u < kGradBatch; ++u)
-    if (j + u < end) {
-      at[u] = __ldg(p.order + j + u);
-      key[u] = __ldg(p.keys + j + u);
+    if (u < count) {
+      at[u] = __ldg(p.order + w.at(u));
+      key[u] = __ldg(p.keys + w.at(u));
     }
-  while (j < end) {
+  for (int64_t i = 0; i < count; i += kGradBatch) {
     Pack<I, V> x[kGradBatch];
-    Pack<O, V> old[ADD ? kGradBatch : 1];
 #pragma unroll
     for (int u = 0; u < kGradBatch; ++u)
-      if (j + u < end) {
+      if (i + u < count)
         x[u] = load<I, V>(src + (int64_t)at[u] * stride);
-        if constexpr (ADD) {
-          const uint32_t before = u > 0 ? key[u > 0 ? u - 1 : 0] : row;
-          if (key[u] != before)
-            old[u] = load<O, V>(dst + (int64_t)before * out_stride);
-        }
-      }
-    const int64_t next = j + kGradBatch;
-    uint32_t now[kGradBatch];
 #pragma unroll
     for (int u = 0; u < kGradBatch; ++u) {
-      now[u] = key[u];
-      if (next + u < end) {
-        at[u] = __ldg(p.order + next + u);
-        key[u] = __ldg(p.keys + next + u);
+      next[u] = key[u];
+      if (i + kGradBatch + u < count) {
+        at[u] = __ldg(p.order + w.at(i + kGradBatch + u));
+        key[u] = __ldg(p.keys + w.at(i + kGradBatch + u));
       }
     }
-#pragma unroll
-    for (int u = 0; u < kGradBatch; ++u)
-      if (j + u < end) {
-        if (now[u] != row) {
-          write_sum<O, V, ADD>(dst + (int64_t)row * out_stride, scale, sum, old[ADD ? u : 0], active);
-          row = now[u];
-#pragma unroll
-          for (int e = 0; e < V; ++e)
-            sum[e] = A(0);
-        }
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          sum[e] += up(x[u].v[e]);
-      }
-    j = next;
+    add_rows<false>(x, next, (int)min((int64_t)kGradBatch, count - i), column, row, sum);
   }
 }
 
-// Sum of the partial sums of chunks first, first + step, ... up to last.
+// By bulk copies: while the threads add up one turn of rows the next is on its
+// way.  The first threads fetch a row each.
+struct Turns {
+  uint64_t bar[2];
+  uint32_t key[2][kTurnRows];
+};
+template <typename I, typename O, int V, bool ADD, typename A>
+__device__ __forceinline__ bool walk_bulk(const I *__restrict__ src, int64_t stride, const GradPlan &p, const Walk &w,
+                                          int here, unsigned char *memory, Turns &turns,
+                                          const GradColumn<O, V, ADD, A> &column, uint32_t &row, Sums<A, V> &sum) {
+  const int64_t count = w.count(), last = (count + kTurnRows - 1) / kTurnRows;
+  const int r = threadIdx.x, mine = (column.active ? r : 0) * V;
+  if (r == 0) {
+    nmb::mbar_init(&turns.bar[0], kTurnRows);
+    nmb::mbar_init(&turns.bar[1], kTurnRows);
+    nmb::mbar_init_fence();
+  }
+  int32_t at = 0;
+  uint32_t key = 0;
+  auto look = [&](int64_t turn) { // the entry that this thread fetches in a turn
+    const int64_t i = turn * kTurnRows + r;
+    if (r < kTurnRows && i < count) {
+      at = __ldg(p.order + w.at(i));
+      key = __ldg(p.keys + w.at(i));
+    }
+  };
+  auto fetch = [&](int64_t turn) {
+    if (r >= kTurnRows)
+      return;
+    const int b = (int)(turn & 1);
+    if (turn * kTurnRows + r < count) {
+      turns.key[b][r] = key;
+      nmb::mbar_expect_tx(&turns.bar[b], (uint32_t)here * 16);
+      nmb::bulk_load(memory + (int64_t)(b * kTurnRows + r) * p.slab_vecs * 16, src + (int64_t)at * stride,
+                     (uint32_t)here * 16, &turns.bar[b]);
+    } else {
+      nmb::mbar_arrive(&turns.bar[b]);
+    }
+  };
+  look(0);
+  __syncthreads();
+  fetch(0);
+  look(1);
+  if (last > 1)
+    fetch(1);
+  look(2);
+  for (int64_t turn = 0; turn < last; ++turn) {
+    const int b = (int)(turn & 1);
+    if (!bulk_arrived(&turns.bar[b], (uint32_t)(turn >> 1) & 1, p.status))
+      return false;
+    const int live = (int)min((int64_t)kTurnRows, count - turn * kTurnRows);
+    const I *from = reinterpret_cast<const I *>(memory) + (int64_t)(b * kTurnRows) * p.slab_vecs * V + mine;
+    Pack<I, V> x[kTurnRows];
+    uint32_t keys[kTurnRows];
+    if (live == kTurnRows) {
+#pragma unroll
+      for (int u = 0; u < kTurnRows; ++u) {
+        keys[u] = turns.key[b][u];
+        x[u] = load<I, V>(from + u * p.slab_vecs * V);
+      }
+      add_rows<true>(x, keys, live, column, row, sum);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kTurnRows; ++u)
+        if (u < live) {
+          keys[u] = turns.key[b][u];
+          x[u] = load<I, V>(from + u * p.slab_vecs * V);
+        }
+      add_rows<false>(x, keys, live, column, row, sum);
+    }
+    __syncthreads(); // the turn's memory is free again
+    if (turn + 2 < last) {
+      fetch(turn + 2);
+      look(turn + 3);
+    }
+  }
+  return true;
+}
+
+// Sum of `count` partial sums: at `first`, then at second, second + step, ...
 template <int V, typename A>
 __device__ __forceinline__ void add_partials(const A *partials, int64_t width, int64_t first, int64_t count,
-                                             int64_t second, int64_t step, A (&sum)[V]) {
-#pragma unroll
-  for (int e = 0; e < V; ++e)
-    sum[e] = A(0);
+                                             int64_t second, int64_t step, Sums<A, V> &sum) {
+  sum.clear();
 #pragma unroll 4
   for (int64_t i = 0; i < count; ++i) {
     const A *from = partials + (i == 0 ? first : second + (i - 1) * step) * width;
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      sum[e] += __ldcg(from + e);
+    sum.add(load_l2<A, V>(from));
   }
 }
 
-template <typename I, typename O, int V, bool ADD>
+// BULK: the group is the block and V elements are 16 bytes of I.
+template <typename I, typename O, int V, bool ADD, bool BULK>
 __global__ void __launch_bounds__(kThreads, 4)
     nmb_take_rows_grad(const I *__restrict__ dout, int64_t stride, const GradPlan p, typename Acc<I>::type scale, O *out,
                        int64_t rows, int64_t out_stride, int64_t vecs) {
   using A = typename Acc<I>::type;
-  __shared__ uint32_t shared_word[kThreads / 64 + 1];
-  const int lanes = 1 << p.lane_bits, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> p.lane_bits;
-  const int groups = kThreads >> p.lane_bits;
-  Pack<O, V> zero;
-#pragma unroll
-  for (int e = 0; e < V; ++e)
-    zero.v[e] = down<O, A>(A(0));
+  extern __shared__ __align__(128) unsigned char memory[]; // BULK: [2][kTurnRows][slab_vecs] accesses
+  __shared__ uint32_t words[kThreads / 64 + 1];
+  __shared__ Turns turns;
+  const Group<BULK> group(p.lane_bits);
 
-  // blocks that clear are spread evenly among the others: theirs are writes
-  // alone, the others mostly wait for reads
-  const uint64_t all_chunks = (uint64_t)p.chunk_blocks * p.slabs, all = all_chunks + p.zero_blocks;
-  const uint64_t chunks_before = (uint64_t)blockIdx.x * all_chunks / all;
-  if (((uint64_t)blockIdx.x + 1) * all_chunks / all == chunks_before) { // rows without entries
-    const int64_t first = (int64_t)(blockIdx.x - chunks_before) * kZeroRows;
+  // every `period`-th block takes a chunk as long as there are any: blocks that
+  // clear are writes alone, the others mostly wait for reads
+  const unsigned turn = blockIdx.x / p.period, work = p.chunk_blocks * p.slabs;
+  if (blockIdx.x % p.period != 0 || turn >= work) { // rows without entries
+    const int64_t first = (int64_t)(blockIdx.x - min(turn + 1, work)) * kZeroRows;
     if (threadIdx.x < 32) {
       const int64_t v = first + threadIdx.x;
+      const int64_t lo = warp_lower_bound(p.keys, 0, p.n, (uint32_t)first);
+      const int64_t hi = warp_lower_bound(p.keys, lo, p.n, (uint32_t)min(first + kZeroRows, rows));
       bool absent = v < rows;
       if (absent) {
-        const int64_t at = lower_bound(p.keys, 0, p.n, (uint32_t)v);
-        absent = at >= p.n || __ldg(p.keys + at) != (uint32_t)v;
+        const int64_t at = lower_bound(p.keys, lo, hi, (uint32_t)v);
+        absent = at >= hi || __ldg(p.keys + at) != (uint32_t)v;
       }
       const uint32_t mask = __ballot_sync(kAll, absent);
       if (threadIdx.x == 0)
-        shared_word[0] = mask;
+        words[0] = mask;
     }
     __syncthreads();
-    const uint32_t mask = shared_word[0];
-    for (int r = group; r < kZeroRows; r += groups)
+    const uint32_t mask = words[0];
+    Pack<O, V> zero;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      zero.v[e] = down<O, A>(A(0));
+    for (int r = group.number; r < kZeroRows; r += (int)blockDim.x / group.lanes)
       if (mask >> r & 1)
-        for (int64_t c = lane; c < vecs; c += lanes)
+        for (int64_t c = group.lane; c < vecs; c += group.lanes)
           store<O, V>(out + (first + r) * out_stride + c * V, zero);
     return;
   }
 
-  const unsigned slab = (unsigned)(chunks_before % p.slabs);
-  const int64_t chunk = (int64_t)(chunks_before / p.slabs) * groups + group;
-  const int64_t column = (int64_t)slab * lanes + lane; // of accesses; a group's spare lanes idle through the barriers
-  const bool active = column < vecs;
+  const unsigned slab = turn % p.slabs;
+  const int64_t chunk = (int64_t)(turn / p.slabs) * (BULK ? 1 : kThreads >> p.lane_bits) + group.number;
+  const int64_t slab_first = (int64_t)slab * p.slab_vecs;
+  const int here = (int)min((int64_t)p.slab_vecs, vecs - slab_first);
+  const bool active = group.lane < here;
+  const int64_t col = slab_first + (active ? group.lane : 0);
   const int64_t begin = chunk * p.span;
   if (begin >= p.n)
     return;
   const int64_t end = min(begin + p.span, p.n);
   const uint32_t first_key = __ldg(p.keys + begin), last_key = __ldg(p.keys + end - 1);
   const uint32_t prev_key = begin > 0 ? __ldg(p.keys + begin - 1) : 0xffffffffu;
+  const uint32_t next_key = end < p.n ? __ldg(p.keys + end) : 0xffffffffu;
   if (first_key >= rows)
     return;
-  const I *src = dout + (active ? column : 0) * V;
-  O *dst = out + (active ? column : 0) * V;
-  auto write_last = [&](uint32_t row, const A(&sum)[V]) {
-    Pack<O, V> old = zero;
-    if (ADD)
-      old = load<O, V>(dst + (int64_t)row * out_stride);
-    write_sum<O, V, ADD>(dst + (int64_t)row * out_stride, scale, sum, old, active);
-  };
+  const GradColumn<O, V, ADD, A> column{out + col * V, out_stride, scale, active};
 
-  A sum[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e)
-    sum[e] = A(0);
-  int64_t owner = chunk, inner = 0; // where the long run began, its inner chunks
-  uint32_t row;
+  int64_t owner = chunk, inner = 0; // where a long run began, its inner chunks
+  Walk walk{begin, end, end, end};
   if (begin > 0 && prev_key == first_key && last_key == first_key && end - begin == p.span) {
     // inside a long run as a whole
-    row = first_key;
-    walk_runs<I, O, V, ADD>(src, stride, p, begin, end, scale, dst, out_stride, active, row, sum);
-    owner = lower_bound(p.keys, 0, begin, row) / p.span;
-    const int64_t run_end = lower_bound(p.keys, end, p.n, row + 1);
+    owner = group.find(p.keys, 0, begin, first_key) / p.span;
+    const int64_t run_end = next_key == first_key ? group.find(p.keys, end, p.n, first_key + 1) : end;
     inner = (run_end - (owner + 1) * p.span) / p.span;
   } else {
     // entries of a run that began before belong to the group it began in
-    int64_t j = prev_key == first_key ? lower_bound(p.keys, begin, end, first_key + 1) : begin;
-    const int64_t stop = last_key >= rows ? lower_bound(p.keys, j, end, (uint32_t)rows) : end;
-    if (j >= stop)
+    if (prev_key == first_key)
+      walk.begin = group.find(p.keys, begin, end, first_key + 1);
+    if (last_key >= rows)
+      walk.middle = group.find(p.keys, walk.begin, end, (uint32_t)rows);
+    if (walk.begin >= walk.middle)
       return;
-    row = __ldg(p.keys + j);
-    walk_runs<I, O, V, ADD>(src, stride, p, j, stop, scale, dst, out_stride, active, row, sum);
-    if (stop == end && end < p.n && __ldg(p.keys + end) == row) {
-      const int64_t run_end = lower_bound(p.keys, end, p.n, row + 1);
-      inner = (run_end - end) / p.span;
-      walk_runs<I, O, V, ADD>(src, stride, p, end + inner * p.span, run_end, scale, dst, out_stride, active, row, sum);
+    if (last_key < rows && next_key == last_key) {
+      walk.end = group.find(p.keys, end, p.n, last_key + 1);
+      inner = (walk.end - end) / p.span;
+      walk.tail = end + inner * p.span;
     }
-    if (inner == 0) {
-      write_last(row, sum);
+  }
+  uint32_t row = __ldg(p.keys + walk.begin);
+  Sums<A, V> sum;
+  sum.clear();
+  if constexpr (BULK) {
+    if (!walk_bulk<I, O, V, ADD>(dout + slab_first * V, stride, p, walk, here, memory, turns, column, row, sum))
       return;
-    }
+  } else {
+    walk_registers<I, O, V, ADD>(dout + col * V, stride, p, walk, column, row, sum);
+  }
+  if (inner == 0) {
+    column.write(row, sum, column.old(row));
+    return;
   }
 
   // A long run: leave the partial sum.  The last group of a bundle of chunks
   // adds its bundle's up, the last of those groups the bundles'.
-  A *partials = static_cast<A *>(p.partials) + column * V;
+  A *partials = static_cast<A *>(p.partials) + col * V;
   const int64_t width = vecs * V;
   auto leave_and_draw = [&](int64_t slot, uint32_t *ticket) {
-    if (active) {
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        __stcg(partials + slot * width + e, sum[e]);
-    }
+    if (active)
+      store<A, V>(partials + slot * width, sum.values());
     __threadfence();
-    group_sync(p.lane_bits, group);
-    uint32_t drawn = 0;
-    if (lane == 0)
-      drawn = atomicAdd(ticket + slab, 1u);
-    if (p.lane_bits <= 5) {
-      const int base = (threadIdx.x & 31) & ~(lanes - 1);
-      drawn = __shfl_sync(p.lane_bits == 5 ? kAll : ((1u << lanes) - 1) << base, drawn, base);
-    } else {
-      if (lane == 0)
-        shared_word[group] = drawn;
-      group_sync(p.lane_bits, group);
-      drawn = shared_word[group];
-    }
+    group.sync();
+    const uint32_t drawn = group.first(group.lane == 0 ? atomicAdd(ticket + slab, 1u) : 0, words);
     __threadfence();
     return drawn;
   };
@@ -443,15 +655,13 @@ __global__ void __launch_bounds__(kThreads, 4)
   const int64_t bundles = last / kBundle - owner / kBundle + 1;
   if (leave_and_draw(chunk, p.tickets + first * p.slabs) != (uint32_t)(count - 1))
     return;
-  add_partials<V>(active ? partials : partials - lane * V, width, first, count, first + 1, 1, sum);
+  add_partials<V>(partials, width, first, count, first + 1, 1, sum);
   if (bundles > 1) {
-    group_sync(p.lane_bits, group);
     if (leave_and_draw(first, p.tickets + (p.chunks + owner) * p.slabs) != (uint32_t)(bundles - 1))
       return;
-    add_partials<V>(active ? partials : partials - lane * V, width, owner, bundles, (owner / kBundle + 1) * kBundle,
-                    kBundle, sum);
+    add_partials<V>(partials, width, owner, bundles, (owner / kBundle + 1) * kBundle, kBundle, sum);
   }
-  write_last(row, sum);
+  column.write(row, sum, column.old(row));
 }
 
 // Entries per chunk: 32, or fewer (down to 4) where that leaves less than four
@@ -535,7 +745,6 @@ constexpr int kBulkChoices = 32;        // most choices of a token
 // took 94.5 us at 16 KB (two slabs a token), 98.1 us at 32 KB.  combine_grad: a
 // token with eight such rows 175.7 us in one turn of 36 KB, 203 us in two.
 constexpr int kBulkBytes = 16384, kBulkGradBytes = 46080;
-constexpr int kBulkLeast = 1024;        // narrower rows are left to the kernels above
 
 // What the threads of a block share about a token's choices.
 template <typename A> struct BulkChoices {
@@ -543,17 +752,6 @@ template <typename A> struct BulkChoices {
   int32_t at[kBulkChoices]; // -1: left out
   A weight[kBulkChoices];
 };
-
-// Waits for the block's copies.  A wait that runs out is reported in the queue's
-// status word; nothing is then written, and the block stays for its copies.
-__device__ __forceinline__ bool bulk_arrived(uint64_t *bar, uint32_t phase, uint32_t *status) {
-  if (nmb::mbar_wait(bar, phase))
-    return true;
-  if (status)
-    atomicExch(status, (uint32_t)nmb::kStatusWaitTimeout);
-  (void)nmb::mbar_wait(bar, phase);
-  return false;
-}
 
 template <typename T>
 __global__ void __launch_bounds__(kBulkThreads)
@@ -731,9 +929,6 @@ __global__ void __launch_bounds__(kThreads, 4)
     }
   }
 }
-
-template <typename A> struct Two { using type = float2; };
-template <> struct Two<double> { using type = double2; };
 
 // The same with the rows fetched by bulk copies, dout's first.  A block takes a
 // whole token; columns beyond a slab come in turns through the same memory.
@@ -1016,17 +1211,21 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
   withPair(dout->type, out->type, [&](auto i, auto o) {
     using I = decltype(i);
     using O = decltype(o);
-    constexpr int most = mostElems<I>() > mostElems<O>() ? mostElems<I>() : mostElems<O>();
-    const int v = accessElems(out->cols, most, {dout, out});
+    constexpr int wide = mostElems<I>();
+    const int v = accessElems(out->cols, wide, {dout, out});
+    const bool bulk = v == wide && out->cols * (int64_t)sizeof(I) >= kBulkLeast;
     const int64_t vecs = out->cols / v;
     const int bits = laneBits(vecs, kThreadBits);
     const int span = gradSpan(ids->count, vecs);
     const int64_t chunks = (ids->count + span - 1) / span;
     const unsigned slabs = (unsigned)((vecs + (int64_t(1) << bits) - 1) >> bits);
+    const int slabVecs = (int)((vecs + slabs - 1) / slabs);
     const unsigned zeros = accumulate ? 0 : (unsigned)((out->rows + kZeroRows - 1) / kZeroRows);
-    const GradPlan plan{order, keys,     ids->count, span,   slabs, blocksFor(chunks, bits),
-                        zeros, partials, tickets,    chunks, bits};
-    const int64_t blocks = (int64_t)plan.chunk_blocks * slabs + zeros;
+    GradPlan plan{order,    keys,    ids->count, span, slabs, slabVecs, bulk ? (unsigned)chunks : blocksFor(chunks, bits),
+                        1,        partials, tickets,   chunks, bits, nmb::statusWordOrNull(queue)};
+    const int64_t work = (int64_t)plan.chunk_blocks * slabs, blocks = work + zeros;
+    if (work > 0)
+      plan.period = (unsigned)(blocks / work);
     if (blocks >= (int64_t(1) << 31)) {
       nmb::setError("%s: too many indices for their width", who);
       ok = false;
@@ -1036,12 +1235,24 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
                               ws + 2 * need.entries + need.tickets + need.partials, tickets, 2 * chunks * slabs);
     if (!ok)
       return;
-    withElems<most>(v, [&](auto V) {
+    auto go = [&](auto kernel, int threads, size_t shared) {
+      kernel<<<(unsigned)blocks, threads, shared, s.stream>>>(static_cast<const I *>(dout->data), dout->stride, plan,
+                                                              (typename Acc<I>::type)scale,
+                                                              static_cast<O *>(out->data), out->rows, out->stride, vecs);
+    };
+    if (bulk) {
       const auto kernel =
-          accumulate ? nmb_take_rows_grad<I, O, V.value, true> : nmb_take_rows_grad<I, O, V.value, false>;
-      kernel<<<(unsigned)blocks, kThreads, 0, s.stream>>>(static_cast<const I *>(dout->data), dout->stride, plan,
-                                                          (typename Acc<I>::type)scale, static_cast<O *>(out->data),
-                                                          out->rows, out->stride, vecs);
+          accumulate ? nmb_take_rows_grad<I, O, wide, true, true> : nmb_take_rows_grad<I, O, wide, false, true>;
+      const size_t shared = (size_t)2 * kTurnRows * slabVecs * 16; // 64 KB at most
+      static std::atomic<bool> ready[2][64];
+      ok = nmb::rows::allowShared(who, kernel, 2 * kTurnRows * kThreads * 16, ready[accumulate ? 1 : 0], s.device);
+      if (ok)
+        go(kernel, (slabVecs + 31) / 32 * 32, shared);
+      return;
+    }
+    withElems<wide>(v, [&](auto V) {
+      go(accumulate ? nmb_take_rows_grad<I, O, V.value, true, false> : nmb_take_rows_grad<I, O, V.value, false, false>,
+         kThreads, 0);
     });
   });
   return ok && launched(who) ? 0 : 1;

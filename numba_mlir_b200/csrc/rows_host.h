@@ -104,6 +104,21 @@ inline bool launched(const char *who) {
   return true;
 }
 
+// Lets a kernel use more than 48 KB of shared memory; once per kernel and device.
+template <typename K> inline bool allowShared(const char *who, K kernel, int bytes, std::atomic<bool> *ready, int device) {
+  if (device >= 0 && device < 64 && ready[device])
+    return true;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) {
+    setError("%s: cudaFuncSetAttribute failed: %s", who, cudaGetErrorString(e));
+    (void)cudaGetLastError();
+    return false;
+  }
+  if (device >= 0 && device < 64)
+    ready[device] = true;
+  return true;
+}
+
 inline bool checkRows(const char *who, const char *name, const GPUXRows *r, bool result) {
   if (!r) {
     setError("%s: %s is null", who, name);
