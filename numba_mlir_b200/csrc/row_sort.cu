@@ -11,9 +11,10 @@
 // What it costs is latency, not bandwidth (an entry is 8 bytes), so the number
 // of dependent steps is what the three forms differ in.  Up to 4096 entries
 // stay in one block's shared memory for all passes: one launch.  Up to about a
-// million take two launches a pass: blocks of 1024 threads count their tiles,
-// then scatter them, each adding up the counts of all blocks for itself (at
-// most 148 of them).  Beyond that a launch in between adds the counts up.
+// million take a launch that counts tiles of 1024 to 8192 entries and one a pass
+// that scatters them: each block adds up the counts of all blocks for itself (at
+// most 148 of them), and counts its entries for the pass after it at the places
+// they go to.  Beyond that a launch a pass adds the counts up.
 #include "rows_host.h"
 
 #include <atomic>
@@ -91,21 +92,27 @@ struct Clear {
   }
 };
 
-// Ranks of a block's entries among its entries of equal digit, and where each
-// digit's entries go.  `counts` are per warp: counts[w][d] holds, in turn, the
-// entries of digit d in warp w and the digit's entries in the warps before w.
-// A digit is looked after by blockDim.x / bins threads, each of which adds up
-// its share of the warps (and of the blocks).
+// Where a block's entries go among its entries of each digit.  An entry's rank
+// is made of three: among the equal digits of its warp (rank), in the warps of
+// its part before that (counts), in the parts before that (parts).  A part is a
+// share of the warps that one thread adds up for a digit.
 struct Digits {
   uint16_t *counts;  // [warps][bins]
-  uint32_t *local;   // [threads]: a thread's share, then [bins] where the digit begins
-  uint32_t *sums;    // [32]
-  int bins, shift;
+  uint32_t *parts;   // [parts][bins]
+  int bins, bin_bits, shift, warps, part_bits; // 1 << part_bits warps to a part
   __device__ __forceinline__ uint32_t of(uint32_t key) const { return (key >> shift) & (uint32_t)(bins - 1); }
+
+  __device__ __forceinline__ Digits(uint16_t *counts, uint32_t *parts, int bin_bits, int shift)
+      : counts(counts), parts(parts), bins(1 << bin_bits), bin_bits(bin_bits), shift(shift),
+        warps((int)blockDim.x >> 5), part_bits(0) {
+    // as many parts as there are threads for every digit
+    while ((warps + (1 << part_bits) - 1) >> part_bits > max((int)blockDim.x >> bin_bits, 1))
+      ++part_bits;
+  }
 
   __device__ __forceinline__ void clear() const {
     uint32_t *words = reinterpret_cast<uint32_t *>(counts);
-    for (int i = threadIdx.x; i < (int)(blockDim.x >> 5) * bins / 2; i += blockDim.x)
+    for (int i = threadIdx.x; i < warps * bins / 2; i += blockDim.x)
       words[i] = 0;
   }
 
@@ -128,6 +135,54 @@ struct Digits {
     __syncwarp();
     return before + __popc(lower);
   }
+
+  // Adds the warps' counts up, four at a time, and the parts'; every thread gets
+  // the sum over its digits [first, last).  Call behind a barrier, and place
+  // another before `rank` results are used.
+  __device__ __forceinline__ uint32_t add_up(int first, int last, uint32_t *totals) const {
+    const int count = (warps + (1 << part_bits) - 1) >> part_bits;
+    for (int i = threadIdx.x; i < count * bins; i += blockDim.x) {
+      const int d = i & (bins - 1), from = i >> bin_bits << part_bits, to = min(from + (1 << part_bits), warps);
+      uint32_t sum = 0;
+      for (int w = from; w < to; w += 4) {
+        uint32_t c[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          c[u] = w + u < to ? counts[(w + u) * bins + d] : 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (w + u < to)
+            counts[(w + u) * bins + d] = (uint16_t)sum;
+          sum += c[u];
+        }
+      }
+      parts[i] = sum;
+    }
+    __syncthreads();
+    uint32_t all = 0;
+    for (int d = first; d < last; ++d) {
+      uint32_t sum = 0;
+      for (int q = 0; q < count; q += 4) {
+        uint32_t c[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          c[u] = q + u < count ? parts[(q + u) * bins + d] : 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (q + u < count)
+            parts[(q + u) * bins + d] = sum;
+          sum += c[u];
+        }
+      }
+      totals[d] = sum;
+      all += sum;
+    }
+    return all;
+  }
+  __device__ __forceinline__ uint32_t before(uint32_t digit) const {
+    const int warp = threadIdx.x >> 5;
+    return parts[(warp >> part_bits << bin_bits) + digit] + counts[(warp << bin_bits) + digit];
+  }
 };
 
 // ---- one block ------------------------------------------------------------------
@@ -135,13 +190,13 @@ template <int PER>
 __global__ void __launch_bounds__(kThreads)
     nmb_sort_one(const Ids ids, int n, int bits, int passes, const Results res, const Clear clear) {
   extern __shared__ uint32_t smem[];
-  uint32_t *keys = smem, *entries = smem + kThreads * PER;
-  Digits dg{reinterpret_cast<uint16_t *>(entries + kThreads * PER), nullptr, nullptr, 0, 0};
-  dg.local = reinterpret_cast<uint32_t *>(dg.counts + kWarps * kBins);
-  dg.sums = dg.local + kBins;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  uint32_t *keys = smem, *entries = smem + kThreads * PER; // [n]
+  uint32_t *start = entries + kThreads * PER;              // [bins]
+  uint32_t *parts = start + kBins;                         // [parts][bins]
+  uint32_t *sums = parts + kBins;                          // [32]
+  uint16_t *counts = reinterpret_cast<uint16_t *>(sums + 32);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int digit_bits = (bits + passes - 1) / passes;
-  dg.bins = 1 << digit_bits;
   const int begin = warp * PER * 32 + lane; // a warp owns PER * 32 consecutive entries
   clear.run();
   uint32_t key[PER], entry[PER], rank[PER];
@@ -151,7 +206,7 @@ __global__ void __launch_bounds__(kThreads)
     key[u] = begin + u * 32 < n ? ids.key(begin + u * 32) : 0;
   }
   for (int pass = 0; pass < passes; ++pass) {
-    dg.shift = pass * digit_bits;
+    const Digits dg(counts, parts, digit_bits, pass * digit_bits);
     dg.clear();
     __syncthreads();
 #pragma unroll
@@ -164,92 +219,94 @@ __global__ void __launch_bounds__(kThreads)
       rank[u] = dg.rank(dg.of(key[u]), i < n);
     }
     __syncthreads();
-    // a thread (or a few, when there are fewer threads than digits) per digit
-    const int each = (dg.bins + blockDim.x - 1) / blockDim.x;
+    // a thread (or a few digits, when there are fewer threads) per digit
+    const int each = (dg.bins + (int)blockDim.x - 1) / (int)blockDim.x;
     const int d0 = min(tid * each, dg.bins), d1 = min(d0 + each, dg.bins);
-    uint32_t total = 0;
+    uint32_t at = block_prefix(dg.add_up(d0, d1, start), sums);
     for (int d = d0; d < d1; ++d) {
-      dg.local[d] = total;
-      for (int w = 0; w < warps; ++w) {
-        const uint32_t c = dg.counts[w * dg.bins + d];
-        dg.counts[w * dg.bins + d] = (uint16_t)(total - dg.local[d]);
-        total += c;
-      }
-    }
-    const uint32_t before = block_prefix(total, dg.sums);
-    for (int d = d0; d < d1; ++d) {
-      dg.local[d] += before;
+      const uint32_t here = start[d];
+      start[d] = at;
       if (passes == 1 && res.offsets && d <= (int)ids.groups)
-        res.offsets[d] = (int32_t)dg.local[d];
+        res.offsets[d] = (int32_t)at;
+      at += here;
     }
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       if (begin + u * 32 < n) {
-        const uint32_t d = dg.of(key[u]), at = dg.local[d] + dg.counts[warp * dg.bins + d] + rank[u];
+        const uint32_t d = dg.of(key[u]), to = start[d] + dg.before(d) + rank[u];
         if (pass + 1 == passes) {
           if (res.order)
-            res.order[at] = (int32_t)entry[u];
+            res.order[to] = (int32_t)entry[u];
           if (res.keys)
-            res.keys[at] = key[u];
+            res.keys[to] = key[u];
           if (res.place)
-            res.place[entry[u]] = (int32_t)at;
+            res.place[entry[u]] = (int32_t)to;
         } else {
-          keys[at] = key[u];
-          entries[at] = entry[u];
+          keys[to] = key[u];
+          entries[to] = entry[u];
         }
       }
     }
     __syncthreads();
   }
 }
-template <int PER> constexpr int oneBytes() {
-  return 2 * kThreads * PER * 4 + kWarps * kBins * 2 + kBins * 4 + 32 * 4;
-}
+constexpr int kSharedWords = 2 * kBins + 32; // start, parts, sums
+template <int PER> constexpr int oneBytes() { return (2 * kThreads * PER + kSharedWords) * 4 + kWarps * kBins * 2; }
 
 // ---- many blocks ----------------------------------------------------------------
+// A block's counts are 16-bit (it has 8192 entries at most), two digits to a
+// word.  With `added` they hold the entries of the blocks before it, in words.
 struct Pass {
   Ids ids;                 // the first pass reads its keys here (keysIn == nullptr)
   const uint32_t *keysIn;
   const int32_t *entriesIn;
-  uint32_t *counts;        // [blocks][bins]: of each block; with `added`, of the blocks before it
-  uint32_t *totals;        // [bins], with `added`
+  uint32_t *counts;        // [blocks][bins / 2], of this pass
+  uint32_t *next;          // the same of the pass after it, zero, or null
+  uint32_t *added;         // [blocks][bins] and then [bins] totals, or null
   int64_t n;
-  int blocks, shift, bins, added;
+  int blocks, shift, bins, digit_bits;
   __device__ __forceinline__ uint32_t key(int64_t i) const { return keysIn ? keysIn[i] : ids.key(i); }
   __device__ __forceinline__ uint32_t digit(uint32_t k) const { return (k >> shift) & (uint32_t)(bins - 1); }
 };
 
-template <int PER> __global__ void __launch_bounds__(kThreads) nmb_sort_count(const Pass p, const Clear clear) {
-  __shared__ uint32_t count[kBins];
+// Counts of the first pass; those of a later one are made by the scatter before
+// it.  Also clears them, and the caller's words.
+template <int PER>
+__global__ void __launch_bounds__(kThreads) nmb_sort_count(const Pass p, const Clear next, const Clear clear) {
+  __shared__ uint32_t count[kBins / 2];
   const int64_t base = (int64_t)blockIdx.x * kThreads * PER + threadIdx.x;
   uint32_t key[PER];
 #pragma unroll
   for (int u = 0; u < PER; ++u)
     key[u] = base + u * kThreads < p.n ? p.key(base + u * kThreads) : 0;
+  next.run();
   clear.run();
-  for (int b = threadIdx.x; b < p.bins; b += kThreads)
+  for (int b = threadIdx.x; b < p.bins / 2; b += kThreads)
     count[b] = 0;
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < PER; ++u)
-    if (base + u * kThreads < p.n)
-      atomicAdd(&count[p.digit(key[u])], 1u);
+    if (base + u * kThreads < p.n) {
+      const uint32_t d = p.digit(key[u]);
+      atomicAdd(&count[d >> 1], d & 1 ? 0x10000u : 1u);
+    }
   __syncthreads();
-  for (int b = threadIdx.x; b < p.bins; b += kThreads)
-    p.counts[(int64_t)blockIdx.x * p.bins + b] = count[b];
+  for (int b = threadIdx.x; b < p.bins / 2; b += kThreads)
+    p.counts[(int64_t)blockIdx.x * (p.bins / 2) + b] = count[b];
 }
 
-// A warp per digit: counts[b][d] <- sum of counts[0..b)[d], totals[d] <- the sum.
+// A warp per digit: added[b][d] <- sum of counts[0..b)[d], and the totals.
 constexpr int kAddThreads = 256;
-__global__ void __launch_bounds__(kAddThreads) nmb_sort_add(uint32_t *counts, uint32_t *totals, int blocks, int bins) {
+__global__ void __launch_bounds__(kAddThreads) nmb_sort_add(const Pass p) {
   const int lane = threadIdx.x & 31, d = blockIdx.x * (kAddThreads / 32) + (threadIdx.x >> 5);
-  if (d >= bins)
+  if (d >= p.bins)
     return;
   uint32_t carry = 0;
-  for (int b0 = 0; b0 < blocks; b0 += 32) {
-    uint32_t *at = counts + (int64_t)(b0 + lane) * bins + d;
-    const uint32_t v = b0 + lane < blocks ? *at : 0;
+  for (int b0 = 0; b0 < p.blocks; b0 += 32) {
+    const int b = b0 + lane;
+    const uint32_t pair = b < p.blocks ? p.counts[(int64_t)b * (p.bins / 2) + (d >> 1)] : 0;
+    const uint32_t v = d & 1 ? pair >> 16 : pair & 0xffff;
     uint32_t inc = v;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
@@ -257,23 +314,24 @@ __global__ void __launch_bounds__(kAddThreads) nmb_sort_add(uint32_t *counts, ui
       if (lane >= s)
         inc += t;
     }
-    if (b0 + lane < blocks)
-      *at = carry + inc - v;
+    if (b < p.blocks)
+      p.added[(int64_t)b * p.bins + d] = carry + inc - v;
     carry += __shfl_sync(kAll, inc, 31);
   }
   if (lane == 0)
-    totals[d] = carry;
+    p.added[(int64_t)p.blocks * p.bins + d] = carry;
 }
 
 template <int PER>
 __global__ void __launch_bounds__(kThreads)
     nmb_sort_scatter(const Pass p, uint32_t *keysOut, int32_t *entriesOut, int32_t *place, int32_t *offsets) {
   extern __shared__ uint32_t smem[];
-  uint32_t *before = smem;                // [threads]: a thread's blocks before this one, all its blocks
-  uint32_t *all = smem + kThreads;        // [threads]
-  Digits dg{reinterpret_cast<uint16_t *>(all + kThreads), nullptr, nullptr, p.bins, p.shift};
-  dg.local = reinterpret_cast<uint32_t *>(dg.counts + kWarps * kBins);
-  dg.sums = dg.local + kBins;
+  uint32_t *start = smem;                   // [bins]
+  uint32_t *parts = start + kBins;          // [parts][bins]
+  uint32_t *sums = parts + kBins;           // [32]
+  uint2 *shares = reinterpret_cast<uint2 *>(sums + 32); // [2][threads]: a thread's blocks before this one, all its blocks
+  uint16_t *counts = reinterpret_cast<uint16_t *>(shares + 2 * kThreads);
+  const Digits dg(counts, parts, p.digit_bits, p.shift);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t begin = ((int64_t)blockIdx.x * kWarps + warp) * PER * 32 + lane;
   uint32_t key[PER], rank[PER];
@@ -285,84 +343,75 @@ __global__ void __launch_bounds__(kThreads)
     entry[u] = i < p.n && p.entriesIn ? p.entriesIn[i] : (int32_t)i;
   }
   dg.clear();
-  // counts of the blocks: thread t adds up blocks t / bins, + share, ... of digit t % bins
-  const int share = kThreads / p.bins, d = tid & (p.bins - 1), part = tid / p.bins;
-  uint32_t mine = 0, sum = 0;
-  if (p.added) {
-    if (part == 0) {
-      mine = p.counts[(int64_t)blockIdx.x * p.bins + d];
-      sum = p.totals[d];
-    }
-  } else {
-    // sixteen loads in flight: one by one they took 15 of the kernel's 19 us at
-    // 131072 entries (an L2 access costs about 700 cycles)
+  // counts of all blocks: a thread adds up every share-th block for two digits,
+  // sixteen loads in flight (one by one they took 15 of the kernel's 19 us at
+  // 131072 entries: an L2 access costs about 700 cycles)
+  const int pairs = p.bins / 2, share = kThreads >> (p.digit_bits - 1), part = tid >> (p.digit_bits - 1);
+  uint2 mine = make_uint2(0, 0), all = make_uint2(0, 0);
+  if (!p.added) {
+    const uint32_t *from = p.counts + (tid & (pairs - 1));
     for (int b0 = part; b0 < p.blocks; b0 += 16 * share) {
       uint32_t c[16];
 #pragma unroll
       for (int u = 0; u < 16; ++u)
-        c[u] = b0 + u * share < p.blocks ? __ldg(p.counts + (int64_t)(b0 + u * share) * p.bins + d) : 0;
+        c[u] = b0 + u * share < p.blocks ? __ldg(from + (int64_t)(b0 + u * share) * pairs) : 0;
 #pragma unroll
       for (int u = 0; u < 16; ++u) {
-        mine += b0 + u * share < (int)blockIdx.x ? c[u] : 0;
-        sum += c[u];
+        const uint32_t lo = c[u] & 0xffff, hi = c[u] >> 16;
+        all.x += lo;
+        all.y += hi;
+        mine.x += b0 + u * share < (int)blockIdx.x ? lo : 0;
+        mine.y += b0 + u * share < (int)blockIdx.x ? hi : 0;
       }
     }
+    shares[tid] = mine;
+    shares[kThreads + tid] = all;
   }
-  before[tid] = mine;
-  all[tid] = sum;
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < PER; ++u)
     rank[u] = dg.rank(dg.of(key[u]), begin + u * 32 < p.n);
+  // where digit tid's entries begin: behind all smaller digits, and behind the
+  // digit's entries in the blocks before this one
+  uint32_t blocks_before = 0, total = 0;
   if (tid < p.bins) {
-    for (int s = 1; s < share; ++s) {
-      mine += before[s * p.bins + d];
-      sum += all[s * p.bins + d];
+    if (p.added) {
+      blocks_before = p.added[(int64_t)blockIdx.x * p.bins + tid];
+      total = p.added[(int64_t)p.blocks * p.bins + tid];
+    } else {
+      const uint32_t *words = reinterpret_cast<const uint32_t *>(shares);
+#pragma unroll 4
+      for (int s = 0; s < share; ++s) {
+        blocks_before += words[s * p.bins + tid];
+        total += words[2 * kThreads + s * p.bins + tid];
+      }
     }
-  } else {
-    mine = sum = 0;
   }
-  const uint32_t start = block_prefix(sum, dg.sums); // the digits begin there; every warp's counts are done
-  if (tid < p.bins) {
-    if (offsets && blockIdx.x == 0 && d <= (int)p.ids.groups)
-      offsets[d] = (int32_t)start;
-    dg.local[d] = start + mine;
-  }
-  // warps before each warp: this thread's share of the warps, then the shares
-  const int rows = kWarps / (share < kWarps ? share : kWarps);
-  uint32_t count = 0;
-  if (part * rows < kWarps)
-    for (int w = part * rows; w < (part + 1) * rows; ++w) {
-      const uint32_t c = dg.counts[w * p.bins + d];
-      dg.counts[w * p.bins + d] = (uint16_t)count;
-      count += c;
-    }
-  __syncthreads();
-  before[tid] = count;
-  __syncthreads();
-  if (part * rows < kWarps) {
-    uint32_t shift = 0;
-    for (int s = 0; s < part; ++s)
-      shift += before[s * p.bins + d];
-    for (int w = part * rows; w < (part + 1) * rows; ++w)
-      dg.counts[w * p.bins + d] += (uint16_t)shift;
-  }
+  const uint32_t digit_start = block_prefix(total, sums); // also: every warp's counts are done
+  if (offsets && blockIdx.x == 0 && tid <= (int)p.ids.groups && tid < p.bins)
+    offsets[tid] = (int32_t)digit_start;
+  dg.add_up(min(tid, p.bins), min(tid + 1, p.bins), start);
+  if (tid < p.bins)
+    start[tid] = digit_start + blocks_before;
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     if (begin + u * 32 < p.n) {
-      const uint32_t digit = dg.of(key[u]);
-      const uint32_t at = dg.local[digit] + dg.counts[warp * p.bins + digit] + rank[u];
+      const uint32_t d = dg.of(key[u]), at = start[d] + dg.before(d) + rank[u];
       if (keysOut)
         keysOut[at] = key[u];
       if (entriesOut)
         entriesOut[at] = entry[u];
       if (place)
         place[entry[u]] = (int32_t)at;
+      if (p.next) { // the digit that the entry has in the next pass, in the block that will read it there
+        const uint32_t e = (key[u] >> (p.shift + p.digit_bits)) & (uint32_t)(p.bins - 1);
+        atomicAdd(p.next + (int64_t)(at / (kThreads * PER)) * pairs + (e >> 1), e & 1 ? 0x10000u : 1u);
+      }
     }
   }
 }
-constexpr int kScatterBytes = 2 * kThreads * 4 + kWarps * kBins * 2 + kBins * 4 + 32 * 4;
+constexpr int kScatterBytes = kSharedWords * 4 + 2 * kThreads * 8 + kWarps * kBins * 2;
 
 // offsets[g] = position of the first key >= g, for the sorts of several passes.
 constexpr int kOffsetThreads = 256;
@@ -413,6 +462,9 @@ int64_t manyBlocks(int64_t n) {
   return (n + tile - 1) / tile;
 }
 
+// Counts of the digits of all blocks, of one pass.
+size_t countBytes(size_t blocks) { return padded(blocks * kBins * 2); }
+
 // Calls f(constant) for 1, 2, 4 or 8.
 template <typename F> bool withPer(int per, F &&f) {
   if (per == 1)
@@ -436,7 +488,8 @@ size_t sortBytes(int64_t count, int64_t groups) {
   const size_t pairs = padded((size_t)count * 4);
   if (fitsOneBlock(count))
     return bitsOf(groups) > kMaxDigitBits ? pairs : 0; // the sorted keys, for the offsets
-  return 4 * pairs + padded((size_t)kBins * (size_t)manyBlocks(count) * 4) + padded(kBins * 4);
+  const size_t blocks = (size_t)manyBlocks(count);
+  return 4 * pairs + 2 * countBytes(blocks) + (blocks > kMostBlocks ? padded((blocks + 1) * kBins * 4) : 0);
 }
 
 bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t groups, int32_t *order,
@@ -476,39 +529,56 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
     const int64_t blocks = manyBlocks(n);
     uint32_t *keyBuf[2] = {reinterpret_cast<uint32_t *>(ws), reinterpret_cast<uint32_t *>(ws + pairs)};
     int32_t *entryBuf[2] = {reinterpret_cast<int32_t *>(ws + 2 * pairs), reinterpret_cast<int32_t *>(ws + 3 * pairs)};
-    uint32_t *counts = reinterpret_cast<uint32_t *>(ws + 4 * pairs);
-    uint32_t *totals =
-        reinterpret_cast<uint32_t *>(ws + 4 * pairs + padded((size_t)kBins * (size_t)blocks * 4));
-    const int digitBits = (bits + passes - 1) / passes;
-    Pass p{in, nullptr, nullptr, counts, totals, n, (int)blocks, 0, 1 << digitBits, blocks > kMostBlocks};
-    for (int pass = 0; pass < passes; ++pass) {
-      const bool last = pass + 1 == passes;
-      // the passes alternate between the buffers so that the last one may write
-      // sorted keys into buffer 0 (see above)
-      const int to = (passes - 1 - pass) & 1;
-      p.shift = pass * digitBits;
-      const bool ok = withPer(perThread(n), [&](auto P) {
-        static std::atomic<bool> ready[64];
-        if (!nmb::rows::allowShared(who, nmb_sort_scatter<P.value>, kScatterBytes, ready, s.device))
-          return false;
-        nmb_sort_count<P.value><<<(unsigned)blocks, kThreads, 0, s.stream>>>(p, Clear{clear, pass == 0 ? clearWords : 0});
-        if (!launched(who))
-          return false;
-        if (p.added) {
-          nmb_sort_add<<<(unsigned)((p.bins + kAddThreads / 32 - 1) / (kAddThreads / 32)), kAddThreads, 0, s.stream>>>(counts, totals, (int)blocks, p.bins);
+    const size_t countSize = countBytes((size_t)blocks);
+    uint32_t *counts[2] = {reinterpret_cast<uint32_t *>(ws + 4 * pairs),
+                           reinterpret_cast<uint32_t *>(ws + 4 * pairs + countSize)};
+    uint32_t *added =
+        blocks > kMostBlocks ? reinterpret_cast<uint32_t *>(ws + 4 * pairs + 2 * countSize) : nullptr;
+    const int digitBits = (bits + passes - 1) / passes, bins = 1 << digitBits;
+    const int64_t countWords = blocks * (bins / 2);
+    Pass p{in, nullptr, nullptr, counts[0], nullptr, added, n, (int)blocks, 0, bins, digitBits};
+    const bool ok = withPer(perThread(n), [&](auto P) {
+      static std::atomic<bool> ready[64];
+      if (!nmb::rows::allowShared(who, nmb_sort_scatter<P.value>, kScatterBytes, ready, s.device))
+        return false;
+      nmb_sort_count<P.value><<<(unsigned)blocks, kThreads, 0, s.stream>>>(
+          p, Clear{counts[1], passes > 1 ? countWords : 0}, Clear{clear, clearWords});
+      if (!launched(who))
+        return false;
+      for (int pass = 0; pass < passes; ++pass) {
+        const bool last = pass + 1 == passes;
+        // the passes alternate between the buffers so that the last one may write
+        // sorted keys into buffer 0 (see above)
+        const int to = (passes - 1 - pass) & 1;
+        p.shift = pass * digitBits;
+        p.counts = counts[pass & 1];
+        p.next = last ? nullptr : counts[(pass + 1) & 1];
+        if (pass > 0 && !last) {
+          // the counts of the pass before, about to be used for the pass after
+          const cudaError_t e = cudaMemsetAsync(p.next, 0, (size_t)countWords * 4, s.stream);
+          if (e != cudaSuccess) {
+            setError("%s: cudaMemsetAsync failed: %s", who, cudaGetErrorString(e));
+            (void)cudaGetLastError();
+            return false;
+          }
+        }
+        if (added) {
+          nmb_sort_add<<<(unsigned)((bins + kAddThreads / 32 - 1) / (kAddThreads / 32)), kAddThreads, 0, s.stream>>>(p);
           if (!launched(who))
             return false;
         }
         nmb_sort_scatter<P.value><<<(unsigned)blocks, kThreads, kScatterBytes, s.stream>>>(
             p, last ? keys : keyBuf[to], last ? order : entryBuf[to], last ? place : nullptr,
             passes == 1 ? offsets : nullptr);
-        return launched(who);
-      });
-      if (!ok)
-        return false;
-      p.keysIn = keyBuf[to];
-      p.entriesIn = entryBuf[to];
-    }
+        if (!launched(who))
+          return false;
+        p.keysIn = keyBuf[to];
+        p.entriesIn = entryBuf[to];
+      }
+      return true;
+    });
+    if (!ok)
+      return false;
   }
   if (offsets && passes > 1) {
     nmb_sort_offsets<<<offsetBlocks, kOffsetThreads, 0, s.stream>>>(keys, n, groups, offsets);
