@@ -186,15 +186,25 @@ inline int laneBits(int64_t vecs, int most) {
   return b;
 }
 
+// Rows of a result that the sort's launches set to zero on the side, from the
+// last one down: a sort keeps few multiprocessors busy.  `left` is the number of
+// rows at the front that are not set yet.
+struct Clearing {
+  unsigned char *data = nullptr;
+  int64_t left = 0;
+  int64_t rowBytes = 0, stride = 0; // in bytes
+  int unit = 1;                     // bytes per access: 16, 8, 4 or 2
+};
+
 // Stable sort of the indices by key, key = id inside [0, groups), groups for
 // every other id.  Any of the results may be null: order[j] = entry at sorted
 // position j, keys[j] its key, place[order[j]] = j, offsets[g] = position of
-// the first key >= g for g <= groups.  `clear` words of the caller's are set to
-// zero on the way.
+// the first key >= g for g <= groups.  `words` (the caller's, `wordCount` of them)
+// are set to zero, and rows of `clearing`.
 size_t sortBytes(int64_t count, int64_t groups);
 bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t groups, int32_t *order,
-               uint32_t *keys, int32_t *place, int32_t *offsets, void *workspace, uint32_t *clear = nullptr,
-               int64_t clearWords = 0);
+               uint32_t *keys, int32_t *place, int32_t *offsets, void *workspace, uint32_t *words = nullptr,
+               int64_t wordCount = 0, Clearing *clearing = nullptr);
 
 } // namespace rows
 } // namespace nmb

@@ -348,17 +348,24 @@ def _result(queue, shape, kind):
 
 
 def _workspace(workspace, name):
-    """(address, bytes) of a caller's workspace, a contiguous device array."""
+    """(address, bytes, operand) of a caller's workspace: a contiguous device
+    array of any type."""
     if workspace is None:
         return None, 0, None
-    if isinstance(workspace, DeviceArray):
-        if not workspace.is_c_contiguous:
+    op = _Operand()
+    op.obj, op.item, op.strides = workspace, 1, (1,)
+    if type(workspace) is not DeviceArray and "torch" in sys.modules and isinstance(
+            workspace, sys.modules["torch"].Tensor) and workspace.is_cuda:
+        if not workspace.is_contiguous():
             raise ValueError(f"{name} must be C-contiguous")
-        op = _Operand()
-        op.obj, op.ptr, op.item, op.shape, op.strides = workspace, workspace.ptr, 1, (workspace.nbytes,), (1,)
-        op.queue, op.device = workspace.queue, workspace.queue.device
-        return op.ptr, workspace.nbytes, op
-    return _workspace(as_device_array(workspace), name)
+        op.ptr, op.shape = workspace.data_ptr(), (workspace.numel() * workspace.element_size(),)
+        op.queue, op.device = None, workspace.get_device()
+    else:
+        arr = as_device_array(workspace)
+        if not arr.is_c_contiguous:
+            raise ValueError(f"{name} must be C-contiguous")
+        op.ptr, op.shape, op.queue, op.device = arr.ptr, (arr.nbytes,), arr.queue, arr.queue.device
+    return op.ptr, op.shape[0], op
 
 
 _ref = ctypes.byref

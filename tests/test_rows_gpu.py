@@ -600,6 +600,46 @@ def test_torch_tensors(queue):
         nm.take_rows(torch.randn(4, 4), ids)
 
 
+def test_torch_graph_with_workspaces(queue):
+    """Calls recorded by torch on a stream of its own, with torch's workspaces
+    and without, replay on new inputs."""
+    import torch
+
+    import numba_mlir_b200 as nm
+
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        ids = torch.randint(-1, 400, (6000,), device="cuda", dtype=torch.int32)
+        d = torch.randn(6000, 520, device="cuda")
+        grads = [torch.empty(400, 520, device="cuda") for _ in range(2)]
+        plan = nm.RowGroups(torch.empty_like(ids), torch.empty_like(ids), torch.empty(401, dtype=torch.int32, device="cuda"))
+        ws = torch.empty(nm.take_rows_grad_workspace(6000, 400, 520), dtype=torch.uint8, device="cuda")
+        ws2 = torch.empty(nm.group_rows_workspace(6000, 400), dtype=torch.uint8, device="cuda")
+
+        def calls():
+            nm.take_rows_grad(d, ids, out=grads[0], workspace=ws)
+            nm.take_rows_grad(d, ids, out=grads[1])
+            nm.group_rows(ids, 400, plan=plan, workspace=ws2)
+
+        calls()
+        st.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            calls()
+        for seed in (1, 2):
+            ids.copy_(torch.randint(-1, 400, (6000,), device="cuda", dtype=torch.int32))
+            d.normal_()
+            g.replay()
+            st.synchronize()
+            want, bound = grad_bound(d.double().cpu().numpy(), ids.cpu().numpy(), 400, 1.0, 2.0**-24)
+            for got in grads:
+                assert_near(got.double().cpu().numpy(), want, bound, "float32")
+            order, place, offsets = plan_of(ids.cpu().numpy(), 400)
+            for got, ref in zip(plan, (order, place, offsets)):
+                assert np.array_equal(got.cpu().numpy(), ref)
+        del g
+
+
 def test_refusals(queue):
     import numba_mlir_b200 as nm
 
