@@ -384,6 +384,14 @@ int _mlir_ciface_nmb_group_rows_device(void *queue, const GPUXIndex *ids, int64_
 int _mlir_ciface_nmb_dispatch_rows_device(void *queue, const GPUXRows *x, int64_t k, const int32_t *place,
                                           const int32_t *kept, const GPUXRows *out);
 
+/* group_rows and dispatch_rows in one call (one launch for up to 4096 entries in
+ * up to 1024 groups): the entries of token t are ids[t * k .. t * k + k), k =
+ * ids->count / x->rows, and out has at least ids->count rows.  The workspace is
+ * group_rows'. */
+int _mlir_ciface_nmb_sort_dispatch_rows_device(void *queue, const GPUXRows *x, const GPUXIndex *ids,
+                                               int64_t groups, int32_t *order, int32_t *place, int32_t *offsets,
+                                               void *workspace, size_t workspaceBytes, const GPUXRows *out);
+
 /* out[t,:] = sum over j < k of weights[t * k + j] * ys[place[t * k + j],:],
  * entries whose position is outside [0, *kept) left out; weights NULL: ones. */
 int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows *ys, int64_t k, const int32_t *place,

@@ -18,6 +18,8 @@ using TakeFn = int (*)(void *, const GPUXRows *, const GPUXIndex *, double, cons
 using TakeGradFn = int (*)(void *, const GPUXRows *, const GPUXIndex *, double, const GPUXRows *, int, void *, size_t);
 using GroupFn = int (*)(void *, const GPUXIndex *, int64_t, int32_t *, int32_t *, int32_t *, void *, size_t);
 using DispatchFn = int (*)(void *, const GPUXRows *, int64_t, const int32_t *, const int32_t *, const GPUXRows *);
+using SortDispatchFn = int (*)(void *, const GPUXRows *, const GPUXIndex *, int64_t, int32_t *, int32_t *, int32_t *,
+                               void *, size_t, const GPUXRows *);
 using CombineFn = int (*)(void *, const GPUXRows *, int64_t, const int32_t *, const int32_t *, const void *, int,
                           const GPUXRows *);
 using CombineGradFn = int (*)(void *, const GPUXRows *, const GPUXRows *, int64_t, const int32_t *, const int32_t *,
@@ -29,6 +31,7 @@ struct Entries {
   DispatchFn dispatch;
   CombineFn combine;
   CombineGradFn combineGrad;
+  SortDispatchFn sortDispatch;
 };
 inline Entries gEntries{};
 inline PyObject *gTypes = nullptr;       // dtype -> (float code or -1, index bytes, item size)
@@ -249,12 +252,14 @@ inline const int32_t *ints(const Operand &o, int64_t at = 0) { return reinterpre
 
 // rows_init(entry addresses, types, array type): binds the C entries.
 inline PyObject *py_rows_init(PyObject *, PyObject *args) {
-  unsigned long long a[6];
+  unsigned long long a[7];
   PyObject *types, *array;
-  if (!PyArg_ParseTuple(args, "(KKKKKK)OO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &types, &array))
+  if (!PyArg_ParseTuple(args, "(KKKKKKK)OO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &types, &array))
     return nullptr;
-  gEntries = {reinterpret_cast<TakeFn>(a[0]),     reinterpret_cast<TakeGradFn>(a[1]), reinterpret_cast<GroupFn>(a[2]),
-              reinterpret_cast<DispatchFn>(a[3]), reinterpret_cast<CombineFn>(a[4]),  reinterpret_cast<CombineGradFn>(a[5])};
+  gEntries = {reinterpret_cast<TakeFn>(a[0]),      reinterpret_cast<TakeGradFn>(a[1]),
+              reinterpret_cast<GroupFn>(a[2]),     reinterpret_cast<DispatchFn>(a[3]),
+              reinterpret_cast<CombineFn>(a[4]),   reinterpret_cast<CombineGradFn>(a[5]),
+              reinterpret_cast<SortDispatchFn>(a[6])};
   Py_INCREF(types);
   Py_XSETREF(gTypes, types);
   Py_INCREF(array);
@@ -353,14 +358,13 @@ inline PyObject *py_rows_dispatch(PyObject *, PyObject *const *a, Py_ssize_t n) 
         offsets.size() != groups + 1 || !apart(all, 4, 6))
       return answer(0);
     const GPUXIndex i = ids.indexArg();
-    if (gEntries.group(q.handle, &i, groups, const_cast<int32_t *>(ints(order)), const_cast<int32_t *>(ints(place)),
-                       const_cast<int32_t *>(ints(offsets)), nullptr, 0))
-      return answer(2);
-  } else {
-    const Operand *all[] = {&out, &x, &place, &offsets};
-    if (!apart(all, 1, 4))
-      return answer(0);
+    return called(gEntries.sortDispatch(q.handle, &xr, &i, groups, const_cast<int32_t *>(ints(order)),
+                                        const_cast<int32_t *>(ints(place)), const_cast<int32_t *>(ints(offsets)),
+                                        nullptr, 0, &o));
   }
+  const Operand *all[] = {&out, &x, &place, &offsets};
+  if (!apart(all, 1, 4))
+    return answer(0);
   return called(gEntries.dispatch(q.handle, &xr, k, ints(place), ints(offsets, offsets.size() - 1), &o));
 }
 

@@ -105,7 +105,8 @@ def _fast():
     """The native call path (csrc/fastcall/rows_call.h), bound on first use."""
     global _native
     fast, lib = _rt.fastcall(), _rt.load()
-    entries = ("take_rows", "take_rows_grad", "group_rows", "dispatch_rows", "combine_rows", "combine_rows_grad")
+    entries = ("take_rows", "take_rows_grad", "group_rows", "dispatch_rows", "combine_rows", "combine_rows_grad",
+               "sort_dispatch_rows")
     fast.rows_init(tuple(ctypes.cast(getattr(lib, f"_mlir_ciface_nmb_{e}_device"), ctypes.c_void_p).value
                          for e in entries), _native_types, DeviceArray)
     _native = fast
@@ -486,25 +487,28 @@ def group_rows(ids, groups, plan=None, workspace=None, queue=None):
     results = [_operand(x, n) for x, n in zip(plan, RowGroups._fields)] if plan is not None else []
     ws, ws_bytes, w = _workspace(workspace, "workspace")
     on = _On(queue, [i] + results + ([w] if w is not None else []))
-    return _group(on, i, groups, plan, results, ws, ws_bytes, w)
-
-
-def _group(on, i, groups, plan, results, ws=None, ws_bytes=0, w=None):
-    index = _index_arg(i, "ids")
-    groups = int(groups)
+    index, groups = _index_arg(i, "ids"), int(groups)
     if groups < 0:
         raise ValueError("a negative number of groups")
     if plan is None:
-        new = lambda shape: empty(shape, np.int32, queue=on.queue)  # noqa: E731
-        plan = RowGroups(new((index.count,)), new(i.shape), new((groups + 1,)))
+        plan = _new_plan(on.queue, i.shape, groups)
         results = [_operand(x, n) for x, n in zip(plan, RowGroups._fields)]
-    order = _int32_arg(results[0], "order", index.count)
-    place = _int32_arg(results[1], "place", index.count)
-    offsets = _int32_arg(results[2], "offsets", groups + 1)
+    order, place, offsets = _whole_plan(results, index.count, groups)
     _no_overlap(results if w is None else results + [w], [i])
     on.done(_rt.load()._mlir_ciface_nmb_group_rows_device(on.queue.handle, _ref(index), groups, order, place, offsets,
                                                           ws, ws_bytes))
     return RowGroups(*plan)
+
+
+def _new_plan(queue, shape, groups):
+    new = lambda s: empty(s, np.int32, queue=queue)  # noqa: E731
+    return RowGroups(new((_size(shape),)), new(shape), new((groups + 1,)))
+
+
+def _whole_plan(results, count, groups):
+    """Addresses of order, place and offsets of a plan that is to be written."""
+    return (_int32_arg(results[0], "order", count), _int32_arg(results[1], "place", count),
+            _int32_arg(results[2], "offsets", groups + 1))
 
 
 def dispatch_rows(x, ids, groups=None, out=None, plan=None, queue=None):
@@ -547,28 +551,21 @@ def dispatch_rows(x, ids, groups=None, out=None, plan=None, queue=None):
         raise TypeError("out must have the type of x")
     dst = _rows_arg(o, "out")
     if not sorted_already:
+        index, groups = _index_arg(i, "ids"), int(groups)
+        if groups < 0:
+            raise ValueError("a negative number of groups")
+        if plan is None:
+            plan = _new_plan(on.queue, i.shape, groups)
+            results = [_operand(a, n) for a, n in zip(plan, RowGroups._fields)]
+        order, place, offsets = _whole_plan(results, index.count, groups)
         _no_overlap([o] + results, [r, i])
-        plan = _group(_Quiet(on), i, groups, plan, results)
-        results = results or [_operand(a, n) for a, n in zip(plan, RowGroups._fields)]
-    else:
-        _no_overlap([o], [r] + results)
+        on.done(_rt.load()._mlir_ciface_nmb_sort_dispatch_rows_device(
+            on.queue.handle, _ref(src), _ref(index), groups, order, place, offsets, None, 0, _ref(dst)))
+        return out, RowGroups(*plan)
+    _no_overlap([o], [r] + results)
     place, kept = _plan_args(results)
     on.done(_rt.load()._mlir_ciface_nmb_dispatch_rows_device(on.queue.handle, _ref(src), k, place, kept, _ref(dst)))
     return out, plan
-
-
-class _Quiet:
-    """`on` for the first step of a call: errors are raised, streams of other
-    arrays wait only for the last step."""
-
-    __slots__ = ("queue", "on")
-
-    def __init__(self, on):
-        self.queue, self.on = on.queue, on
-
-    def done(self, failed):
-        if failed:
-            self.on.done(failed)
 
 
 def _choices(rows, entries, name):

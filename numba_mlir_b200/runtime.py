@@ -106,6 +106,7 @@ SIGNATURES = {
     "_mlir_ciface_nmb_group_rows_workspace": (_sz, [_i64, _i64]),
     "_mlir_ciface_nmb_group_rows_device": (_i, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz]),
     "_mlir_ciface_nmb_dispatch_rows_device": (_i, [_vp, _vp, _i64, _vp, _vp, _vp]),
+    "_mlir_ciface_nmb_sort_dispatch_rows_device": (_i, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "_mlir_ciface_nmb_combine_rows_device": (_i, [_vp, _vp, _i64, _vp, _vp, _vp, _i, _vp]),
     "_mlir_ciface_nmb_combine_rows_grad_device": (_i, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i, _vp, _vp]),
     "gpuxMemcpy": (_vp, [_vp, _vp, _vp, _sz, _i, _vp]),

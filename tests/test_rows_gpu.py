@@ -281,7 +281,7 @@ def test_group_rows_edges(queue):
 
 # --------------------------------------------------------------- dispatch ---
 ROUTES = [(1, 1, 1, 1, 0), (4, 8, 64, 2048, 0), (33, 3, 17, 1001, 0), (100, 2, 8, 40, 8), (3000, 6, 60, 24, 0),
-          (257, 10, 300, 7, 1), (2000, 8, 128, 130, 2)]
+          (257, 10, 300, 7, 1), (2000, 8, 128, 130, 2), (1, 8, 1024, 16, 0), (3, 2, 1025, 5, 0), (512, 8, 1000, 9, 0), (585, 7, 64, 33, 0)]
 
 
 def route(tokens, k, groups, rng, drop=0.1):
