@@ -9,7 +9,7 @@
 // the equal digits of its warp's 32 comes from votes over the warp.
 //
 // What it costs is latency, not bandwidth (an entry is 8 bytes), so the number
-// of dependent steps is what the three forms differ in.  Up to 4096 entries
+// of dependent steps is what the three forms differ in.  Up to 2048 entries
 // stay in one block's shared memory for all passes: one launch.  Up to about a
 // million take a launch that counts tiles of 1024 to 8192 entries and one a pass
 // that scatters them: each block adds up the counts of all blocks for itself (at
@@ -221,6 +221,7 @@ template <int PER>
 __global__ void __launch_bounds__(kThreads)
     nmb_sort_one(const Ids ids, int n, int bits, int passes, const Results res, const Clear clear,
                  const Fill fill) {
+  nmb::rows::let_next_begin();
   if (fill.run())
     return;
   extern __shared__ uint32_t smem[];
@@ -309,6 +310,7 @@ struct Pass {
 template <int PER>
 __global__ void __launch_bounds__(kThreads) nmb_sort_count(const Pass p, const Clear next, const Clear clear,
                                                             const Fill fill) {
+  nmb::rows::let_next_begin();
   if (fill.run())
     return;
   __shared__ uint32_t count[kBins / 2];
@@ -363,6 +365,7 @@ template <int PER>
 __global__ void __launch_bounds__(kThreads)
     nmb_sort_scatter(const Pass p, uint32_t *keysOut, int32_t *entriesOut, int32_t *place, int32_t *offsets,
                      const Fill fill) {
+  nmb::rows::let_next_begin();
   if (fill.run())
     return;
   extern __shared__ uint32_t smem[];
@@ -376,13 +379,14 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t begin = ((int64_t)blockIdx.x * kWarps + warp) * PER * 32 + lane;
   uint32_t key[PER], rank[PER];
   int32_t entry[PER];
+  dg.clear();
+  nmb::rows::wait_for_previous();
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     const int64_t i = begin + u * 32;
     key[u] = i < p.n ? p.key(i) : 0;
     entry[u] = i < p.n && p.entriesIn ? p.entriesIn[i] : (int32_t)i;
   }
-  dg.clear();
   // counts of all blocks: a thread adds up every share-th block for two digits,
   // sixteen loads in flight (one by one they took 15 of the kernel's 19 us at
   // 131072 entries: an L2 access costs about 700 cycles)
@@ -486,7 +490,7 @@ int bitsOf(int64_t groups) {
 
 size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-constexpr int64_t kOneMost = 4096;
+constexpr int64_t kOneMost = 2048;
 bool fitsOneBlock(int64_t n) { return n <= kOneMost; }
 
 // Entries per thread of the many blocks: the fewest that keep them at 148 at
@@ -569,9 +573,8 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
   if (passes > 1 && offsets && !keys)
     keys = reinterpret_cast<uint32_t *>(ws); // the sorted keys, wanted for the offsets below
   if (fitsOneBlock(n)) {
-    const int per = n <= kThreads ? 1 : n <= 2 * kThreads ? 2 : 4;
-    const bool ok = withPer(per, [&](auto P) {
-      constexpr int kPer = P.value < 4 ? P.value : 4;
+    const bool ok = withPer(n <= kThreads ? 1 : 2, [&](auto P) {
+      constexpr int kPer = P.value < 2 ? P.value : 2;
       static std::atomic<bool> ready[64];
       if (!nmb::rows::allowShared(who, nmb_sort_one<kPer>, oneBytes<kPer>(), ready, s.device))
         return false;
@@ -633,8 +636,8 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
             return false;
         }
         const Fill fill = takeRows(clearing, (int)blocks, &grid);
-        nmb_sort_scatter<P.value><<<grid, kThreads, kScatterBytes, s.stream>>>(
-            p, last ? keys : keyBuf[to], last ? order : entryBuf[to], last ? place : nullptr,
+        launchBehind(
+            nmb_sort_scatter<P.value>, grid, kThreads, kScatterBytes, s.stream, p, last ? keys : keyBuf[to], last ? order : entryBuf[to], last ? place : nullptr,
             passes == 1 ? offsets : nullptr, fill);
         if (!launched(who))
           return false;
@@ -664,16 +667,8 @@ GPUX_EXPORT int _mlir_ciface_nmb_group_rows_device(void *queue, const GPUXIndex 
                                                    int32_t *place, int32_t *offsets, void *workspace,
                                                    size_t workspaceBytes) {
   const char *who = "group_rows";
-  if (!nmb::rows::checkIndex(who, ids))
+  if (!nmb::rows::checkIndex(who, ids) || !nmb::rows::checkGroups(who, ids, groups, order, place, offsets))
     return 1;
-  if (groups < 0 || groups >= 0x7fffffff) {
-    nmb::setError("%s: the number of groups must be in 0 .. 2^31 - 2", who);
-    return 1;
-  }
-  if (!offsets || (ids->count > 0 && (!order || !place))) {
-    nmb::setError("%s: null result", who);
-    return 1;
-  }
   nmb::rows::Stream s(queue);
   if (!s.ok)
     return 1;

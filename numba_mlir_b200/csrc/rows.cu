@@ -616,6 +616,7 @@ __global__ void __launch_bounds__(kThreads, 4)
   __shared__ uint32_t words[kThreads / 64 + 1];
   __shared__ Turns turns;
   const Group<BULK> group(p.lane_bits);
+  nmb::rows::wait_for_previous(); // the sort
 
   // every `period`-th block takes a chunk as long as there are any: blocks that
   // clear are writes alone, the others mostly wait for reads
@@ -749,6 +750,7 @@ __global__ void __launch_bounds__(kThreads)
                       int64_t out_rows, int64_t out_stride, int64_t vecs, int lane_bits) {
   const int lane = threadIdx.x & ((1 << lane_bits) - 1);
   const int64_t t = (int64_t)blockIdx.x * (kThreads >> lane_bits) + (threadIdx.x >> lane_bits);
+  nmb::rows::wait_for_previous();
   if (t >= tokens)
     return;
   const int64_t live = *kept;
@@ -1398,9 +1400,9 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
                         bits,
                         nmb::statusWordOrNull(queue)};
     auto go = [&](auto kernel, int threads, size_t shared) {
-      kernel<<<(unsigned)blocks, threads, shared, s.stream>>>(static_cast<const I *>(dout->data), dout->stride, plan,
-                                                              (typename Acc<I>::type)scale,
-                                                              static_cast<O *>(out->data), out->rows, out->stride, vecs);
+      nmb::rows::launchBehind(kernel, (unsigned)blocks, (unsigned)threads, shared, s.stream,
+                              static_cast<const I *>(dout->data), dout->stride, plan, (typename Acc<I>::type)scale,
+                              static_cast<O *>(out->data), out->rows, out->stride, vecs);
       ok = launched(who);
     };
     if (bulk) {
@@ -1438,25 +1440,38 @@ template <typename F> void withCopy(const GPUXRows *x, const GPUXRows *out, F &&
 }
 } // namespace
 
+namespace {
+// `behind`: right behind the sort that makes the places.
+int dispatchRows(const Stream &s, const GPUXRows *x, int64_t k, const int32_t *place, const int32_t *kept,
+                 const GPUXRows *out, bool behind) {
+  if (x->rows == 0 || x->cols == 0 || k == 0 || out->rows == 0)
+    return 0;
+  withCopy(x, out, [&](auto u, auto V, int64_t vecs) {
+    using U = decltype(u);
+    const int bits = laneBits(vecs, kThreadBits);
+    const auto kernel = nmb_dispatch_rows<U, V.value>;
+    const unsigned blocks = blocksFor(x->rows, bits);
+    const U *from = static_cast<const U *>(x->data);
+    U *to = static_cast<U *>(out->data);
+    if (behind)
+      nmb::rows::launchBehind(kernel, blocks, kThreads, 0, s.stream, from, x->rows, x->stride, k, place, kept, to,
+                              out->rows, out->stride, vecs, bits);
+    else
+      kernel<<<blocks, kThreads, 0, s.stream>>>(from, x->rows, x->stride, k, place, kept, to, out->rows, out->stride,
+                                                vecs, bits);
+  });
+  return launched("dispatch_rows") ? 0 : 1;
+}
+} // namespace
+
 GPUX_EXPORT int _mlir_ciface_nmb_dispatch_rows_device(void *queue, const GPUXRows *x, int64_t k, const int32_t *place,
                                                       const int32_t *kept, const GPUXRows *out) {
   const char *who = "dispatch_rows";
   if (!checkRows(who, "x", x, false) || !checkRows(who, "out", out, true) || !sameType(who, x, out) ||
       !sameWidth(who, x, out) || !checkPlaces(who, x->rows, k, place, kept) || !gridFits(who, x->rows))
     return 1;
-  if (x->rows == 0 || x->cols == 0 || k == 0 || out->rows == 0)
-    return 0;
   Stream s(queue);
-  if (!s.ok)
-    return 1;
-  withCopy(x, out, [&](auto u, auto V, int64_t vecs) {
-    using U = decltype(u);
-    const int bits = laneBits(vecs, kThreadBits);
-    nmb_dispatch_rows<U, V.value><<<blocksFor(x->rows, bits), kThreads, 0, s.stream>>>(
-        static_cast<const U *>(x->data), x->rows, x->stride, k, place, kept, static_cast<U *>(out->data), out->rows,
-        out->stride, vecs, bits);
-  });
-  return launched(who) ? 0 : 1;
+  return s.ok ? dispatchRows(s, x, k, place, kept, out, false) : 1;
 }
 
 GPUX_EXPORT int _mlir_ciface_nmb_sort_dispatch_rows_device(void *queue, const GPUXRows *x, const GPUXIndex *ids,
@@ -1473,8 +1488,9 @@ GPUX_EXPORT int _mlir_ciface_nmb_sort_dispatch_rows_device(void *queue, const GP
                   (long long)x->rows);
     return 1;
   }
-  if (ids->count > 0 && ids->count <= kCountEntries && groups >= 0 && groups <= kCountGroups && order && place &&
-      offsets && x->cols > 0) {
+  if (!nmb::rows::checkGroups(who, ids, groups, order, place, offsets))
+    return 1;
+  if (ids->count > 0 && ids->count <= kCountEntries && groups <= kCountGroups && x->cols > 0) {
     Stream s(queue);
     if (!s.ok)
       return 1;
@@ -1486,9 +1502,14 @@ GPUX_EXPORT int _mlir_ciface_nmb_sort_dispatch_rows_device(void *queue, const GP
     });
     return launched(who) ? 0 : 1;
   }
-  if (_mlir_ciface_nmb_group_rows_device(queue, ids, groups, order, place, offsets, workspace, workspaceBytes))
+  Stream s(queue);
+  if (!s.ok)
     return 1;
-  return _mlir_ciface_nmb_dispatch_rows_device(queue, x, k, place, offsets + groups, out);
+  nmb::rows::Workspace ws(s, who, workspace, workspaceBytes, nmb::rows::sortBytes(ids->count, groups));
+  if (!ws.ok || !nmb::rows::sortByKey(s, who, *ids, groups, order, nullptr, place, offsets, ws.data))
+    return 1;
+  // groups of several passes end with a kernel that lets nothing begin early
+  return dispatchRows(s, x, k, place, offsets + groups, out, ids->count > 0);
 }
 
 GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows *ys, int64_t k, const int32_t *place,

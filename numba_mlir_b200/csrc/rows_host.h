@@ -104,6 +104,31 @@ inline bool launched(const char *who) {
   return true;
 }
 
+// Launches a kernel that may begin while the kernel before it in the stream, one
+// of the same call, is still running (it calls let_next_begin): its blocks are
+// set up and then wait in wait_for_previous before they read what that kernel
+// and those before it write.
+template <typename K, typename... Args>
+inline void launchBehind(K kernel, unsigned grid, unsigned threads, size_t shared, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = shared;
+  config.stream = stream;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  (void)cudaLaunchKernelEx(&config, kernel, args...);
+}
+#ifdef __CUDACC__
+// A kernel completes only when the one before it has, since each that is
+// launched behind another waits for it: so a wait covers all kernels before.
+__device__ __forceinline__ void let_next_begin() { cudaTriggerProgrammaticLaunchCompletion(); }
+__device__ __forceinline__ void wait_for_previous() { cudaGridDependencySynchronize(); }
+#endif
+
 // Lets a kernel use more than 48 KB of shared memory; once per kernel and device.
 template <typename K> inline bool allowShared(const char *who, K kernel, int bytes, std::atomic<bool> *ready, int device) {
   if (device >= 0 && device < 64 && ready[device])
@@ -154,6 +179,19 @@ inline bool checkIndex(const char *who, const GPUXIndex *ids) {
   }
   if (ids->count >= (int64_t(1) << 31)) {
     setError("%s: 2^31 indices or more", who);
+    return false;
+  }
+  return true;
+}
+
+inline bool checkGroups(const char *who, const GPUXIndex *ids, int64_t groups, const int32_t *order,
+                        const int32_t *place, const int32_t *offsets) {
+  if (groups < 0 || groups >= 0x7fffffff) {
+    setError("%s: the number of groups must be in 0 .. 2^31 - 2", who);
+    return false;
+  }
+  if (!offsets || (ids->count > 0 && (!order || !place))) {
+    setError("%s: null result", who);
     return false;
   }
   return true;

@@ -151,6 +151,12 @@ def test_c_entries_refuse(runtime_lib):
     refused("groups", group, _index(B, 3), -1, C, C, C, None, 0)
     refused("groups", group, _index(B, 3), 2**31 - 1, C, C, C, None, 0)
     refused("null result", group, _index(B, 3), 4, None, C, C, None, 0)
+    sdisp = lib._mlir_ciface_nmb_sort_dispatch_rows_device
+    refused("for 5 tokens", sdisp, _rows(A, 5, 8), _index(B, 9), 4, C, C, C, None, 0, _rows(C, 10, 8))
+    refused("for 5 tokens", sdisp, _rows(A, 5, 8), _index(B, 10), 4, C, C, C, None, 0, _rows(C, 9, 8))
+    refused("for 0 tokens", sdisp, _rows(A, 0, 8), _index(B, 1), 4, C, C, C, None, 0, _rows(C, 9, 8))
+    refused("groups", sdisp, _rows(A, 5, 8), _index(B, 10), -1, C, C, C, None, 0, _rows(C, 10, 8))
+    refused("null result", sdisp, _rows(A, 5, 8), _index(B, 10), 4, C, None, C, None, 0, _rows(C, 10, 8))
     refused("different types", disp, _rows(A, 5, 8), 2, B, B, _rows(C, 10, 8, kind=2))
     refused("below 2", disp, _rows(A, 2**30, 8), 2, B, B, _rows(C, 2**31 - 1, 8))
     refused("null positions", disp, _rows(A, 5, 8), 2, None, B, _rows(C, 10, 8))
