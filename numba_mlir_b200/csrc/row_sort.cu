@@ -101,10 +101,15 @@ struct Fill {
   int64_t per_row, stride;
   int unit;
   int first;
+  int head, tail;      // bytes before and behind, where rows follow one another
   __device__ __forceinline__ bool run() const {
     if ((int)blockIdx.x < first)
       return false;
     const int64_t per_block = kFillBytes / unit;
+    if ((int)blockIdx.x == first && (int)threadIdx.x * 2 < head + tail) {
+      const int at = (int)threadIdx.x * 2;
+      *reinterpret_cast<short *>(at < head ? data - head + at : data + accesses * unit + (at - head)) = 0;
+    }
     const int64_t begin = (int64_t)(blockIdx.x - first) * per_block, end = min(begin + per_block, accesses);
     for (int64_t i = begin + threadIdx.x; i < end; i += blockDim.x) {
       // rows that follow one another are one long row
@@ -517,15 +522,25 @@ constexpr int64_t kFillMost = 48 << 20;
 Fill takeRows(nmb::rows::Clearing *c, int first, unsigned *blocks) {
   *blocks = (unsigned)first;
   if (!c || c->left == 0 || c->rowBytes == 0)
-    return Fill{nullptr, 0, 1, 0, 16, first};
+    return Fill{nullptr, 0, 1, 0, 16, first, 0, 0};
   int64_t rows = kFillMost / c->rowBytes;
   rows = rows < 1 ? 1 : rows < c->left ? rows : c->left;
   c->left -= rows;
-  const int64_t perRow = c->rowBytes / c->unit, accesses = rows * perRow;
-  const int64_t perBlock = kFillBytes / c->unit;
-  *blocks += (unsigned)((accesses + perBlock - 1) / perBlock);
-  return Fill{c->data + c->left * c->stride, accesses, c->stride == c->rowBytes ? accesses : perRow, c->stride,
-              c->unit, first};
+  unsigned char *data = c->data + c->left * c->stride;
+  Fill fill{data, rows * (c->rowBytes / c->unit), c->rowBytes / c->unit, c->stride, c->unit, first, 0, 0};
+  if (c->stride == c->rowBytes) {
+    // one long row: 16-byte stores whatever the rows' own boundaries
+    const int64_t bytes = rows * c->rowBytes;
+    const int64_t head = (int64_t)(-reinterpret_cast<intptr_t>(data) & 15);
+    fill.head = (int)(head < bytes ? head : bytes);
+    fill.data = data + fill.head;
+    fill.unit = 16;
+    fill.accesses = fill.per_row = (bytes - fill.head) / 16;
+    fill.tail = (int)((bytes - fill.head) % 16);
+  }
+  const int64_t perBlock = kFillBytes / fill.unit, fillBlocks = (fill.accesses + perBlock - 1) / perBlock;
+  *blocks += (unsigned)(fillBlocks > 0 ? fillBlocks : 1);
+  return fill;
 }
 
 // Calls f(constant) for 1, 2, 4 or 8.

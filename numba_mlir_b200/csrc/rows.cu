@@ -171,6 +171,49 @@ __device__ __forceinline__ bool bulk_arrived(uint64_t *bar, uint32_t phase, uint
   return false;
 }
 
+// A row's way into shared memory, issued by one thread: a bulk copy starts and
+// ends on 16-byte boundaries.  LOOSE rows do not: the words they lie in are copied
+// as a whole, neighbours' elements included, as far as the operand's memory
+// reaches; elements in the words at its very ends are copied one by one.  Returns
+// the place of the row's first element in `to`.
+template <typename T> struct Bounds {
+  const T *lo, *hi; // the operand's memory
+};
+template <bool LOOSE, typename T>
+__device__ __forceinline__ int fetch_row(const T *from, int count, unsigned char *to, uint64_t *bar,
+                                         const Bounds<T> &m) {
+  if constexpr (!LOOSE) {
+    nmb::mbar_expect_tx(bar, (uint32_t)count * (uint32_t)sizeof(T));
+    nmb::bulk_load(to, from, (uint32_t)count * (uint32_t)sizeof(T), bar);
+    return 0;
+  } else {
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(from), end = begin + (uintptr_t)count * sizeof(T);
+    const uintptr_t base = begin & ~uintptr_t(15);
+    uintptr_t a = base, b = (end + 15) & ~uintptr_t(15);
+    if (a < reinterpret_cast<uintptr_t>(m.lo))
+      a += 16;
+    if (b > reinterpret_cast<uintptr_t>(m.hi))
+      b -= 16;
+    for (uintptr_t p = begin; p < min(a, end); p += sizeof(T))
+      *reinterpret_cast<T *>(to + (p - base)) = *reinterpret_cast<const T *>(p);
+    for (uintptr_t p = max(max(a, b), begin); p < end; p += sizeof(T))
+      *reinterpret_cast<T *>(to + (p - base)) = *reinterpret_cast<const T *>(p);
+    if (b > a) {
+      nmb::mbar_expect_tx(bar, (uint32_t)(b - a));
+      nmb::bulk_load(to + (a - base), reinterpret_cast<const void *>(a), (uint32_t)(b - a), bar);
+    } else {
+      nmb::mbar_arrive(bar);
+    }
+    return (int)((begin - base) / sizeof(T));
+  }
+}
+// Bytes of shared memory for a row of `count` elements.
+template <bool LOOSE, typename T> __host__ __device__ __forceinline__ int fetched_bytes(int count) {
+  return ((int)sizeof(T) * count + 15) / 16 * 16 + (LOOSE ? 16 : 0);
+}
+// Elements per access of a row in shared memory.
+template <bool LOOSE, typename T> constexpr int kBulkElems = LOOSE ? 1 : 16 / (int)sizeof(T);
+
 // ------------------------------------------------------------------- take ---
 // A thread has up to four accesses of a row in flight.
 constexpr int kTakeBatch = 4;
@@ -214,55 +257,55 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kTakeThreads = 128;
 constexpr int kTakeRows = 16;          // most rows of a block
 constexpr int kTakeBytes = 8192;       // most bytes in flight per block
-constexpr int64_t kTakeBulkLeast = 8 << 20; // bytes from which on it pays
+constexpr int64_t kTakeBulkLeast = 8 << 20, kTakeLooseLeast = 1 << 20; // bytes from which on it pays
 
-template <typename I, typename O>
+template <typename I, typename O, bool LOOSE>
 __global__ void __launch_bounds__(kTakeThreads)
     nmb_take_rows_bulk(const I *__restrict__ table, int64_t rows, int64_t stride, const void *__restrict__ ids,
                        int id_bytes, int64_t n, typename Acc<I>::type scale, O *__restrict__ out, int64_t out_stride,
-                       int64_t vecs, int slab_vecs, int each, uint32_t *status) {
+                       int64_t cols, int slab, int each, const Bounds<I> bounds, uint32_t *status) {
   using A = typename Acc<I>::type;
-  constexpr int V = 16 / (int)sizeof(I);
-  extern __shared__ __align__(128) unsigned char memory[]; // [each][slab_vecs] accesses
+  constexpr int V = kBulkElems<LOOSE, I>;
+  extern __shared__ __align__(128) unsigned char memory[]; // [each] rows
   __shared__ uint64_t bar;
-  __shared__ bool inside[kTakeRows];
-  const int64_t i0 = (int64_t)blockIdx.x * each, first = (int64_t)blockIdx.y * slab_vecs;
-  const int here = (int)min((int64_t)slab_vecs, vecs - first), r = threadIdx.x;
-  int64_t id = -1;
-  if (r < each) {
-    id = i0 + r < n ? index_at(ids, id_bytes, i0 + r) : -1;
-    id = id < rows ? id : -1;
-    inside[r] = id >= 0;
-  }
+  __shared__ int at[kTakeRows]; // first element, -1: a row of zeros
+  const int64_t i0 = (int64_t)blockIdx.x * each, first = (int64_t)blockIdx.y * slab;
+  const int here = (int)min((int64_t)slab, cols - first), r = threadIdx.x, bytes = fetched_bytes<LOOSE, I>(slab);
   if (r == 0) {
     nmb::mbar_init(&bar, (uint32_t)each);
     nmb::mbar_init_fence();
   }
   __syncthreads();
   if (r < each) {
-    if (id >= 0) {
-      nmb::mbar_expect_tx(&bar, (uint32_t)here * 16);
-      nmb::bulk_load(memory + (int64_t)r * slab_vecs * 16, table + id * stride + first * V, (uint32_t)here * 16, &bar);
-    } else {
+    const int64_t id = i0 + r < n ? index_at(ids, id_bytes, i0 + r) : -1;
+    at[r] = -1;
+    if (id >= 0 && id < rows)
+      at[r] = fetch_row<LOOSE>(table + id * stride + first, here, memory + r * bytes, &bar, bounds);
+    else
       nmb::mbar_arrive(&bar);
-    }
   }
+  __syncthreads(); // `at` is written behind the arrivals
   if (!bulk_arrived(&bar, 0, status))
     return;
   const int live = (int)min((int64_t)each, n - i0);
-  O *dst = out + i0 * out_stride + first * V;
+  O *dst = out + i0 * out_stride + first;
   for (int j = 0; j < live; ++j, dst += out_stride) {
-    const I *src = reinterpret_cast<const I *>(memory) + (int64_t)j * slab_vecs * V;
+    const int begin = at[j];
+    const I *src = reinterpret_cast<const I *>(memory + j * bytes) + max(begin, 0);
 #pragma unroll 4
-    for (int col = r; col < here; col += kTakeThreads) {
-      Pack<O, V> y{};
-      if (inside[j]) {
-        const Pack<I, V> x = load<I, V>(src + col * V);
+    for (int col = r * V; col < here; col += kTakeThreads * V) {
+      if constexpr (LOOSE) {
+        dst[col] = down<O, A>(begin < 0 ? A(0) : up(src[col]) * scale);
+      } else {
+        Pack<O, V> y{};
+        if (begin >= 0) {
+          const Pack<I, V> x = load<I, V>(src + col);
 #pragma unroll
-        for (int e = 0; e < V / 2; ++e)
-          down2(y.v + 2 * e, mul2(scale, up2(x.v + 2 * e)));
+          for (int e = 0; e < V / 2; ++e)
+            down2(y.v + 2 * e, mul2(scale, up2(x.v + 2 * e)));
+        }
+        store<O, V>(dst + col, y);
       }
-      store<O, V>(dst + col * V, y);
     }
   }
 }
@@ -307,7 +350,7 @@ struct GradPlan {
   int64_t n;
   int span;
   unsigned slabs;          // groups side by side over the columns
-  int slab_vecs;           // accesses of a slab
+  int slab;                // elements of a slab
   unsigned chunk_blocks;   // blocks over chunks
   unsigned period;         // one block of so many takes a chunk
   void *partials;          // [chunks][cols]
@@ -426,22 +469,36 @@ template <typename A, int V> struct Sums {
 };
 
 // A thread's columns of the result.
-template <typename O, int V, bool ADD, typename A> struct GradColumn {
+// V neighbouring ones, or, LOOSE, every step-th one.
+template <typename O, int V, bool ADD, bool LOOSE, typename A> struct GradColumn {
   O *out;          // the thread's first column of row 0
   int64_t stride;
   A scale;
   bool active;     // threads without columns go along for the barriers
+  int live, step;  // LOOSE: how many columns, how far apart
   __device__ __forceinline__ Pack<O, V> old(uint32_t row) const {
     Pack<O, V> v{};
-    if (ADD && active)
+    if constexpr (ADD && LOOSE) {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < live)
+          v.v[e] = out[(int64_t)row * stride + e * step];
+    } else if (ADD && active) {
       v = load<O, V>(out + (int64_t)row * stride);
+    }
     return v;
   }
   // A run's row: scale * sum, or that added to what the row holds.
   __device__ __forceinline__ void write(uint32_t row, const Sums<A, V> &sum, const Pack<O, V> &old) const {
     const Pack<O, V> y = sum.template result<ADD, O>(scale, old);
-    if (active)
+    if constexpr (LOOSE) {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < live)
+          out[(int64_t)row * stride + e * step] = y.v[e];
+    } else if (active) {
       store<O, V>(out + (int64_t)row * stride, y);
+    }
   }
 };
 
@@ -458,9 +515,9 @@ struct Walk {
 // Adds up one after another the rows of a batch of N entries, writing a run's
 // row when the next begins.  Where the results are added to, the rows to be
 // written are read for the whole batch first.
-template <bool WHOLE, int N, typename I, typename O, int V, bool ADD, typename A>
+template <bool WHOLE, int N, typename I, typename O, int V, bool ADD, bool LOOSE, typename A>
 __device__ __forceinline__ void add_rows(const Pack<I, V> (&x)[N], const uint32_t (&key)[N], int live,
-                                         const GradColumn<O, V, ADD, A> &column, uint32_t &row, Sums<A, V> &sum) {
+                                         const GradColumn<O, V, ADD, LOOSE, A> &column, uint32_t &row, Sums<A, V> &sum) {
   Pack<O, V> old[ADD ? N : 1] = {};
   if constexpr (ADD) {
 #pragma unroll
@@ -484,9 +541,9 @@ __device__ __forceinline__ void add_rows(const Pack<I, V> (&x)[N], const uint32_
 
 // Through registers: the indices of the next batch are read along with the rows
 // of this one.  The row and the sum of the last run stay behind.
-template <typename I, typename O, int V, bool ADD, typename A>
+template <typename I, typename O, int V, bool ADD, bool LOOSE, typename A>
 __device__ __forceinline__ void walk_registers(const I *__restrict__ src, int64_t stride, const GradPlan &p,
-                                               const Walk &w, const GradColumn<O, V, ADD, A> &column, uint32_t &row,
+                                               const Walk &w, const GradColumn<O, V, ADD, LOOSE, A> &column, uint32_t &row,
                                                Sums<A, V> &sum) {
   const int64_t count = w.count();
   int32_t at[kGradBatch] = {};
@@ -520,13 +577,15 @@ __device__ __forceinline__ void walk_registers(const I *__restrict__ src, int64_
 struct Turns {
   uint64_t bar[2];
   uint32_t key[2][kTurnRows];
+  int begin[2][kTurnRows];
 };
-template <typename I, typename O, int V, bool ADD, typename A>
-__device__ __forceinline__ bool walk_bulk(const I *__restrict__ src, int64_t stride, const GradPlan &p, const Walk &w,
-                                          int here, unsigned char *memory, Turns &turns,
-                                          const GradColumn<O, V, ADD, A> &column, uint32_t &row, Sums<A, V> &sum) {
+template <typename I, typename O, int V, bool ADD, bool LOOSE, typename A>
+__device__ __forceinline__ bool walk_bulk(const I *__restrict__ src, int64_t stride, const Bounds<I> &bounds,
+                                          const GradPlan &p, const Walk &w, int here, unsigned char *memory, Turns &turns,
+                                          const GradColumn<O, V, ADD, LOOSE, A> &column, uint32_t &row, Sums<A, V> &sum) {
   const int64_t count = w.count(), last = (count + kTurnRows - 1) / kTurnRows;
-  const int r = threadIdx.x, mine = (column.active ? r : 0) * V;
+  const int r = threadIdx.x, mine = LOOSE ? r : (column.active ? r : 0) * V;
+  const int bytes = fetched_bytes<LOOSE, I>(p.slab);
   if (r == 0) {
     nmb::mbar_init(&turns.bar[0], kTurnRows);
     nmb::mbar_init(&turns.bar[1], kTurnRows);
@@ -547,9 +606,8 @@ __device__ __forceinline__ bool walk_bulk(const I *__restrict__ src, int64_t str
     const int b = (int)(turn & 1);
     if (turn * kTurnRows + r < count) {
       turns.key[b][r] = key;
-      nmb::mbar_expect_tx(&turns.bar[b], (uint32_t)here * 16);
-      nmb::bulk_load(memory + (int64_t)(b * kTurnRows + r) * p.slab_vecs * 16, src + (int64_t)at * stride,
-                     (uint32_t)here * 16, &turns.bar[b]);
+      turns.begin[b][r] = fetch_row<LOOSE>(src + (int64_t)at * stride, here, memory + (b * kTurnRows + r) * bytes,
+                                           &turns.bar[b], bounds);
     } else {
       nmb::mbar_arrive(&turns.bar[b]);
     }
@@ -561,28 +619,37 @@ __device__ __forceinline__ bool walk_bulk(const I *__restrict__ src, int64_t str
   if (last > 1)
     fetch(1);
   look(2);
+  if (LOOSE)
+    __syncthreads(); // `begin` is written behind the arrivals
   for (int64_t turn = 0; turn < last; ++turn) {
     const int b = (int)(turn & 1);
     if (!bulk_arrived(&turns.bar[b], (uint32_t)(turn >> 1) & 1, p.status))
       return false;
     const int live = (int)min((int64_t)kTurnRows, count - turn * kTurnRows);
-    const I *from = reinterpret_cast<const I *>(memory) + (int64_t)(b * kTurnRows) * p.slab_vecs * V + mine;
     Pack<I, V> x[kTurnRows];
     uint32_t keys[kTurnRows];
+    auto take = [&](int u) {
+      keys[u] = turns.key[b][u];
+      const I *from = reinterpret_cast<const I *>(memory + (b * kTurnRows + u) * bytes) + mine;
+      if constexpr (LOOSE) {
+        from += turns.begin[b][u];
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          x[u].v[e] = e < column.live ? from[e * column.step] : I(0.0f);
+      } else {
+        x[u] = load<I, V>(from);
+      }
+    };
     if (live == kTurnRows) {
 #pragma unroll
-      for (int u = 0; u < kTurnRows; ++u) {
-        keys[u] = turns.key[b][u];
-        x[u] = load<I, V>(from + u * p.slab_vecs * V);
-      }
+      for (int u = 0; u < kTurnRows; ++u)
+        take(u);
       add_rows<true>(x, keys, live, column, row, sum);
     } else {
 #pragma unroll
       for (int u = 0; u < kTurnRows; ++u)
-        if (u < live) {
-          keys[u] = turns.key[b][u];
-          x[u] = load<I, V>(from + u * p.slab_vecs * V);
-        }
+        if (u < live)
+          take(u);
       add_rows<false>(x, keys, live, column, row, sum);
     }
     __syncthreads(); // the turn's memory is free again
@@ -590,29 +657,41 @@ __device__ __forceinline__ bool walk_bulk(const I *__restrict__ src, int64_t str
       fetch(turn + 2);
       look(turn + 3);
     }
+    if (LOOSE)
+      __syncthreads();
   }
   return true;
 }
 
 // Sum of `count` partial sums: at `first`, then at second, second + step, ...
-template <int V, typename A>
+template <bool LOOSE, int V, typename A, typename C>
 __device__ __forceinline__ void add_partials(const A *partials, int64_t width, int64_t first, int64_t count,
-                                             int64_t second, int64_t step, Sums<A, V> &sum) {
+                                             int64_t second, int64_t step, const C &column, Sums<A, V> &sum) {
   sum.clear();
 #pragma unroll 4
   for (int64_t i = 0; i < count; ++i) {
     const A *from = partials + (i == 0 ? first : second + (i - 1) * step) * width;
-    sum.add(load_l2<A, V>(from));
+    if constexpr (LOOSE) {
+      Pack<A, V> x{};
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < column.live)
+          x.v[e] = __ldcg(from + e * column.step);
+      sum.add(x);
+    } else {
+      sum.add(load_l2<A, V>(from));
+    }
   }
 }
 
-// BULK: the group is the block and V elements are 16 bytes of I.
-template <typename I, typename O, int V, bool ADD, bool BULK>
+// BULK: the group is the block and V elements are 16 bytes of I; LOOSE: a
+// thread's V columns are as many threads apart.
+template <typename I, typename O, int V, bool ADD, bool BULK, bool LOOSE>
 __global__ void __launch_bounds__(kThreads, 4)
     nmb_take_rows_grad(const I *__restrict__ dout, int64_t stride, const GradPlan p, typename Acc<I>::type scale, O *out,
-                       int64_t rows, int64_t out_stride, int64_t vecs) {
+                       int64_t rows, int64_t out_stride, int64_t cols, const Bounds<I> bounds) {
   using A = typename Acc<I>::type;
-  extern __shared__ __align__(128) unsigned char memory[]; // BULK: [2][kTurnRows][slab_vecs] accesses
+  extern __shared__ __align__(128) unsigned char memory[]; // BULK: [2][kTurnRows] rows
   __shared__ uint32_t words[kThreads / 64 + 1];
   __shared__ Turns turns;
   const Group<BULK> group(p.lane_bits);
@@ -644,17 +723,22 @@ __global__ void __launch_bounds__(kThreads, 4)
       zero.v[e] = down<O, A>(A(0));
     for (int r = group.number; r < kZeroRows; r += (int)blockDim.x / group.lanes)
       if (mask >> r & 1)
-        for (int64_t c = group.lane; c < vecs; c += group.lanes)
-          store<O, V>(out + (first + r) * out_stride + c * V, zero);
+        for (int64_t c = group.lane * (LOOSE ? 1 : V); c < cols; c += group.lanes * (LOOSE ? 1 : V)) {
+          if constexpr (LOOSE)
+            out[(first + r) * out_stride + c] = zero.v[0];
+          else
+            store<O, V>(out + (first + r) * out_stride + c, zero);
+        }
     return;
   }
 
   const unsigned slab = turn % p.slabs;
   const int64_t chunk = (int64_t)(turn / p.slabs) * (BULK ? 1 : kThreads >> p.lane_bits) + group.number;
-  const int64_t slab_first = (int64_t)slab * p.slab_vecs;
-  const int here = (int)min((int64_t)p.slab_vecs, vecs - slab_first);
-  const bool active = group.lane < here;
-  const int64_t col = slab_first + (active ? group.lane : 0);
+  const int64_t slab_first = (int64_t)slab * p.slab;
+  const int here = (int)min((int64_t)p.slab, cols - slab_first);
+  const bool active = group.lane * (LOOSE ? 1 : V) < here;
+  const int64_t col = slab_first + (active ? group.lane * (LOOSE ? 1 : V) : 0); // the thread's first
+  const int mine = LOOSE ? (here - group.lane + group.lanes - 1) / group.lanes : 0; // how many, when apart
   const int64_t begin = chunk * p.span;
   if (begin >= p.n)
     return;
@@ -664,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 4)
   const uint32_t next_key = end < p.n ? __ldg(p.keys + end) : 0xffffffffu;
   if (first_key >= rows)
     return;
-  const GradColumn<O, V, ADD, A> column{out + col * V, out_stride, scale, active};
+  const GradColumn<O, V, ADD, LOOSE, A> column{out + col, out_stride, scale, active, active ? mine : 0, group.lanes};
 
   int64_t owner = chunk, inner = 0; // where a long run began, its inner chunks
   Walk walk{begin, end, end, end};
@@ -691,10 +775,10 @@ __global__ void __launch_bounds__(kThreads, 4)
   Sums<A, V> sum;
   sum.clear();
   if constexpr (BULK) {
-    if (!walk_bulk<I, O, V, ADD>(dout + slab_first * V, stride, p, walk, here, memory, turns, column, row, sum))
+    if (!walk_bulk<I, O, V, ADD, LOOSE>(dout + slab_first, stride, bounds, p, walk, here, memory, turns, column, row, sum))
       return;
   } else {
-    walk_registers<I, O, V, ADD>(dout + col * V, stride, p, walk, column, row, sum);
+    walk_registers<I, O, V, ADD, LOOSE>(dout + col, stride, p, walk, column, row, sum);
   }
   if (inner == 0) {
     column.write(row, sum, column.old(row));
@@ -703,11 +787,17 @@ __global__ void __launch_bounds__(kThreads, 4)
 
   // A long run: leave the partial sum.  The last group of a bundle of chunks
   // adds its bundle's up, the last of those groups the bundles'.
-  A *partials = static_cast<A *>(p.partials) + col * V;
-  const int64_t width = vecs * V;
+  A *partials = static_cast<A *>(p.partials) + col;
   auto leave_and_draw = [&](int64_t slot, uint32_t *ticket) {
-    if (active)
-      store<A, V>(partials + slot * width, sum.values());
+    if constexpr (LOOSE) {
+      const Pack<A, V> v = sum.values();
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < column.live)
+          partials[slot * cols + e * column.step] = v.v[e];
+    } else if (active) {
+      store<A, V>(partials + slot * cols, sum.values());
+    }
     __threadfence();
     group.sync();
     const uint32_t drawn = group.first(group.lane == 0 ? atomicAdd(ticket + slab, 1u) : 0, words);
@@ -719,11 +809,11 @@ __global__ void __launch_bounds__(kThreads, 4)
   const int64_t bundles = last / kBundle - owner / kBundle + 1;
   if (leave_and_draw(chunk, p.tickets + first * p.slabs) != (uint32_t)(count - 1))
     return;
-  add_partials<V>(partials, width, first, count, first + 1, 1, sum);
+  add_partials<LOOSE>(partials, cols, first, count, first + 1, 1, column, sum);
   if (bundles > 1) {
     if (leave_and_draw(first, p.tickets + (p.chunks + owner) * p.slabs) != (uint32_t)(bundles - 1))
       return;
-    add_partials<V>(partials, width, owner, bundles, (owner / kBundle + 1) * kBundle, kBundle, sum);
+    add_partials<LOOSE>(partials, cols, owner, bundles, (owner / kBundle + 1) * kBundle, kBundle, column, sum);
   }
   column.write(row, sum, column.old(row));
 }
@@ -762,6 +852,41 @@ __global__ void __launch_bounds__(kThreads)
       if (at >= 0 && at < out_rows)
         store<U, V>(out + at * out_stride + c * V, at < live ? row : Pack<U, V>{});
     }
+  }
+}
+
+// Rows that are not aligned to 16 bytes: a token's row goes into shared memory by
+// a bulk copy, and from there element by element to its places.
+constexpr int kCopyThreads = 128, kCopyBytes = 8192;
+template <typename U>
+__global__ void __launch_bounds__(kCopyThreads)
+    nmb_dispatch_rows_bulk(const U *__restrict__ x, int64_t stride, int64_t k, const int32_t *__restrict__ place,
+                           const int32_t *__restrict__ kept, U *__restrict__ out, int64_t out_rows, int64_t out_stride,
+                           int64_t cols, int slab, const Bounds<U> bounds, uint32_t *status) {
+  extern __shared__ __align__(128) unsigned char memory[];
+  __shared__ uint64_t bar;
+  __shared__ int begin;
+  const int64_t t = blockIdx.x, first = (int64_t)blockIdx.y * slab;
+  const int here = (int)min((int64_t)slab, cols - first);
+  nmb::rows::wait_for_previous();
+  if (threadIdx.x == 0) {
+    nmb::mbar_init(&bar, 1);
+    nmb::mbar_init_fence();
+    begin = fetch_row<true>(x + t * stride + first, here, memory, &bar, bounds);
+  }
+  __syncthreads();
+  const int64_t live = __ldg(kept);
+  if (!bulk_arrived(&bar, 0, status))
+    return;
+  const U *row = reinterpret_cast<const U *>(memory) + begin;
+  for (int64_t j = 0; j < k; ++j) {
+    const int64_t at = __ldg(place + t * k + j);
+    if (at < 0 || at >= out_rows)
+      continue;
+    U *to = out + at * out_stride + first;
+#pragma unroll 4
+    for (int col = threadIdx.x; col < here; col += kCopyThreads)
+      to[col] = at < live ? row[col] : U(0);
   }
 }
 
@@ -878,28 +1003,27 @@ constexpr int kBulkBytes = 16384, kBulkGradBytes = 46080;
 // What the threads of a block share about a token's choices.
 template <typename A> struct BulkChoices {
   uint64_t bar;
-  int32_t at[kBulkChoices]; // -1: left out
+  int32_t at[kBulkChoices]; // where the row begins in shared memory, or where it goes; -1: left out
   A weight[kBulkChoices];
 };
 
-template <typename T>
+template <typename T, bool LOOSE>
 __global__ void __launch_bounds__(kBulkThreads)
     nmb_combine_rows_bulk(const T *__restrict__ ys, int64_t y_rows, int64_t stride, int k,
                           const int32_t *__restrict__ place, const int32_t *__restrict__ kept,
                           const void *__restrict__ weights, int weight_type, T *__restrict__ out, int64_t out_stride,
-                          int64_t vecs, int slab_vecs, uint32_t *status) {
+                          int64_t cols, int slab, const Bounds<T> bounds, uint32_t *status) {
   using A = typename Acc<T>::type;
-  constexpr int V = 16 / (int)sizeof(T);
-  extern __shared__ __align__(128) unsigned char rows[]; // [k][slab_vecs] accesses
+  constexpr int V = kBulkElems<LOOSE, T>;
+  extern __shared__ __align__(128) unsigned char rows[]; // [k] rows
   __shared__ BulkChoices<A> c;
-  const int64_t t = blockIdx.x, first = (int64_t)blockIdx.y * slab_vecs;
-  const int here = (int)min((int64_t)slab_vecs, vecs - first);
+  const int64_t t = blockIdx.x, first = (int64_t)blockIdx.y * slab;
+  const int here = (int)min((int64_t)slab, cols - first), bytes = fetched_bytes<LOOSE, T>(slab);
   const int j = threadIdx.x;
   int32_t at = -1;
   if (j < k) {
     at = __ldg(place + t * k + j);
     at = at < min((int64_t)__ldg(kept), y_rows) ? at : -1;
-    c.at[j] = at;
     c.weight[j] = weights ? scalar_at<A>(weights, weight_type, t * k + j) : A(1);
   }
   if (j == 0) {
@@ -908,21 +1032,22 @@ __global__ void __launch_bounds__(kBulkThreads)
   }
   __syncthreads();
   if (j < k) {
-    if (at >= 0) {
-      nmb::mbar_expect_tx(&c.bar, (uint32_t)here * 16);
-      nmb::bulk_load(rows + (int64_t)j * slab_vecs * 16, ys + at * stride + first * V, (uint32_t)here * 16, &c.bar);
-    } else {
+    c.at[j] = -1;
+    if (at >= 0)
+      c.at[j] = j * bytes + (int)sizeof(T) * fetch_row<LOOSE>(ys + at * stride + first, here, rows + j * bytes, &c.bar,
+                                                              bounds);
+    else
       nmb::mbar_arrive(&c.bar);
-    }
   }
+  __syncthreads();
   if (!bulk_arrived(&c.bar, 0, status))
     return;
-  for (int col = threadIdx.x; col < here; col += kBulkThreads) {
+  for (int col = threadIdx.x * V; col < here; col += kBulkThreads * V) {
     A sum[V] = {};
 #pragma unroll 4
     for (int i = 0; i < k; ++i)
       if (c.at[i] >= 0) {
-        const Pack<T, V> y = load<T, V>(reinterpret_cast<const T *>(rows) + ((int64_t)i * slab_vecs + col) * V);
+        const Pack<T, V> y = load<T, V>(reinterpret_cast<const T *>(rows + c.at[i]) + col);
 #pragma unroll
         for (int e = 0; e < V; ++e)
           sum[e] = madd(c.weight[i], up(y.v[e]), sum[e]);
@@ -931,19 +1056,21 @@ __global__ void __launch_bounds__(kBulkThreads)
 #pragma unroll
     for (int e = 0; e < V; ++e)
       r.v[e] = down<T, A>(sum[e]);
-    store<T, V>(out + t * out_stride + (first + col) * V, r);
+    store<T, V>(out + t * out_stride + first + col, r);
   }
 }
 
-// Accesses of a slab where `rows` rows share `most` bytes: equal shares of the
-// row in as few slabs as that allows.  0: not by bulk copies (rows that are
-// narrow or not aligned, too many choices).
-int bulkSlab(int64_t cols, int type, int v, int64_t choices, int rows, int most) {
-  const int64_t bytes = cols * elemBytes(type), vecs = bytes / 16;
-  if (v * elemBytes(type) != 16 || choices < 1 || choices > kBulkChoices || bytes < kBulkLeast)
+// Elements of a slab where `rows` rows share `most` bytes: equal shares of the
+// row in as few slabs as that allows.  0: not by bulk copies (narrow rows, too
+// many choices).
+int bulkSlab(int64_t cols, int type, bool loose, int64_t choices, int rows, int most) {
+  const int size = elemBytes(type), step = loose ? 1 : 16 / size;
+  if (choices < 1 || choices > kBulkChoices || cols * size < kBulkLeast)
     return 0;
-  const int64_t slabs = (vecs * rows * 16 + most - 1) / most;
-  return slabs <= 65535 ? (int)((vecs + slabs - 1) / slabs) : 0;
+  const int64_t room = most / rows - (loose ? 32 : 0); // bytes of a row
+  const int64_t slabs = (cols * size + room - 1) / room;
+  const int64_t slab = ((cols + slabs - 1) / slabs + step - 1) / step * step;
+  return slabs <= 65535 ? (int)slab : 0;
 }
 
 // ----------------------------------------------------------- combine_grad ---
@@ -1061,20 +1188,21 @@ __global__ void __launch_bounds__(kThreads, 4)
 
 // The same with the rows fetched by bulk copies, dout's first.  A block takes a
 // whole token; columns beyond a slab come in turns through the same memory.
-template <typename T>
+template <typename T, bool LOOSE>
 __global__ void __launch_bounds__(kBulkThreads)
     nmb_combine_rows_grad_bulk(const T *__restrict__ dout, int64_t stride, const T *__restrict__ ys, int64_t y_rows,
                                int64_t y_stride, int k, const int32_t *__restrict__ place,
                                const int32_t *__restrict__ kept, const void *__restrict__ weights, int weight_type,
-                               T *__restrict__ dys, int64_t dy_rows, int64_t dy_stride, void *dweights, int64_t vecs,
-                               int slab_vecs, uint32_t *status) {
+                               T *__restrict__ dys, int64_t dy_rows, int64_t dy_stride, void *dweights, int64_t cols,
+                               int slab, const Bounds<T> dbounds, const Bounds<T> ybounds, uint32_t *status) {
   using A = typename Acc<T>::type;
-  constexpr int V = 16 / (int)sizeof(T), kWarps = kBulkThreads / 32, kGradChoices = 8;
-  extern __shared__ __align__(128) unsigned char rows[]; // [1 + k][slab_vecs] accesses
+  constexpr int V = kBulkElems<LOOSE, T>, kWarps = kBulkThreads / 32, kGradChoices = 8, kPairs = V > 1 ? V / 2 : 1;
+  extern __shared__ __align__(128) unsigned char rows[]; // [1 + k] rows, dout's first
   __shared__ BulkChoices<A> c;
+  __shared__ int begin[kBulkChoices + 1]; // where each row's first element is
   __shared__ A parts[kWarps][kBulkChoices];
   const int64_t t = blockIdx.x;
-  const int j = threadIdx.x, lane = j & 31, warp = j >> 5;
+  const int j = threadIdx.x, lane = j & 31, warp = j >> 5, bytes = fetched_bytes<LOOSE, T>(slab);
   const int64_t live = min((int64_t)__ldg(kept), y_rows);
   int32_t at = -1;
   if (j < k) {
@@ -1090,49 +1218,63 @@ __global__ void __launch_bounds__(kBulkThreads)
     (&parts[0][0])[i] = A(0);
   __syncthreads();
   uint32_t phase = 0;
-  for (int64_t first = 0; first < vecs; first += slab_vecs, phase ^= 1) {
-    const int here = (int)min((int64_t)slab_vecs, vecs - first);
+  for (int64_t first = 0; first < cols; first += slab, phase ^= 1) {
+    const int here = (int)min((int64_t)slab, cols - first);
     if (j <= k) { // thread k fetches dout
-      const int64_t row = j < k ? at : t;
-      if (j == k || (at >= 0 && at < live)) {
-        nmb::mbar_expect_tx(&c.bar, (uint32_t)here * 16);
-        nmb::bulk_load(rows + (int64_t)(j < k ? j + 1 : 0) * slab_vecs * 16,
-                       (j < k ? ys + row * y_stride : dout + row * stride) + first * V, (uint32_t)here * 16, &c.bar);
-      } else {
+      unsigned char *to = rows + (j < k ? j + 1 : 0) * bytes;
+      if (j == k)
+        begin[0] = fetch_row<LOOSE>(dout + t * stride + first, here, to, &c.bar, dbounds);
+      else if (at >= 0 && at < live)
+        begin[j + 1] = fetch_row<LOOSE>(ys + at * y_stride + first, here, to, &c.bar, ybounds);
+      else
         nmb::mbar_arrive(&c.bar);
-      }
     }
+    if (LOOSE)
+      __syncthreads(); // `begin` is written behind the arrivals
     if (!bulk_arrived(&c.bar, phase, status))
       return; // every thread gives up by itself: no barrier is left waiting
-    const T *mem = reinterpret_cast<const T *>(rows);
+    const T *drow = reinterpret_cast<const T *>(rows) + (LOOSE ? begin[0] : 0);
     for (int j0 = 0; j0 < k; j0 += kGradChoices) {
       int32_t to[kGradChoices];
       A w[kGradChoices];
+      const T *yrow[kGradChoices];
       typename Two<A>::type dots[kGradChoices] = {};
 #pragma unroll
       for (int i = 0; i < kGradChoices; ++i) {
         to[i] = j0 + i < k ? c.at[j0 + i] : -1;
         w[i] = j0 + i < k ? c.weight[j0 + i] : A(0);
+        yrow[i] = reinterpret_cast<const T *>(rows + (j0 + i + 1) * bytes);
+        if (LOOSE && to[i] >= 0 && to[i] < live)
+          yrow[i] += begin[j0 + i + 1];
       }
-      for (int col = j; col < here; col += kBulkThreads) {
-        const Pack<T, V> x = load<T, V>(mem + (int64_t)col * V);
-        typename Two<A>::type d[V / 2];
+      for (int col = j * V; col < here; col += kBulkThreads * V) {
+        const Pack<T, V> x = load<T, V>(drow + col);
+        typename Two<A>::type d[kPairs];
 #pragma unroll
-        for (int e = 0; e < V / 2; ++e)
-          d[e] = up2(x.v + 2 * e);
+        for (int e = 0; e < kPairs; ++e) {
+          if constexpr (V > 1)
+            d[e] = up2(x.v + 2 * e);
+          else
+            d[e].x = up(x.v[0]);
+        }
 #pragma unroll
         for (int i = 0; i < kGradChoices; ++i)
           if (to[i] >= 0) {
             Pack<T, V> r{};
             if (to[i] < live) {
-              const Pack<T, V> y = load<T, V>(mem + ((int64_t)(j0 + i + 1) * slab_vecs + col) * V);
+              const Pack<T, V> y = load<T, V>(yrow[i] + col);
+              if constexpr (V > 1) {
 #pragma unroll
-              for (int e = 0; e < V / 2; ++e) {
-                dots[i] = madd2(d[e], up2(y.v + 2 * e), dots[i]);
-                down2(r.v + 2 * e, mul2(w[i], d[e]));
+                for (int e = 0; e < kPairs; ++e) {
+                  dots[i] = madd2(d[e], up2(y.v + 2 * e), dots[i]);
+                  down2(r.v + 2 * e, mul2(w[i], d[e]));
+                }
+              } else {
+                dots[i].x = madd(d[0].x, up(y.v[0]), dots[i].x);
+                r.v[0] = down<T, A>(w[i] * d[0].x);
               }
             }
-            store<T, V>(dys + to[i] * dy_stride + (first + col) * V, r);
+            store<T, V>(dys + to[i] * dy_stride + first + col, r);
           }
       }
       A dot[kGradChoices];
@@ -1182,6 +1324,13 @@ template <int MOST, typename F> void withElems(int v, F &&f) {
     if (v == 2)
       return f(std::integral_constant<int, 2>());
   f(std::integral_constant<int, 1>());
+}
+
+// The memory that rows lie in.
+template <typename T> Bounds<T> boundsOf(const GPUXRows *r) {
+  const T *data = static_cast<const T *>(r->data);
+  const int64_t far = r->rows > 1 ? (r->rows - 1) * r->stride : 0;
+  return {data + (far < 0 ? far : 0), data + (far > 0 ? far : 0) + r->cols};
 }
 
 template <typename F> void withType(int type, F &&f) {
@@ -1280,16 +1429,19 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_device(void *queue, const GPUXRows *t
     const int v = accessElems(out->cols, most, {table, out});
     const int64_t vecs = out->cols / v;
     const int64_t row_bytes = out->cols * (int64_t)sizeof(I);
-    if (v >= mostElems<I>() && row_bytes >= kBulkLeast && out->rows * row_bytes >= kTakeBulkLeast) {
+    const bool loose = v < mostElems<I>();
+    if (row_bytes >= kBulkLeast && out->rows * row_bytes >= (loose ? kTakeLooseLeast : kTakeBulkLeast)) {
       // equal slabs of a row that does not fit, several rows that do
-      const int64_t wide = row_bytes / 16, slabs = (row_bytes + kTakeBytes - 1) / kTakeBytes;
-      const int slab = (int)((wide + slabs - 1) / slabs);
-      const int fit = kTakeBytes / 16 / slab, each = fit < kTakeRows ? fit : kTakeRows;
+      const int64_t step = loose ? 1 : mostElems<I>(), slabs = (row_bytes + kTakeBytes - 1) / kTakeBytes;
+      const int slab = (int)(((out->cols + slabs - 1) / slabs + step - 1) / step * step);
+      const int bytes = loose ? fetched_bytes<true, I>(slab) : fetched_bytes<false, I>(slab);
+      const int fit = kTakeBytes / bytes, each = fit < 1 ? 1 : fit < kTakeRows ? fit : kTakeRows;
       if (slabs <= 65535) {
-        nmb_take_rows_bulk<I, O><<<dim3((unsigned)((out->rows + each - 1) / each), (unsigned)slabs), kTakeThreads,
-                                   (size_t)each * slab * 16, s.stream>>>(
-            static_cast<const I *>(table->data), table->rows, table->stride, ids->data, ids->bytes, ids->count,
-            (typename Acc<I>::type)scale, static_cast<O *>(out->data), out->stride, wide, slab, each, status);
+        const auto kernel = loose ? nmb_take_rows_bulk<I, O, true> : nmb_take_rows_bulk<I, O, false>;
+        kernel<<<dim3((unsigned)((out->rows + each - 1) / each), (unsigned)slabs), kTakeThreads, (size_t)each * bytes,
+                 s.stream>>>(static_cast<const I *>(table->data), table->rows, table->stride, ids->data, ids->bytes,
+                             ids->count, (typename Acc<I>::type)scale, static_cast<O *>(out->data), out->stride,
+                             out->cols, slab, each, boundsOf<I>(table), status);
         return;
       }
     }
@@ -1357,13 +1509,13 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
     using O = decltype(o);
     constexpr int wide = mostElems<I>();
     const int v = accessElems(out->cols, wide, {dout, out});
-    const bool bulk = v == wide && out->cols * (int64_t)sizeof(I) >= kBulkLeast;
-    const int64_t vecs = out->cols / v;
+    const bool bulk = out->cols * (int64_t)sizeof(I) >= kBulkLeast, loose = bulk && v < wide;
+    const int64_t vecs = bulk ? (out->cols + wide - 1) / wide : out->cols / v;
     const int bits = laneBits(vecs, kThreadBits);
     const int span = gradSpan(ids->count, vecs);
     const int64_t chunks = (ids->count + span - 1) / span;
     const unsigned slabs = (unsigned)((vecs + (int64_t(1) << bits) - 1) >> bits);
-    const int slabVecs = (int)((vecs + slabs - 1) / slabs);
+    const int slab = (int)((vecs + slabs - 1) / slabs) * (bulk ? wide : v);
     const unsigned chunkBlocks = bulk ? (unsigned)chunks : blocksFor(chunks, bits);
     const int64_t work = (int64_t)chunkBlocks * slabs;
     if (work + (out->rows + kZeroRows - 1) / kZeroRows >= (int64_t(1) << 31)) {
@@ -1376,7 +1528,8 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
     clearing.left = accumulate ? 0 : out->rows;
     clearing.rowBytes = out->cols * (int64_t)sizeof(O);
     clearing.stride = out->stride * (int64_t)sizeof(O);
-    clearing.unit = v * (int)sizeof(O) < 16 ? v * (int)sizeof(O) : 16;
+    const int alone = accessElems(out->cols, mostElems<O>(), {out}); // elements per access of the result by itself
+    clearing.unit = alone * (int)sizeof(O) < 16 ? alone * (int)sizeof(O) : 16;
     ok = nmb::rows::sortByKey(s, who, *ids, out->rows, order, keys, nullptr, nullptr,
                               ws + 2 * need.entries + need.tickets + need.partials, tickets, 2 * chunks * slabs,
                               &clearing);
@@ -1390,7 +1543,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
                         ids->count,
                         span,
                         slabs,
-                        slabVecs,
+                        slab,
                         chunkBlocks,
                         work > 0 ? (unsigned)(blocks / work) : 1,
                         partials,
@@ -1402,21 +1555,26 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
     auto go = [&](auto kernel, int threads, size_t shared) {
       nmb::rows::launchBehind(kernel, (unsigned)blocks, (unsigned)threads, shared, s.stream,
                               static_cast<const I *>(dout->data), dout->stride, plan, (typename Acc<I>::type)scale,
-                              static_cast<O *>(out->data), out->rows, out->stride, vecs);
+                              static_cast<O *>(out->data), out->rows, out->stride, out->cols, boundsOf<I>(dout));
       ok = launched(who);
     };
     if (bulk) {
-      const auto kernel =
-          accumulate ? nmb_take_rows_grad<I, O, wide, true, true> : nmb_take_rows_grad<I, O, wide, false, true>;
-      const size_t shared = (size_t)2 * kTurnRows * slabVecs * 16; // 64 KB at most
-      static std::atomic<bool> ready[2][64];
-      ok = nmb::rows::allowShared(who, kernel, 2 * kTurnRows * kThreads * 16, ready[accumulate ? 1 : 0], s.device);
-      if (ok)
-        go(kernel, (slabVecs + 31) / 32 * 32, shared);
+      auto launch = [&](auto LOOSE) {
+        constexpr bool kLoose = LOOSE.value;
+        const auto kernel = accumulate ? nmb_take_rows_grad<I, O, wide, true, true, kLoose>
+                                       : nmb_take_rows_grad<I, O, wide, false, true, kLoose>;
+        const size_t shared = (size_t)2 * kTurnRows * fetched_bytes<kLoose, I>(slab); // 33 KB at most
+        go(kernel, (slab / wide + 31) / 32 * 32, shared);
+      };
+      if (loose)
+        launch(std::true_type());
+      else
+        launch(std::false_type());
       return;
     }
     withElems<wide>(v, [&](auto V) {
-      go(accumulate ? nmb_take_rows_grad<I, O, V.value, true, false> : nmb_take_rows_grad<I, O, V.value, false, false>,
+      go(accumulate ? nmb_take_rows_grad<I, O, V.value, true, false, false>
+                    : nmb_take_rows_grad<I, O, V.value, false, false, false>,
          kThreads, 0);
     });
   });
@@ -1442,12 +1600,28 @@ template <typename F> void withCopy(const GPUXRows *x, const GPUXRows *out, F &&
 
 namespace {
 // `behind`: right behind the sort that makes the places.
-int dispatchRows(const Stream &s, const GPUXRows *x, int64_t k, const int32_t *place, const int32_t *kept,
+int dispatchRows(void *queue, const Stream &s, const GPUXRows *x, int64_t k, const int32_t *place, const int32_t *kept,
                  const GPUXRows *out, bool behind) {
   if (x->rows == 0 || x->cols == 0 || k == 0 || out->rows == 0)
     return 0;
+  uint32_t *status = nmb::statusWordOrNull(queue);
   withCopy(x, out, [&](auto u, auto V, int64_t vecs) {
     using U = decltype(u);
+    const int64_t slabs = (x->cols * (int64_t)sizeof(U) + kCopyBytes - 1) / kCopyBytes;
+    if (V.value < mostElems<U>() && x->cols * (int64_t)sizeof(U) >= kBulkLeast && slabs <= 65535) {
+      const int slab = (int)((x->cols + slabs - 1) / slabs);
+      const dim3 grid((unsigned)x->rows, (unsigned)slabs);
+      const size_t shared = (size_t)fetched_bytes<true, U>(slab);
+      const U *from = static_cast<const U *>(x->data);
+      U *to = static_cast<U *>(out->data);
+      if (behind)
+        nmb::rows::launchBehind(nmb_dispatch_rows_bulk<U>, grid, kCopyThreads, shared, s.stream, from, x->stride, k,
+                                place, kept, to, out->rows, out->stride, x->cols, slab, boundsOf<U>(x), status);
+      else
+        nmb_dispatch_rows_bulk<U><<<grid, kCopyThreads, shared, s.stream>>>(
+            from, x->stride, k, place, kept, to, out->rows, out->stride, x->cols, slab, boundsOf<U>(x), status);
+      return;
+    }
     const int bits = laneBits(vecs, kThreadBits);
     const auto kernel = nmb_dispatch_rows<U, V.value>;
     const unsigned blocks = blocksFor(x->rows, bits);
@@ -1471,7 +1645,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_dispatch_rows_device(void *queue, const GPUXRow
       !sameWidth(who, x, out) || !checkPlaces(who, x->rows, k, place, kept) || !gridFits(who, x->rows))
     return 1;
   Stream s(queue);
-  return s.ok ? dispatchRows(s, x, k, place, kept, out, false) : 1;
+  return s.ok ? dispatchRows(queue, s, x, k, place, kept, out, false) : 1;
 }
 
 GPUX_EXPORT int _mlir_ciface_nmb_sort_dispatch_rows_device(void *queue, const GPUXRows *x, const GPUXIndex *ids,
@@ -1509,7 +1683,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_sort_dispatch_rows_device(void *queue, const GP
   if (!ws.ok || !nmb::rows::sortByKey(s, who, *ids, groups, order, nullptr, place, offsets, ws.data))
     return 1;
   // groups of several passes end with a kernel that lets nothing begin early
-  return dispatchRows(s, x, k, place, offsets + groups, out, ids->count > 0);
+  return dispatchRows(queue, s, x, k, place, offsets + groups, out, ids->count > 0);
 }
 
 GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows *ys, int64_t k, const int32_t *place,
@@ -1531,11 +1705,13 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows
     const int v = accessElems(out->cols, mostElems<T>(), {ys, out});
     const int64_t vecs = out->cols / v;
     const int bits = laneBits(vecs, kThreadBits);
-    if (const int slab = bulkSlab(out->cols, out->type, v, k, (int)k, kBulkBytes)) {
-      nmb_combine_rows_bulk<T><<<dim3((unsigned)out->rows, (unsigned)((vecs + slab - 1) / slab)), kBulkThreads,
-                                 (size_t)k * slab * 16, s.stream>>>(
+    const bool loose = v < mostElems<T>();
+    if (const int slab = bulkSlab(out->cols, out->type, loose, k, (int)k, kBulkBytes)) {
+      const auto kernel = loose ? nmb_combine_rows_bulk<T, true> : nmb_combine_rows_bulk<T, false>;
+      const size_t shared = (size_t)k * (loose ? fetched_bytes<true, T>(slab) : fetched_bytes<false, T>(slab));
+      kernel<<<dim3((unsigned)out->rows, (unsigned)((out->cols + slab - 1) / slab)), kBulkThreads, shared, s.stream>>>(
           static_cast<const T *>(ys->data), ys->rows, ys->stride, (int)k, place, kept, weights, weightType,
-          static_cast<T *>(out->data), out->stride, vecs, slab, status);
+          static_cast<T *>(out->data), out->stride, out->cols, slab, boundsOf<T>(ys), status);
       return;
     }
     withElems<mostElems<T>()>(v, [&](auto V) {
@@ -1569,11 +1745,14 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_grad_device(void *queue, const GPU
     const int v = dout->cols ? accessElems(dout->cols, mostElems<T>(), {dout, ys, dys}) : 1;
     const int64_t vecs = dout->cols / v;
     const int bits = laneBits(vecs, kThreadBits);
-    if (const int slab = bulkSlab(dout->cols, dout->type, v, k, (int)k + 1, kBulkGradBytes)) {
-      nmb_combine_rows_grad_bulk<T><<<(unsigned)dout->rows, kBulkThreads, (size_t)(k + 1) * slab * 16, s.stream>>>(
+    const bool loose = v < mostElems<T>();
+    if (const int slab = bulkSlab(dout->cols, dout->type, loose, k, (int)k + 1, kBulkGradBytes)) {
+      const auto kernel = loose ? nmb_combine_rows_grad_bulk<T, true> : nmb_combine_rows_grad_bulk<T, false>;
+      const size_t shared = (size_t)(k + 1) * (loose ? fetched_bytes<true, T>(slab) : fetched_bytes<false, T>(slab));
+      kernel<<<(unsigned)dout->rows, kBulkThreads, shared, s.stream>>>(
           static_cast<const T *>(dout->data), dout->stride, static_cast<const T *>(ys->data), ys->rows, ys->stride,
           (int)k, place, kept, weights, weightType, static_cast<T *>(dys->data), dys->rows, dys->stride, dweights,
-          vecs, slab, status);
+          dout->cols, slab, boundsOf<T>(dout), boundsOf<T>(ys), status);
       return;
     }
     withElems<mostElems<T>()>(v, [&](auto V) {

@@ -109,9 +109,9 @@ inline bool launched(const char *who) {
 // set up and then wait in wait_for_previous before they read what that kernel
 // and those before it write.
 template <typename K, typename... Args>
-inline void launchBehind(K kernel, unsigned grid, unsigned threads, size_t shared, cudaStream_t stream, Args... args) {
+inline void launchBehind(K kernel, dim3 grid, unsigned threads, size_t shared, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(grid);
+  config.gridDim = grid;
   config.blockDim = dim3(threads);
   config.dynamicSmemBytes = shared;
   config.stream = stream;

@@ -89,7 +89,7 @@ def plan_on_device(ids, groups):
 
 # ------------------------------------------------------------------- take ---
 @pytest.mark.parametrize("name", TYPES)
-@pytest.mark.parametrize("rows,dim,shape,pad", [(1, 1, (1,), 0), (7, 3, (5,), 0), (50, 64, (4, 9), 8), (33, 1000, (77,), 0),
+@pytest.mark.parametrize("rows,dim,shape,pad", [(60, 2047, (33,), 0), (60, 259, (33,), 3), (60, 514, (4,), 1), (60, 33, (70,), 0), (1, 1, (1,), 0), (7, 3, (5,), 0), (50, 64, (4, 9), 8), (33, 1000, (77,), 0),
                                                 (100, 4096, (3,), 0), (20, 1025, (16,), 3), (300, 130, (2, 3, 11), 2)])
 def test_take_rows(queue, name, rows, dim, shape, pad):
     import numba_mlir_b200 as nm
@@ -167,7 +167,7 @@ def grad_bound(d, ids, rows, scale, u):
 @pytest.mark.parametrize("n,rows,dim,pad,kind", [
     (1, 1, 1, 0, "any"), (5, 3, 7, 0, "any"), (77, 1000, 64, 8, "any"), (300, 20, 130, 2, "any"), (31, 40, 4096, 0, "any"),
     (257, 9, 33, 0, "one"), (1000, 5, 24, 0, "one"), (1000, 300, 1001, 0, "few"), (2500, 70000, 16, 0, "few"),
-    (9000, 50, 8, 0, "any"), (20000, 3000, 12, 0, "few"), (9001, 2000000, 1, 0, "any"), (640, 100, 48, 0, "none")])
+    (300, 20, 131, 2, "any"), (700, 9, 1023, 0, "few"), (900, 400, 66, 1, "any"), (4000, 3, 35, 0, "any"), (2100, 4000, 263, 5, "any"), (9000, 50, 8, 0, "any"), (20000, 3000, 12, 0, "few"), (9001, 2000000, 1, 0, "any"), (640, 100, 48, 0, "none")])
 def test_take_rows_grad(queue, name, n, rows, dim, pad, kind):
     import numba_mlir_b200 as nm
 
@@ -281,7 +281,7 @@ def test_group_rows_edges(queue):
 
 # --------------------------------------------------------------- dispatch ---
 ROUTES = [(1, 1, 1, 1, 0), (4, 8, 64, 2048, 0), (33, 3, 17, 1001, 0), (100, 2, 8, 40, 8), (3000, 6, 60, 24, 0),
-          (257, 10, 300, 7, 1), (2000, 8, 128, 130, 2), (1, 8, 1024, 16, 0), (3, 2, 1025, 5, 0), (512, 8, 1000, 9, 0), (585, 7, 64, 33, 0)]
+          (257, 10, 300, 7, 1), (2000, 8, 128, 130, 2), (1, 8, 1024, 16, 0), (3, 2, 1025, 5, 0), (512, 8, 1000, 9, 0), (585, 7, 64, 33, 0), (40, 5, 9, 2047, 0), (1000, 6, 20, 262, 3), (90, 9, 20, 263, 1)]
 
 
 def route(tokens, k, groups, rng, drop=0.1):
