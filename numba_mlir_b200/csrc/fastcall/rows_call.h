@@ -43,7 +43,7 @@ inline PyObject *name(const char *text) { return PyUnicode_InternFromString(text
 struct Names {
   PyObject *dtype = name("dtype"), *shape = name("shape"), *strides = name("strides"), *stride = name("stride"),
            *addr = name("_addr"), *buf = name("_buf"), *queue = name("queue"), *data_ptr = name("data_ptr"),
-           *is_cuda = name("is_cuda"), *requires_grad = name("requires_grad"), *get_device = name("get_device"),
+           *requires_grad = name("requires_grad"), *get_device = name("get_device"),
            *handle = name("handle"), *device = name("device"), *raw = name("_raw_stream");
 };
 inline Names &names() {
@@ -194,10 +194,9 @@ inline bool read(PyObject *obj, Queue &q, Operand &op) {
            takeInts(PyObject_GetAttr(obj, n.shape), op.shape, op.nd, 1) &&
            takeInts(PyObject_GetAttr(obj, n.strides), op.stride, strides, op.item) && strides == op.nd;
   }
-  if (!gTensorType || !PyObject_TypeCheck(obj, (PyTypeObject *)gTensorType) || !isTrue(obj, n.is_cuda) ||
-      isTrue(obj, n.requires_grad))
+  if (!gTensorType || !PyObject_TypeCheck(obj, (PyTypeObject *)gTensorType) || isTrue(obj, n.requires_grad))
     return false;
-  int64_t device;
+  int64_t device; // -1 for a tensor that is not on a GPU
   if (!takeInt(PyObject_CallMethodNoArgs(obj, n.get_device), device) || device != q.device)
     return false;
   if (q.torchHere < 0) {

@@ -9,8 +9,8 @@
 // the equal digits of its warp's 32 comes from votes over the warp.
 //
 // What it costs is latency, not bandwidth (an entry is 8 bytes), so the number
-// of dependent steps is what the three forms differ in.  Up to 2048 entries
-// stay in one block's shared memory for all passes: one launch.  Up to about a
+// of dependent steps is what the three forms differ in.  Up to 2048 entries (4096
+// of many groups) are not sorted in passes at all: every position is counted.  Up to about a
 // million take a launch that counts tiles of 1024 to 8192 entries and one a pass
 // that scatters them: each block adds up the counts of all blocks for itself (at
 // most 148 of them), and counts its entries for the pass after it at the places
@@ -142,7 +142,7 @@ struct Digits {
       : counts(counts), parts(parts), bins(1 << bin_bits), bin_bits(bin_bits), shift(shift),
         warps((int)blockDim.x >> 5), part_bits(0) {
     // as many parts as there are threads for every digit
-    while ((warps + (1 << part_bits) - 1) >> part_bits > max((int)blockDim.x >> bin_bits, 1))
+    while ((warps + (1 << part_bits) - 1) >> part_bits > (int)blockDim.x >> bin_bits)
       ++part_bits;
   }
 
@@ -172,10 +172,9 @@ struct Digits {
     return before + __popc(lower);
   }
 
-  // Adds the warps' counts up, four at a time, and the parts'; every thread gets
-  // the sum over its digits [first, last).  Call behind a barrier, and place
-  // another before `rank` results are used.
-  __device__ __forceinline__ uint32_t add_up(int first, int last, uint32_t *totals) const {
+  // Adds the warps' counts up, four at a time, then the parts', for `before`.
+  // Between two barriers of the caller's.
+  __device__ __forceinline__ void add_up() const {
     const int count = (warps + (1 << part_bits) - 1) >> part_bits;
     for (int i = threadIdx.x; i < count * bins; i += blockDim.x) {
       const int d = i & (bins - 1), from = i >> bin_bits << part_bits, to = min(from + (1 << part_bits), warps);
@@ -195,8 +194,8 @@ struct Digits {
       parts[i] = sum;
     }
     __syncthreads();
-    uint32_t all = 0;
-    for (int d = first; d < last; ++d) {
+    const int d = threadIdx.x; // a block has at least as many threads as digits
+    if (d < bins) {
       uint32_t sum = 0;
       for (int q = 0; q < count; q += 4) {
         uint32_t c[4];
@@ -210,10 +209,7 @@ struct Digits {
           sum += c[u];
         }
       }
-      totals[d] = sum;
-      all += sum;
     }
-    return all;
   }
   __device__ __forceinline__ uint32_t before(uint32_t digit) const {
     const int warp = threadIdx.x >> 5;
@@ -221,79 +217,60 @@ struct Digits {
   }
 };
 
-// ---- one block ------------------------------------------------------------------
-template <int PER>
-__global__ void __launch_bounds__(kThreads)
-    nmb_sort_one(const Ids ids, int n, int bits, int passes, const Results res, const Clear clear,
-                 const Fill fill) {
+// ---- few entries ------------------------------------------------------------------
+// No passes: a warp finds an entry's position by counting the entries of smaller
+// keys and the earlier ones of the same key.  That is a comparison for every pair
+// of entries, but they depend on nothing and fill the machine; a radix sort of
+// the same entries in one block took 4 to 8 us a pass.
+constexpr int kFew = 4096, kFewThreads = 256, kFewWarps = kFewThreads / 32;
+constexpr int kFewGroups = 1023; // more groups: their offsets come from a launch of their own
+
+__global__ void __launch_bounds__(kFewThreads)
+    nmb_sort_few(const Ids ids, int n, int blocks, const Results res, const Clear clear, const Fill fill) {
   nmb::rows::let_next_begin();
   if (fill.run())
     return;
-  extern __shared__ uint32_t smem[];
-  uint32_t *keys = smem, *entries = smem + kThreads * PER; // [n]
-  uint32_t *start = entries + kThreads * PER;              // [bins]
-  uint32_t *parts = start + kBins;                         // [parts][bins]
-  uint32_t *sums = parts + kBins;                          // [32]
-  uint16_t *counts = reinterpret_cast<uint16_t *>(sums + 32);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int digit_bits = (bits + passes - 1) / passes;
-  const int begin = warp * PER * 32 + lane; // a warp owns PER * 32 consecutive entries
-  clear.run(1);
-  uint32_t key[PER], entry[PER], rank[PER];
-#pragma unroll
-  for (int u = 0; u < PER; ++u) {
-    entry[u] = begin + u * 32;
-    key[u] = begin + u * 32 < n ? ids.key(begin + u * 32) : 0;
+  __shared__ __align__(16) uint32_t keys[kFew];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int padded = (n + 127) / 128 * 128; // whole rows of four keys a lane, the rest above every key
+  for (int i = threadIdx.x; i < padded; i += kFewThreads)
+    keys[i] = i < n ? ids.key(i) : 0xffffffffu;
+  clear.run(blocks);
+  __syncthreads();
+  const int e = (int)blockIdx.x * kFewWarps + warp;
+  if (e < n) {
+    const uint32_t key = keys[e];
+    int before = 0;
+    for (int i = lane * 4; i < padded; i += 128) {
+      const uint4 k = *reinterpret_cast<const uint4 *>(keys + i);
+      // keys of earlier entries count when equal, too
+      before += (k.x < key + (i < e)) + (k.y < key + (i + 1 < e)) + (k.z < key + (i + 2 < e)) +
+                (k.w < key + (i + 3 < e));
+    }
+    before = __reduce_add_sync(kAll, before);
+    if (lane == 0) {
+      if (res.order)
+        res.order[before] = e;
+      if (res.keys)
+        res.keys[before] = key;
+      if (res.place)
+        res.place[e] = before;
+    }
   }
-  for (int pass = 0; pass < passes; ++pass) {
-    const Digits dg(counts, parts, digit_bits, pass * digit_bits);
-    dg.clear();
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const int i = begin + u * 32;
-      if (pass > 0 && i < n) {
-        key[u] = keys[i];
-        entry[u] = entries[i];
+  if (res.offsets)
+    for (int g = (int)blockIdx.x * kFewWarps + warp; g <= (int)ids.groups; g += blocks * kFewWarps) {
+      int before = 0;
+      for (int i = lane * 4; i < padded; i += 128) {
+        const uint4 k = *reinterpret_cast<const uint4 *>(keys + i);
+        before += (k.x < (uint32_t)g) + (k.y < (uint32_t)g) + (k.z < (uint32_t)g) + (k.w < (uint32_t)g);
       }
-      rank[u] = dg.rank(dg.of(key[u]), i < n);
+      before = __reduce_add_sync(kAll, before);
+      if (lane == 0)
+        res.offsets[g] = before;
     }
-    __syncthreads();
-    // a thread (or a few digits, when there are fewer threads) per digit
-    const int each = (dg.bins + (int)blockDim.x - 1) / (int)blockDim.x;
-    const int d0 = min(tid * each, dg.bins), d1 = min(d0 + each, dg.bins);
-    uint32_t at = block_prefix(dg.add_up(d0, d1, start), sums);
-    for (int d = d0; d < d1; ++d) {
-      const uint32_t here = start[d];
-      start[d] = at;
-      if (passes == 1 && res.offsets && d <= (int)ids.groups)
-        res.offsets[d] = (int32_t)at;
-      at += here;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      if (begin + u * 32 < n) {
-        const uint32_t d = dg.of(key[u]), to = start[d] + dg.before(d) + rank[u];
-        if (pass + 1 == passes) {
-          if (res.order)
-            res.order[to] = (int32_t)entry[u];
-          if (res.keys)
-            res.keys[to] = key[u];
-          if (res.place)
-            res.place[entry[u]] = (int32_t)to;
-        } else {
-          keys[to] = key[u];
-          entries[to] = entry[u];
-        }
-      }
-    }
-    __syncthreads();
-  }
 }
-constexpr int kSharedWords = 2 * kBins + 32; // start, parts, sums
-template <int PER> constexpr int oneBytes() { return (2 * kThreads * PER + kSharedWords) * 4 + kWarps * kBins * 2; }
 
+constexpr int kSharedWords = 2 * kBins + 32; // start, parts, sums
 // ---- many blocks ----------------------------------------------------------------
 // A block's counts are 16-bit (it has 8192 entries at most), two digits to a
 // word.  With `added` they hold the entries of the blocks before it, in words.
@@ -439,7 +416,7 @@ __global__ void __launch_bounds__(kThreads)
   const uint32_t digit_start = block_prefix(total, sums); // also: every warp's counts are done
   if (offsets && blockIdx.x == 0 && tid <= (int)p.ids.groups && tid < p.bins)
     offsets[tid] = (int32_t)digit_start;
-  dg.add_up(min(tid, p.bins), min(tid + 1, p.bins), start);
+  dg.add_up();
   if (tid < p.bins)
     start[tid] = digit_start + blocks_before;
   __syncthreads();
@@ -495,8 +472,9 @@ int bitsOf(int64_t groups) {
 
 size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-constexpr int64_t kOneMost = 2048;
-bool fitsOneBlock(int64_t n) { return n <= kOneMost; }
+// Counting beats one pass of a sort up to 2048 entries (4.8 against 6.5 us, at
+// 4096 10.1 against 7), two passes up to 4096 (13.7 against 16).
+bool isFew(int64_t n, int64_t groups) { return n <= (groups > kFewGroups ? kFew : kFew / 2); }
 
 // Entries per thread of the many blocks: the fewest that keep them at 148 at
 // most, and never more than 8.
@@ -564,8 +542,8 @@ namespace rows {
 // buffer, for the offsets.
 size_t sortBytes(int64_t count, int64_t groups) {
   const size_t pairs = padded((size_t)count * 4);
-  if (fitsOneBlock(count))
-    return bitsOf(groups) > kMaxDigitBits ? pairs : 0; // the sorted keys, for the offsets
+  if (isFew(count, groups))
+    return groups > kFewGroups ? pairs : 0; // the sorted keys, for the offsets
   const size_t blocks = (size_t)manyBlocks(count);
   return 4 * pairs + 2 * countBytes(blocks) + (blocks > kMostBlocks ? padded((blocks + 1) * kBins * 4) : 0);
 }
@@ -585,26 +563,19 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
   }
   unsigned char *ws = static_cast<unsigned char *>(workspace);
   const size_t pairs = padded((size_t)n * 4);
-  if (passes > 1 && offsets && !keys)
+  const bool offsetsApart = isFew(n, groups) ? groups > kFewGroups : passes > 1;
+  if (offsetsApart && offsets && !keys)
     keys = reinterpret_cast<uint32_t *>(ws); // the sorted keys, wanted for the offsets below
-  if (fitsOneBlock(n)) {
-    const bool ok = withPer(n <= kThreads ? 1 : 2, [&](auto P) {
-      constexpr int kPer = P.value < 2 ? P.value : 2;
-      static std::atomic<bool> ready[64];
-      if (!nmb::rows::allowShared(who, nmb_sort_one<kPer>, oneBytes<kPer>(), ready, s.device))
-        return false;
-      // as many warps as the entries fill, and threads for most of the digits
-      const int digits = 1 << (bits + passes - 1) / passes;
-      int threads = (int)((n + 32 * kPer - 1) / (32 * kPer)) * 32;
-      threads = threads >= digits || threads >= 512 ? threads : digits < 512 ? (digits + 31) / 32 * 32 : 512;
-      unsigned blocks;
-      const Fill fill = takeRows(clearing, 1, &blocks);
-      nmb_sort_one<kPer><<<blocks, threads, oneBytes<kPer>(), s.stream>>>(
-          in, (int)n, bits, passes, Results{order, keys, place, passes == 1 ? offsets : nullptr},
-          Clear{words, wordCount}, fill);
-      return launched(who);
-    });
-    if (!ok)
+  if (isFew(n, groups)) {
+    // a warp per entry, and for every few of the offsets
+    const int64_t warps = offsets && groups <= kFewGroups && groups / 4 > n ? groups / 4 : n;
+    const int blocks = (int)((warps + kFewWarps - 1) / kFewWarps);
+    unsigned grid;
+    const Fill fill = takeRows(clearing, blocks, &grid);
+    nmb_sort_few<<<grid, kFewThreads, 0, s.stream>>>(
+        in, (int)n, blocks, Results{order, keys, place, groups <= kFewGroups ? offsets : nullptr},
+        Clear{words, wordCount}, fill);
+    if (!launched(who))
       return false;
   } else {
     const int64_t blocks = manyBlocks(n);
@@ -664,7 +635,7 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
     if (!ok)
       return false;
   }
-  if (offsets && passes > 1) {
+  if (offsets && offsetsApart) {
     nmb_sort_offsets<<<offsetBlocks, kOffsetThreads, 0, s.stream>>>(keys, n, groups, offsets);
     return launched(who);
   }

@@ -372,10 +372,8 @@ def _workspace(workspace, name):
 _ref = ctypes.byref
 
 
-def _default(queue, first):
+def _default(first):
     """The queue of a call whose arrays are like `first` (None: not known)."""
-    if queue is not None:
-        return queue
     if type(first) is DeviceArray:
         return first._buf.queue
     if "torch" in sys.modules and isinstance(first, sys.modules["torch"].Tensor) and first.is_cuda:
@@ -383,12 +381,10 @@ def _default(queue, first):
     return None
 
 
-def _done(code):
-    """Whether the native path ran the call (it leaves what is not ordinary)."""
-    if code == 2:
-        _rt.check()
-        raise _rt.GpuRuntimeError("a row operation failed")
-    return code
+def _failed():
+    """The native path reached the library and that refused or failed."""
+    _rt.check()
+    raise _rt.GpuRuntimeError("a row operation failed")
 
 
 # ---------------------------------------------------------------- routines ---
@@ -399,8 +395,10 @@ def take_rows(table, ids, scale=1.0, out=None, queue=None):
     wide; the product is rounded once, to that type."""
     if lazy.current_trace() is not None:
         return _trace_take(table, ids, scale, out)
-    if out is not None and _done((_native or _fast()).rows_take(_default(queue, table), table, ids, scale, out)):
-        return out
+    if out is not None:
+        done = (_native or _fast()).rows_take(queue or _default(table), table, ids, scale, out)
+        if done:
+            return out if done == 1 else _failed()
     t, i = _operand(table, "table"), _operand(ids, "ids")
     o = _operand(out, "out") if out is not None else None
     on = _On(queue, (t, i) if o is None else (t, i, o))
@@ -432,9 +430,10 @@ def take_rows_grad(dout, ids, rows=None, scale=1.0, out=None, accumulate=False, 
     takes memory from the stream-ordered pool."""
     if lazy.current_trace() is not None:
         return _trace_take_grad(dout, ids, rows, scale, out, accumulate)
-    if out is not None and rows is None and workspace is None and _done((_native or _fast()).rows_take_grad(
-            _default(queue, dout), dout, ids, scale, out, bool(accumulate))):
-        return out
+    if out is not None and rows is None and workspace is None:
+        done = (_native or _fast()).rows_take_grad(queue or _default(dout), dout, ids, scale, out, bool(accumulate))
+        if done:
+            return out if done == 1 else _failed()
     d, i = _operand(dout, "dout"), _operand(ids, "ids")
     o = _operand(out, "out") if out is not None else None
     ws, ws_bytes, w = _workspace(workspace, "workspace")
@@ -480,9 +479,10 @@ def group_rows(ids, groups, plan=None, workspace=None, queue=None):
     RowGroups, written into the arrays of `plan` when one is given."""
     if lazy.current_trace() is not None:
         return _trace_group(ids, groups, plan)
-    if plan is not None and workspace is None and _done((_native or _fast()).rows_group(
-            _default(queue, ids), ids, groups, plan)):
-        return RowGroups(*plan)
+    if plan is not None and workspace is None:
+        done = (_native or _fast()).rows_group(queue or _default(ids), ids, groups, plan)
+        if done:
+            return RowGroups(*plan) if done == 1 else _failed()
     i = _operand(ids, "ids")
     results = [_operand(x, n) for x, n in zip(plan, RowGroups._fields)] if plan is not None else []
     ws, ws_bytes, w = _workspace(workspace, "workspace")
@@ -524,9 +524,10 @@ def dispatch_rows(x, ids, groups=None, out=None, plan=None, queue=None):
     sorted_already = isinstance(ids, RowGroups)
     if out is not None and (plan is None if sorted_already else plan is not None):
         known, entries = (ids, None) if sorted_already else (plan, ids)
-        if (groups is None) == sorted_already and _done((_native or _fast()).rows_dispatch(
-                _default(queue, x), x, entries, groups, known, out)):
-            return out, RowGroups(*known)
+        done = (groups is None) == sorted_already and (_native or _fast()).rows_dispatch(
+            queue or _default(x), x, entries, groups, known, out)
+        if done:
+            return (out, known if type(known) is RowGroups else RowGroups(*known)) if done == 1 else _failed()
     r = _operand(x, "x")
     if sorted_already:
         if groups is not None or plan is not None:
@@ -598,8 +599,10 @@ def combine_rows(ys, plan, weights=None, out=None, queue=None):
 
 
 def _combine(ys, plan, weights, out, queue, name):
-    if out is not None and _done((_native or _fast()).rows_combine(_default(queue, ys), ys, plan, weights, out)):
-        return out
+    if out is not None:
+        done = (_native or _fast()).rows_combine(queue or _default(ys), ys, plan, weights, out)
+        if done:
+            return out if done == 1 else _failed()
     y = _operand(ys, name)
     results = [_operand(plan[1], "place"), _operand(plan[2], "offsets")]
     w = _operand(weights, "weights") if weights is not None else None
@@ -643,9 +646,10 @@ def combine_rows_grad(dout, ys, plan, weights=None, out=None, dweights=None, que
     dweights has the type of the weights (float32 when they are None)."""
     if lazy.current_trace() is not None:
         return _trace_combine_grad(dout, ys, plan, weights, out, dweights)
-    if out is not None and dweights is not None and _done((_native or _fast()).rows_combine_grad(
-            _default(queue, dout), dout, ys, plan, weights, out, dweights)):
-        return out, dweights
+    if out is not None and dweights is not None:
+        done = (_native or _fast()).rows_combine_grad(queue or _default(dout), dout, ys, plan, weights, out, dweights)
+        if done:
+            return (out, dweights) if done == 1 else _failed()
     d, y = _operand(dout, "dout"), _operand(ys, "ys")
     results = [_operand(plan[1], "place"), _operand(plan[2], "offsets")]
     w = _operand(weights, "weights") if weights is not None else None

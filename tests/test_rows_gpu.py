@@ -252,7 +252,7 @@ def test_offsets_past_32_bits(queue):
                                       (4096, 1024), (20000, 128), (70001, 511), (12289, 5000), (300, 100000),
                                       (9000, 2**31 - 2), (50, 2**31 - 2), (200000, 16),
                                       (1025, 7), (2049, 2000), (40000, 130000), (131072, 128), (131071, 3), (131073, 128), (150000, 4000),
-                                      (4097, 5), (400000, 64), (1300000, 300), (1300000, 5000)])
+                                      (4095, 1023), (4096, 1024), (4097, 5), (127, 9), (128, 1), (129, 70000), (400000, 64), (1300000, 300), (1300000, 5000)])
 @pytest.mark.parametrize("kind", ["any", "one"])
 def test_group_rows(queue, n, groups, kind):
     import numba_mlir_b200 as nm
