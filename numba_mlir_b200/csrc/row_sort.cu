@@ -32,11 +32,14 @@ struct Ids {
   const void *data;
   int bytes;
   uint32_t groups;
-  __device__ __forceinline__ uint32_t key(int64_t i) const {
-    const int64_t id = bytes == 8 ? __ldg(static_cast<const long long *>(data) + i)
-                                  : (int64_t)__ldg(static_cast<const int *>(data) + i);
+  __device__ __forceinline__ int64_t raw(int64_t i) const {
+    return bytes == 8 ? __ldg(static_cast<const long long *>(data) + i)
+                      : (int64_t)__ldg(static_cast<const int *>(data) + i);
+  }
+  __device__ __forceinline__ uint32_t cooked(int64_t id) const {
     return id >= 0 && id < (int64_t)groups ? (uint32_t)id : groups;
   }
+  __device__ __forceinline__ uint32_t key(int64_t i) const { return cooked(raw(i)); }
 };
 
 // Exclusive prefix of v over the block's threads (blockDim.x a multiple of 32);
@@ -71,7 +74,7 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *sums) {
 }
 
 constexpr int kThreads = 1024;
-constexpr int kWarps = kThreads / 32;
+constexpr int kThreadBits = 10, kWarpBits = 5, kWarps = kThreads / 32;
 constexpr int kMostPerThread = 8;
 constexpr int kMostBlocks = 148;
 
@@ -131,24 +134,22 @@ struct Fill {
 // Where a block's entries go among its entries of each digit.  An entry's rank
 // is made of three: among the equal digits of its warp (rank), in the warps of
 // its part before that (counts), in the parts before that (parts).  A part is a
-// share of the warps that one thread adds up for a digit.
+// share of the warps that one thread adds up, for two digits at a time: a block's
+// counts fit 16 bits, and two of them add in one word.
 struct Digits {
   uint16_t *counts;  // [warps][bins]
-  uint32_t *parts;   // [parts][bins]
-  int bins, bin_bits, shift, warps, part_bits; // 1 << part_bits warps to a part
+  uint16_t *parts;   // [parts][bins]
+  int bins, bin_bits, shift, part_bits; // 1 << part_bits warps to a part
   __device__ __forceinline__ uint32_t of(uint32_t key) const { return (key >> shift) & (uint32_t)(bins - 1); }
 
-  __device__ __forceinline__ Digits(uint16_t *counts, uint32_t *parts, int bin_bits, int shift)
+  __device__ __forceinline__ Digits(uint16_t *counts, uint16_t *parts, int bin_bits, int shift)
       : counts(counts), parts(parts), bins(1 << bin_bits), bin_bits(bin_bits), shift(shift),
-        warps((int)blockDim.x >> 5), part_bits(0) {
-    // as many parts as there are threads for every digit
-    while ((warps + (1 << part_bits) - 1) >> part_bits > (int)blockDim.x >> bin_bits)
-      ++part_bits;
-  }
+        // kThreads / (bins / 2) parts, but not more than warps
+        part_bits(max(kWarpBits - (kThreadBits - bin_bits + 1), 0)) {}
 
   __device__ __forceinline__ void clear() const {
     uint32_t *words = reinterpret_cast<uint32_t *>(counts);
-    for (int i = threadIdx.x; i < warps * bins / 2; i += blockDim.x)
+    for (int i = threadIdx.x; i < kWarps * bins / 2; i += kThreads)
       words[i] = 0;
   }
 
@@ -175,37 +176,37 @@ struct Digits {
   // Adds the warps' counts up, four at a time, then the parts', for `before`.
   // Between two barriers of the caller's.
   __device__ __forceinline__ void add_up() const {
-    const int count = (warps + (1 << part_bits) - 1) >> part_bits;
-    for (int i = threadIdx.x; i < count * bins; i += blockDim.x) {
-      const int d = i & (bins - 1), from = i >> bin_bits << part_bits, to = min(from + (1 << part_bits), warps);
+    uint32_t *pairs = reinterpret_cast<uint32_t *>(counts), *sums = reinterpret_cast<uint32_t *>(parts);
+    const int half = bins / 2, count = kWarps >> part_bits, rows = 1 << part_bits;
+    const int pair = threadIdx.x & (half - 1), part = threadIdx.x >> (bin_bits - 1);
+    if (part < count) {
       uint32_t sum = 0;
-      for (int w = from; w < to; w += 4) {
+      for (int w = part * rows; w < (part + 1) * rows; w += 4) {
         uint32_t c[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          c[u] = w + u < to ? counts[(w + u) * bins + d] : 0;
+          c[u] = u < rows ? pairs[(w + u) * half + pair] : 0;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          if (w + u < to)
-            counts[(w + u) * bins + d] = (uint16_t)sum;
+          if (u < rows)
+            pairs[(w + u) * half + pair] = sum;
           sum += c[u];
         }
       }
-      parts[i] = sum;
+      sums[part * half + pair] = sum;
     }
     __syncthreads();
-    const int d = threadIdx.x; // a block has at least as many threads as digits
-    if (d < bins) {
+    if (part == 0) {
       uint32_t sum = 0;
       for (int q = 0; q < count; q += 4) {
         uint32_t c[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          c[u] = q + u < count ? parts[(q + u) * bins + d] : 0;
+          c[u] = q + u < count ? sums[(q + u) * half + pair] : 0;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           if (q + u < count)
-            parts[(q + u) * bins + d] = sum;
+            sums[(q + u) * half + pair] = sum;
           sum += c[u];
         }
       }
@@ -270,7 +271,6 @@ __global__ void __launch_bounds__(kFewThreads)
     }
 }
 
-constexpr int kSharedWords = 2 * kBins + 32; // start, parts, sums
 // ---- many blocks ----------------------------------------------------------------
 // A block's counts are 16-bit (it has 8192 entries at most), two digits to a
 // word.  With `added` they hold the entries of the blocks before it, in words.
@@ -283,7 +283,10 @@ struct Pass {
   uint32_t *added;         // [blocks][bins] and then [bins] totals, or null
   int64_t n;
   int blocks, shift, bins, digit_bits;
-  __device__ __forceinline__ uint32_t key(int64_t i) const { return keysIn ? keysIn[i] : ids.key(i); }
+  // an entry's key in two steps: what is read, and what is made of it
+  __device__ __forceinline__ int64_t raw(int64_t i) const { return keysIn ? (int64_t)keysIn[i] : ids.raw(i); }
+  __device__ __forceinline__ uint32_t cooked(int64_t id) const { return ids.cooked(id); }
+  __device__ __forceinline__ uint32_t key(int64_t i) const { return cooked(raw(i)); }
   __device__ __forceinline__ uint32_t digit(uint32_t k) const { return (k >> shift) & (uint32_t)(bins - 1); }
 };
 
@@ -352,10 +355,10 @@ __global__ void __launch_bounds__(kThreads)
     return;
   extern __shared__ uint32_t smem[];
   uint32_t *start = smem;                   // [bins]
-  uint32_t *parts = start + kBins;          // [parts][bins]
-  uint32_t *sums = parts + kBins;           // [32]
+  uint32_t *sums = start + kBins;           // [32]
   uint2 *shares = reinterpret_cast<uint2 *>(sums + 32); // [2][threads]: a thread's blocks before this one, all its blocks
   uint16_t *counts = reinterpret_cast<uint16_t *>(shares + 2 * kThreads);
+  uint16_t *parts = counts + kWarps * kBins; // [parts][bins]: 2 * kThreads at most
   const Digits dg(counts, parts, p.digit_bits, p.shift);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t begin = ((int64_t)blockIdx.x * kWarps + warp) * PER * 32 + lane;
@@ -363,24 +366,30 @@ __global__ void __launch_bounds__(kThreads)
   int32_t entry[PER];
   dg.clear();
   nmb::rows::wait_for_previous();
+  // counts of all blocks: a thread adds up every share-th block for two digits,
+  // sixteen loads in flight (one by one they took 15 of the kernel's 19 us at
+  // 131072 entries: an L2 access costs about 700 cycles), and the entries' own
+  // with the first of them
+  const int pairs = p.bins / 2, share = kThreads >> (p.digit_bits - 1), part = tid >> (p.digit_bits - 1);
+  const uint32_t *from = p.counts + (tid & (pairs - 1));
+  uint32_t c[16];
+  auto read_counts = [&](int b0) {
+#pragma unroll
+    for (int u = 0; u < 16; ++u)
+      c[u] = b0 + u * share < p.blocks ? __ldg(from + (int64_t)(b0 + u * share) * pairs) : 0;
+  };
+  if (!p.added)
+    read_counts(part);
+  int64_t id[PER];
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     const int64_t i = begin + u * 32;
-    key[u] = i < p.n ? p.key(i) : 0;
+    id[u] = i < p.n ? p.raw(i) : 0;
     entry[u] = i < p.n && p.entriesIn ? p.entriesIn[i] : (int32_t)i;
   }
-  // counts of all blocks: a thread adds up every share-th block for two digits,
-  // sixteen loads in flight (one by one they took 15 of the kernel's 19 us at
-  // 131072 entries: an L2 access costs about 700 cycles)
-  const int pairs = p.bins / 2, share = kThreads >> (p.digit_bits - 1), part = tid >> (p.digit_bits - 1);
-  uint2 mine = make_uint2(0, 0), all = make_uint2(0, 0);
   if (!p.added) {
-    const uint32_t *from = p.counts + (tid & (pairs - 1));
-    for (int b0 = part; b0 < p.blocks; b0 += 16 * share) {
-      uint32_t c[16];
-#pragma unroll
-      for (int u = 0; u < 16; ++u)
-        c[u] = b0 + u * share < p.blocks ? __ldg(from + (int64_t)(b0 + u * share) * pairs) : 0;
+    uint2 mine = make_uint2(0, 0), all = make_uint2(0, 0);
+    for (int b0 = part;;) {
 #pragma unroll
       for (int u = 0; u < 16; ++u) {
         const uint32_t lo = c[u] & 0xffff, hi = c[u] >> 16;
@@ -389,10 +398,17 @@ __global__ void __launch_bounds__(kThreads)
         mine.x += b0 + u * share < (int)blockIdx.x ? lo : 0;
         mine.y += b0 + u * share < (int)blockIdx.x ? hi : 0;
       }
+      b0 += 16 * share;
+      if (b0 >= p.blocks)
+        break;
+      read_counts(b0);
     }
     shares[tid] = mine;
     shares[kThreads + tid] = all;
   }
+#pragma unroll
+  for (int u = 0; u < PER; ++u)
+    key[u] = p.cooked(id[u]);
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < PER; ++u)
@@ -437,7 +453,7 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
 }
-constexpr int kScatterBytes = kSharedWords * 4 + 2 * kThreads * 8 + kWarps * kBins * 2;
+constexpr int kScatterBytes = (kBins + 32) * 4 + 2 * kThreads * 8 + kWarps * kBins * 2 + 2 * kThreads * 2;
 
 // offsets[g] = position of the first key >= g, for the sorts of several passes.
 constexpr int kOffsetThreads = 256;
@@ -469,6 +485,8 @@ int bitsOf(int64_t groups) {
     ++b;
   return b; // keys are 0 .. groups
 }
+
+int passesOf(int64_t groups) { return (bitsOf(groups) + kMaxDigitBits - 1) / kMaxDigitBits; }
 
 size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
@@ -544,8 +562,8 @@ size_t sortBytes(int64_t count, int64_t groups) {
   const size_t pairs = padded((size_t)count * 4);
   if (isFew(count, groups))
     return groups > kFewGroups ? pairs : 0; // the sorted keys, for the offsets
-  const size_t blocks = (size_t)manyBlocks(count);
-  return 4 * pairs + 2 * countBytes(blocks) + (blocks > kMostBlocks ? padded((blocks + 1) * kBins * 4) : 0);
+  const size_t blocks = (size_t)manyBlocks(count), passes = (size_t)passesOf(groups);
+  return 4 * pairs + passes * countBytes(blocks) + (blocks > kMostBlocks ? padded((blocks + 1) * kBins * 4) : 0);
 }
 
 bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t groups, int32_t *order,
@@ -553,7 +571,7 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
                int64_t wordCount, Clearing *clearing) {
   const int64_t n = ids.count;
   const Ids in{ids.data, ids.bytes, (uint32_t)groups};
-  const int bits = bitsOf(groups), passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
+  const int bits = bitsOf(groups), passes = passesOf(groups);
   const unsigned offsetBlocks = (unsigned)((groups + kOffsetThreads) / kOffsetThreads);
   if (n == 0) {
     if (!offsets)
@@ -582,13 +600,14 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
     uint32_t *keyBuf[2] = {reinterpret_cast<uint32_t *>(ws), reinterpret_cast<uint32_t *>(ws + pairs)};
     int32_t *entryBuf[2] = {reinterpret_cast<int32_t *>(ws + 2 * pairs), reinterpret_cast<int32_t *>(ws + 3 * pairs)};
     const size_t countSize = countBytes((size_t)blocks);
-    uint32_t *counts[2] = {reinterpret_cast<uint32_t *>(ws + 4 * pairs),
-                           reinterpret_cast<uint32_t *>(ws + 4 * pairs + countSize)};
-    uint32_t *added =
-        blocks > kMostBlocks ? reinterpret_cast<uint32_t *>(ws + 4 * pairs + 2 * countSize) : nullptr;
+    // the counts of each pass in memory of their own, one behind the other
     const int digitBits = (bits + passes - 1) / passes, bins = 1 << digitBits;
+    uint32_t *counts = reinterpret_cast<uint32_t *>(ws + 4 * pairs);
     const int64_t countWords = blocks * (bins / 2);
-    Pass p{in, nullptr, nullptr, counts[0], nullptr, added, n, (int)blocks, 0, bins, digitBits};
+    uint32_t *added = blocks > kMostBlocks
+                          ? reinterpret_cast<uint32_t *>(ws + 4 * pairs + (size_t)passes * countSize)
+                          : nullptr;
+    Pass p{in, nullptr, nullptr, counts, nullptr, added, n, (int)blocks, 0, bins, digitBits};
     const bool ok = withPer(perThread(n), [&](auto P) {
       static std::atomic<bool> ready[64];
       if (!nmb::rows::allowShared(who, nmb_sort_scatter<P.value>, kScatterBytes, ready, s.device))
@@ -596,7 +615,7 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
       unsigned grid;
       const Fill beside = takeRows(clearing, (int)blocks, &grid);
       nmb_sort_count<P.value><<<grid, kThreads, 0, s.stream>>>(
-          p, Clear{counts[1], passes > 1 ? countWords : 0}, Clear{words, wordCount}, beside);
+          p, Clear{counts + countWords, (passes - 1) * countWords}, Clear{words, wordCount}, beside);
       if (!launched(who))
         return false;
       for (int pass = 0; pass < passes; ++pass) {
@@ -605,17 +624,8 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
         // sorted keys into buffer 0 (see above)
         const int to = (passes - 1 - pass) & 1;
         p.shift = pass * digitBits;
-        p.counts = counts[pass & 1];
-        p.next = last ? nullptr : counts[(pass + 1) & 1];
-        if (pass > 0 && !last) {
-          // the counts of the pass before, about to be used for the pass after
-          const cudaError_t e = cudaMemsetAsync(p.next, 0, (size_t)countWords * 4, s.stream);
-          if (e != cudaSuccess) {
-            setError("%s: cudaMemsetAsync failed: %s", who, cudaGetErrorString(e));
-            (void)cudaGetLastError();
-            return false;
-          }
-        }
+        p.counts = counts + pass * countWords;
+        p.next = last ? nullptr : p.counts + countWords;
         if (added) {
           nmb_sort_add<<<(unsigned)((bins + kAddThreads / 32 - 1) / (kAddThreads / 32)), kAddThreads, 0, s.stream>>>(p);
           if (!launched(who))

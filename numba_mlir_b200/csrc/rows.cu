@@ -339,7 +339,7 @@ int takeLaneBits(int64_t n, int64_t vecs) {
 // rows up in the sorted keys, one row a lane.  The last rows (of a vocabulary:
 // the rare tokens) have been cleared beside the sort, whether they have entries
 // or not.
-constexpr int kGradBatch = 2;   // incoming rows in flight per thread, through registers
+constexpr int kGradBatch = 4;   // incoming rows in flight per thread, through registers
 constexpr int kTurnRows = 4;    // rows of a turn, by bulk copies
 constexpr int kZeroRows = 32;   // rows looked up by a block that clears
 constexpr int kBundle = 32;     // partial sums added up by one group
@@ -389,6 +389,43 @@ __device__ __forceinline__ int64_t warp_lower_bound(const uint32_t *__restrict__
   return lo;
 }
 
+// The end of the run of `key` that goes on at keys[at], and the begin of the one
+// that keys[at - 1] belongs to, for the threads of a warp or for one.  Most runs
+// end nearby: a warp looks at 1024 places first (two reads), a thread at ever
+// longer steps.
+__device__ __forceinline__ int64_t warp_run_end(const uint32_t *__restrict__ keys, int64_t at, int64_t n, uint32_t key) {
+  const int64_t probe = at + (threadIdx.x & 31) * 32 + 31;
+  const unsigned past = __ballot_sync(kAll, probe >= n || __ldg(keys + (probe < n ? probe : at)) != key);
+  if (past == 0)
+    return warp_lower_bound(keys, at + 1024, n, key + 1);
+  const int64_t first = at + (int64_t)(__ffs(past) - 1) * 32, place = first + (threadIdx.x & 31);
+  return first + __popc(__ballot_sync(kAll, place < n && __ldg(keys + (place < n ? place : at)) == key));
+}
+__device__ __forceinline__ int64_t warp_run_begin(const uint32_t *__restrict__ keys, int64_t at, uint32_t key) {
+  const int64_t probe = at - 32 - (threadIdx.x & 31) * 32;
+  const unsigned past = __ballot_sync(kAll, probe < 0 || __ldg(keys + (probe < 0 ? at - 1 : probe)) != key);
+  if (past == 0)
+    return warp_lower_bound(keys, 0, at - 1024, key);
+  const int64_t last = at - (int64_t)(__ffs(past) - 1) * 32, place = last - 1 - (threadIdx.x & 31);
+  return last - __popc(__ballot_sync(kAll, place >= 0 && __ldg(keys + (place < 0 ? at - 1 : place)) == key));
+}
+__device__ __forceinline__ int64_t run_end(const uint32_t *__restrict__ keys, int64_t at, int64_t n, uint32_t key) {
+  int64_t step = 1;
+  while (at + step < n && __ldg(keys + at + step) == key) {
+    at += step;
+    step *= 2;
+  }
+  return lower_bound(keys, at, min(at + step, n), key + 1);
+}
+__device__ __forceinline__ int64_t run_begin(const uint32_t *__restrict__ keys, int64_t at, uint32_t key) {
+  int64_t step = 1;
+  while (at - step >= 0 && __ldg(keys + at - step) == key) {
+    at -= step;
+    step *= 2;
+  }
+  return lower_bound(keys, max(at - step, (int64_t)0), at, key);
+}
+
 // The threads that share a chunk: a block, or 1 << bits of its threads.
 template <bool BLOCK> struct Group {
   int bits, lanes, lane, number;
@@ -420,6 +457,12 @@ template <bool BLOCK> struct Group {
   }
   __device__ __forceinline__ int64_t find(const uint32_t *keys, int64_t lo, int64_t hi, uint32_t key) const {
     return BLOCK || bits >= 5 ? warp_lower_bound(keys, lo, hi, key) : lower_bound(keys, lo, hi, key);
+  }
+  __device__ __forceinline__ int64_t end_of(const uint32_t *keys, int64_t at, int64_t n, uint32_t key) const {
+    return BLOCK || bits >= 5 ? warp_run_end(keys, at, n, key) : run_end(keys, at, n, key);
+  }
+  __device__ __forceinline__ int64_t begin_of(const uint32_t *keys, int64_t at, uint32_t key) const {
+    return BLOCK || bits >= 5 ? warp_run_begin(keys, at, key) : run_begin(keys, at, key);
   }
 };
 
@@ -468,8 +511,22 @@ template <typename A, int V> struct Sums {
   }
 };
 
-// A thread's columns of the result.
-// V neighbouring ones, or, LOOSE, every step-th one.
+// Sets a row to zero: 16-byte stores between its own boundaries.
+template <typename O> __device__ __forceinline__ void clear_row(O *row, int64_t cols, int lane, int lanes) {
+  const int64_t head =
+      min(cols, (int64_t)((-reinterpret_cast<intptr_t>(row) & 15) / (int)sizeof(O)));
+  const int64_t whole = (cols - head) * (int64_t)sizeof(O) / 16, tail = head + whole * (16 / (int)sizeof(O));
+  int4 *words = reinterpret_cast<int4 *>(row + head);
+  for (int64_t i = lane; i < whole; i += lanes)
+    words[i] = make_int4(0, 0, 0, 0);
+  for (int64_t i = lane; i < head; i += lanes)
+    row[i] = O(0.0f);
+  for (int64_t i = tail + lane; i < cols; i += lanes)
+    row[i] = O(0.0f);
+}
+
+// A thread's columns of the result: V neighbouring ones, or, LOOSE, every step-th
+// one.
 template <typename O, int V, bool ADD, bool LOOSE, typename A> struct GradColumn {
   O *out;          // the thread's first column of row 0
   int64_t stride;
@@ -687,7 +744,7 @@ __device__ __forceinline__ void add_partials(const A *partials, int64_t width, i
 // BULK: the group is the block and V elements are 16 bytes of I; LOOSE: a
 // thread's V columns are as many threads apart.
 template <typename I, typename O, int V, bool ADD, bool BULK, bool LOOSE>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, BULK ? 4 : 3)
     nmb_take_rows_grad(const I *__restrict__ dout, int64_t stride, const GradPlan p, typename Acc<I>::type scale, O *out,
                        int64_t rows, int64_t out_stride, int64_t cols, const Bounds<I> bounds) {
   using A = typename Acc<I>::type;
@@ -717,18 +774,9 @@ __global__ void __launch_bounds__(kThreads, 4)
     }
     __syncthreads();
     const uint32_t mask = words[0];
-    Pack<O, V> zero;
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      zero.v[e] = down<O, A>(A(0));
     for (int r = group.number; r < kZeroRows; r += (int)blockDim.x / group.lanes)
       if (mask >> r & 1)
-        for (int64_t c = group.lane * (LOOSE ? 1 : V); c < cols; c += group.lanes * (LOOSE ? 1 : V)) {
-          if constexpr (LOOSE)
-            out[(first + r) * out_stride + c] = zero.v[0];
-          else
-            store<O, V>(out + (first + r) * out_stride + c, zero);
-        }
+        clear_row(out + (first + r) * out_stride, cols, group.lane, group.lanes);
     return;
   }
 
@@ -754,9 +802,9 @@ __global__ void __launch_bounds__(kThreads, 4)
   Walk walk{begin, end, end, end};
   if (begin > 0 && prev_key == first_key && last_key == first_key && end - begin == p.span) {
     // inside a long run as a whole
-    owner = group.find(p.keys, 0, begin, first_key) / p.span;
-    const int64_t run_end = next_key == first_key ? group.find(p.keys, end, p.n, first_key + 1) : end;
-    inner = (run_end - (owner + 1) * p.span) / p.span;
+    owner = group.begin_of(p.keys, begin, first_key) / p.span;
+    const int64_t stop = next_key == first_key ? group.end_of(p.keys, end, p.n, first_key) : end;
+    inner = (stop - (owner + 1) * p.span) / p.span;
   } else {
     // entries of a run that began before belong to the group it began in
     if (prev_key == first_key)
@@ -766,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     if (walk.begin >= walk.middle)
       return;
     if (last_key < rows && next_key == last_key) {
-      walk.end = group.find(p.keys, end, p.n, last_key + 1);
+      walk.end = group.end_of(p.keys, end, p.n, last_key);
       inner = (walk.end - end) / p.span;
       walk.tail = end + inner * p.span;
     }
@@ -818,14 +866,15 @@ __global__ void __launch_bounds__(kThreads, 4)
   column.write(row, sum, column.old(row));
 }
 
-// Entries per chunk: 32, or fewer (down to 4) where that leaves less than four
+// Entries per chunk: 32, or fewer (down to 4) where that leaves less than two
 // blocks a multiprocessor.  With 777 entries of 1000 float32 chunks of 4 give
-// 195 blocks, chunks of 32 only 25.
+// 195 blocks, chunks of 32 only 25; 52004 entries of 248 bfloat16 took 29.4 us
+// with two, 34.8 us with four (shorter chunks leave more partial sums).
 int gradSpan(int64_t n, int64_t vecs) {
   const int bits = laneBits(vecs, kThreadBits);
   const int64_t slabs = (vecs + (int64_t(1) << bits) - 1) >> bits;
   int span = 32;
-  while (span > 4 && (n / span >> (kThreadBits - bits)) * slabs < 148 * 4)
+  while (span > 4 && (n / span >> (kThreadBits - bits)) * slabs < 148 * 2)
     span /= 2;
   return span;
 }
