@@ -1060,27 +1060,29 @@ template <typename T, bool LOOSE>
 __global__ void __launch_bounds__(kBulkThreads)
     nmb_combine_rows_bulk(const T *__restrict__ ys, int64_t y_rows, int64_t stride, int k,
                           const int32_t *__restrict__ place, const int32_t *__restrict__ kept,
-                          const void *__restrict__ weights, int weight_type, T *__restrict__ out, int64_t out_stride,
-                          int64_t cols, int slab, const Bounds<T> bounds, uint32_t *status) {
+                          const void *__restrict__ weights, int weight_type, T *__restrict__ out, int64_t tokens,
+                          int64_t out_stride, int64_t cols, int slab, int each, const Bounds<T> bounds,
+                          uint32_t *status) {
   using A = typename Acc<T>::type;
   constexpr int V = kBulkElems<LOOSE, T>;
-  extern __shared__ __align__(128) unsigned char rows[]; // [k] rows
+  extern __shared__ __align__(128) unsigned char rows[]; // [each][k] rows
   __shared__ BulkChoices<A> c;
-  const int64_t t = blockIdx.x, first = (int64_t)blockIdx.y * slab;
+  const int64_t t0 = (int64_t)blockIdx.x * each, first = (int64_t)blockIdx.y * slab;
   const int here = (int)min((int64_t)slab, cols - first), bytes = fetched_bytes<LOOSE, T>(slab);
+  const int entries = k * (int)min((int64_t)each, tokens - t0);
   const int j = threadIdx.x;
   int32_t at = -1;
-  if (j < k) {
-    at = __ldg(place + t * k + j);
+  if (j < entries) {
+    at = __ldg(place + t0 * k + j);
     at = at < min((int64_t)__ldg(kept), y_rows) ? at : -1;
-    c.weight[j] = weights ? scalar_at<A>(weights, weight_type, t * k + j) : A(1);
+    c.weight[j] = weights ? scalar_at<A>(weights, weight_type, t0 * k + j) : A(1);
   }
   if (j == 0) {
-    nmb::mbar_init(&c.bar, (uint32_t)k);
+    nmb::mbar_init(&c.bar, (uint32_t)entries);
     nmb::mbar_init_fence();
   }
   __syncthreads();
-  if (j < k) {
+  if (j < entries) {
     c.at[j] = -1;
     if (at >= 0)
       c.at[j] = j * bytes + (int)sizeof(T) * fetch_row<LOOSE>(ys + at * stride + first, here, rows + j * bytes, &c.bar,
@@ -1091,21 +1093,27 @@ __global__ void __launch_bounds__(kBulkThreads)
   __syncthreads();
   if (!bulk_arrived(&c.bar, 0, status))
     return;
-  for (int col = threadIdx.x * V; col < here; col += kBulkThreads * V) {
+  const int threads = kBulkThreads / each, token = j / threads; // of a token
+  if (t0 + token >= tokens)
+    return;
+  const int32_t *begin = c.at + token * k;
+  const A *weight = c.weight + token * k;
+  T *dst = out + (t0 + token) * out_stride + first;
+  for (int col = (j - token * threads) * V; col < here; col += threads * V) {
     A sum[V] = {};
 #pragma unroll 4
     for (int i = 0; i < k; ++i)
-      if (c.at[i] >= 0) {
-        const Pack<T, V> y = load<T, V>(reinterpret_cast<const T *>(rows + c.at[i]) + col);
+      if (begin[i] >= 0) {
+        const Pack<T, V> y = load<T, V>(reinterpret_cast<const T *>(rows + begin[i]) + col);
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          sum[e] = madd(c.weight[i], up(y.v[e]), sum[e]);
+          sum[e] = madd(weight[i], up(y.v[e]), sum[e]);
       }
     Pack<T, V> r;
 #pragma unroll
     for (int e = 0; e < V; ++e)
       r.v[e] = down<T, A>(sum[e]);
-    store<T, V>(out + t * out_stride + first + col, r);
+    store<T, V>(dst + col, r);
   }
 }
 
@@ -1120,6 +1128,17 @@ int bulkSlab(int64_t cols, int type, bool loose, int64_t choices, int rows, int 
   const int64_t slabs = (cols * size + room - 1) / room;
   const int64_t slab = ((cols + slabs - 1) / slabs + step - 1) / step * step;
   return slabs <= 65535 ? (int)slab : 0;
+}
+
+// Tokens of a block where their rows are so narrow that a block of one token is
+// mostly its own beginning: up to four, as long as `most` bytes and the choices
+// hold them and four blocks a multiprocessor are left.  30000 tokens with two
+// rows of 1 KB took 29.2 us with a block each.
+int bulkTokens(int64_t tokens, int64_t bytesEach, int64_t entriesEach, int most) {
+  int each = 4;
+  while (each > 1 && (each * bytesEach > most || each * entriesEach > kBulkChoices || tokens / each < 148 * 4))
+    each /= 2;
+  return each;
 }
 
 // ----------------------------------------------------------- combine_grad ---
@@ -1237,30 +1256,35 @@ __global__ void __launch_bounds__(kThreads, 4)
 
 // The same with the rows fetched by bulk copies, dout's first.  A block takes a
 // whole token; columns beyond a slab come in turns through the same memory.
-template <typename T, bool LOOSE>
+template <typename T, bool LOOSE, int CHOICES>
 __global__ void __launch_bounds__(kBulkThreads)
-    nmb_combine_rows_grad_bulk(const T *__restrict__ dout, int64_t stride, const T *__restrict__ ys, int64_t y_rows,
+    nmb_combine_rows_grad_bulk(const T *__restrict__ dout, int64_t tokens, int64_t stride, const T *__restrict__ ys, int64_t y_rows,
                                int64_t y_stride, int k, const int32_t *__restrict__ place,
                                const int32_t *__restrict__ kept, const void *__restrict__ weights, int weight_type,
                                T *__restrict__ dys, int64_t dy_rows, int64_t dy_stride, void *dweights, int64_t cols,
-                               int slab, const Bounds<T> dbounds, const Bounds<T> ybounds, uint32_t *status) {
+                               int slab, int each, const Bounds<T> dbounds, const Bounds<T> ybounds, uint32_t *status) {
   using A = typename Acc<T>::type;
-  constexpr int V = kBulkElems<LOOSE, T>, kWarps = kBulkThreads / 32, kGradChoices = 8, kPairs = V > 1 ? V / 2 : 1;
-  extern __shared__ __align__(128) unsigned char rows[]; // [1 + k] rows, dout's first
+  constexpr int V = kBulkElems<LOOSE, T>, kWarps = kBulkThreads / 32, kPairs = V > 1 ? V / 2 : 1;
+  extern __shared__ __align__(128) unsigned char rows[]; // [each][1 + k] rows, dout's first
   __shared__ BulkChoices<A> c;
-  __shared__ int begin[kBulkChoices + 1]; // where each row's first element is
+  __shared__ int begin[2 * kBulkChoices]; // where each row's first element is
   __shared__ A parts[kWarps][kBulkChoices];
-  const int64_t t = blockIdx.x;
+  const int64_t t0 = (int64_t)blockIdx.x * each;
   const int j = threadIdx.x, lane = j & 31, warp = j >> 5, bytes = fetched_bytes<LOOSE, T>(slab);
+  const int here_tokens = (int)min((int64_t)each, tokens - t0), entries = here_tokens * k;
+  const int threads = kBulkThreads / each, token = j / threads, mine = j - token * threads; // a token's threads
   const int64_t live = min((int64_t)__ldg(kept), y_rows);
+  // thread j fetches dout's row of a token or that of a choice
+  const int fetches = here_tokens * (k + 1), ftoken = j / (k + 1), fchoice = j - ftoken * (k + 1) - 1;
   int32_t at = -1;
-  if (j < k) {
-    at = __ldg(place + t * k + j);
-    c.at[j] = at < dy_rows ? at : -1;
-    c.weight[j] = weights ? scalar_at<A>(weights, weight_type, t * k + j) : A(1);
+  if (j < fetches && fchoice >= 0) {
+    const int e = ftoken * k + fchoice;
+    at = __ldg(place + t0 * k + e);
+    c.at[e] = at < dy_rows ? at : -1;
+    c.weight[e] = weights ? scalar_at<A>(weights, weight_type, t0 * k + e) : A(1);
   }
   if (j == 0) {
-    nmb::mbar_init(&c.bar, (uint32_t)k + 1);
+    nmb::mbar_init(&c.bar, (uint32_t)fetches);
     nmb::mbar_init_fence();
   }
   for (int i = j; i < kWarps * kBulkChoices; i += kBulkThreads)
@@ -1269,12 +1293,12 @@ __global__ void __launch_bounds__(kBulkThreads)
   uint32_t phase = 0;
   for (int64_t first = 0; first < cols; first += slab, phase ^= 1) {
     const int here = (int)min((int64_t)slab, cols - first);
-    if (j <= k) { // thread k fetches dout
-      unsigned char *to = rows + (j < k ? j + 1 : 0) * bytes;
-      if (j == k)
-        begin[0] = fetch_row<LOOSE>(dout + t * stride + first, here, to, &c.bar, dbounds);
+    if (j < fetches) {
+      unsigned char *to = rows + j * bytes;
+      if (fchoice < 0)
+        begin[j] = fetch_row<LOOSE>(dout + (t0 + ftoken) * stride + first, here, to, &c.bar, dbounds);
       else if (at >= 0 && at < live)
-        begin[j + 1] = fetch_row<LOOSE>(ys + at * y_stride + first, here, to, &c.bar, ybounds);
+        begin[j] = fetch_row<LOOSE>(ys + at * y_stride + first, here, to, &c.bar, ybounds);
       else
         nmb::mbar_arrive(&c.bar);
     }
@@ -1282,21 +1306,22 @@ __global__ void __launch_bounds__(kBulkThreads)
       __syncthreads(); // `begin` is written behind the arrivals
     if (!bulk_arrived(&c.bar, phase, status))
       return; // every thread gives up by itself: no barrier is left waiting
-    const T *drow = reinterpret_cast<const T *>(rows) + (LOOSE ? begin[0] : 0);
-    for (int j0 = 0; j0 < k; j0 += kGradChoices) {
-      int32_t to[kGradChoices];
-      A w[kGradChoices];
-      const T *yrow[kGradChoices];
-      typename Two<A>::type dots[kGradChoices] = {};
+    const int row0 = token * (k + 1), entry0 = token * k;
+    const T *drow = reinterpret_cast<const T *>(rows + row0 * bytes) + (LOOSE ? begin[row0] : 0);
+    for (int j0 = 0; j0 < k && token < here_tokens; j0 += CHOICES) {
+      int32_t to[CHOICES];
+      A w[CHOICES];
+      const T *yrow[CHOICES];
+      typename Two<A>::type dots[CHOICES] = {};
 #pragma unroll
-      for (int i = 0; i < kGradChoices; ++i) {
-        to[i] = j0 + i < k ? c.at[j0 + i] : -1;
-        w[i] = j0 + i < k ? c.weight[j0 + i] : A(0);
-        yrow[i] = reinterpret_cast<const T *>(rows + (j0 + i + 1) * bytes);
+      for (int i = 0; i < CHOICES; ++i) {
+        to[i] = j0 + i < k ? c.at[entry0 + j0 + i] : -1;
+        w[i] = j0 + i < k ? c.weight[entry0 + j0 + i] : A(0);
+        yrow[i] = reinterpret_cast<const T *>(rows + (row0 + j0 + i + 1) * bytes);
         if (LOOSE && to[i] >= 0 && to[i] < live)
-          yrow[i] += begin[j0 + i + 1];
+          yrow[i] += begin[row0 + j0 + i + 1];
       }
-      for (int col = j * V; col < here; col += kBulkThreads * V) {
+      for (int col = mine * V; col < here; col += threads * V) {
         const Pack<T, V> x = load<T, V>(drow + col);
         typename Two<A>::type d[kPairs];
 #pragma unroll
@@ -1307,7 +1332,7 @@ __global__ void __launch_bounds__(kBulkThreads)
             d[e].x = up(x.v[0]);
         }
 #pragma unroll
-        for (int i = 0; i < kGradChoices; ++i)
+        for (int i = 0; i < CHOICES; ++i)
           if (to[i] >= 0) {
             Pack<T, V> r{};
             if (to[i] < live) {
@@ -1326,23 +1351,24 @@ __global__ void __launch_bounds__(kBulkThreads)
             store<T, V>(dys + to[i] * dy_stride + first + col, r);
           }
       }
-      A dot[kGradChoices];
+      A dot[CHOICES];
 #pragma unroll
-      for (int i = 0; i < kGradChoices; ++i)
+      for (int i = 0; i < CHOICES; ++i)
         dot[i] = dots[i].x + dots[i].y;
       meet(dot, 32);
-      const int mine = (lane & 1) << 2 | (lane & 2) | (lane & 4) >> 2;
-      if (lane < kGradChoices && j0 + mine < k)
-        parts[warp][j0 + mine] += dot[0];
+      const int which = CHOICES == 8 ? (lane & 1) << 2 | (lane & 2) | (lane & 4) >> 2 : lane & 1; // see meet
+      if (lane < CHOICES && j0 + which < k)
+        parts[warp][j0 + which] += dot[0];
     }
     __syncthreads(); // the slab's memory is free again, the sums are in place
   }
-  if (j < k && dweights) {
+  if (j < entries && dweights) {
+    // a token's warps in order
+    const int of = j / k, warps = kWarps / each;
     A sum = A(0);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w)
-      sum += parts[w][j];
-    set_scalar<A>(dweights, weight_type, t * k + j, sum);
+    for (int w = 0; w < warps; ++w)
+      sum += parts[of * warps + w][j - of * k];
+    set_scalar<A>(dweights, weight_type, t0 * k + j, sum);
   }
 }
 
@@ -1757,10 +1783,12 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows
     const bool loose = v < mostElems<T>();
     if (const int slab = bulkSlab(out->cols, out->type, loose, k, (int)k, kBulkBytes)) {
       const auto kernel = loose ? nmb_combine_rows_bulk<T, true> : nmb_combine_rows_bulk<T, false>;
-      const size_t shared = (size_t)k * (loose ? fetched_bytes<true, T>(slab) : fetched_bytes<false, T>(slab));
-      kernel<<<dim3((unsigned)out->rows, (unsigned)((out->cols + slab - 1) / slab)), kBulkThreads, shared, s.stream>>>(
+      const int64_t bytes = k * (loose ? fetched_bytes<true, T>(slab) : fetched_bytes<false, T>(slab));
+      const int each = slab >= out->cols ? bulkTokens(out->rows, bytes, k, kBulkBytes) : 1;
+      kernel<<<dim3((unsigned)((out->rows + each - 1) / each), (unsigned)((out->cols + slab - 1) / slab)), kBulkThreads,
+               (size_t)(each * bytes), s.stream>>>(
           static_cast<const T *>(ys->data), ys->rows, ys->stride, (int)k, place, kept, weights, weightType,
-          static_cast<T *>(out->data), out->stride, out->cols, slab, boundsOf<T>(ys), status);
+          static_cast<T *>(out->data), out->rows, out->stride, out->cols, slab, each, boundsOf<T>(ys), status);
       return;
     }
     withElems<mostElems<T>()>(v, [&](auto V) {
@@ -1796,12 +1824,16 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_grad_device(void *queue, const GPU
     const int bits = laneBits(vecs, kThreadBits);
     const bool loose = v < mostElems<T>();
     if (const int slab = bulkSlab(dout->cols, dout->type, loose, k, (int)k + 1, kBulkGradBytes)) {
-      const auto kernel = loose ? nmb_combine_rows_grad_bulk<T, true> : nmb_combine_rows_grad_bulk<T, false>;
-      const size_t shared = (size_t)(k + 1) * (loose ? fetched_bytes<true, T>(slab) : fetched_bytes<false, T>(slab));
-      kernel<<<(unsigned)dout->rows, kBulkThreads, shared, s.stream>>>(
-          static_cast<const T *>(dout->data), dout->stride, static_cast<const T *>(ys->data), ys->rows, ys->stride,
+      // with one or two choices a thread needs half the registers of eight, and
+      // that many more blocks have their rows on the way
+      const auto kernel = k <= 2 ? (loose ? nmb_combine_rows_grad_bulk<T, true, 2> : nmb_combine_rows_grad_bulk<T, false, 2>)
+                                 : (loose ? nmb_combine_rows_grad_bulk<T, true, 8> : nmb_combine_rows_grad_bulk<T, false, 8>);
+      const int64_t bytes = (k + 1) * (loose ? fetched_bytes<true, T>(slab) : fetched_bytes<false, T>(slab));
+      const int each = slab >= dout->cols ? bulkTokens(dout->rows, bytes, k, kBulkGradBytes / 2) : 1;
+      kernel<<<(unsigned)((dout->rows + each - 1) / each), kBulkThreads, (size_t)(each * bytes), s.stream>>>(
+          static_cast<const T *>(dout->data), dout->rows, dout->stride, static_cast<const T *>(ys->data), ys->rows, ys->stride,
           (int)k, place, kept, weights, weightType, static_cast<T *>(dys->data), dys->rows, dys->stride, dweights,
-          dout->cols, slab, boundsOf<T>(dout), boundsOf<T>(ys), status);
+          dout->cols, slab, each, boundsOf<T>(dout), boundsOf<T>(ys), status);
       return;
     }
     withElems<mostElems<T>()>(v, [&](auto V) {
