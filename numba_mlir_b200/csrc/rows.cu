@@ -1118,11 +1118,17 @@ __global__ void __launch_bounds__(kBulkThreads)
 }
 
 // Elements of a slab where `rows` rows share `most` bytes: equal shares of the
-// row in as few slabs as that allows.  0: not by bulk copies (narrow rows, too
-// many choices).
+// row in as few slabs as that allows.  0: not by bulk copies (too many choices, or
+// rows so narrow that the registers' kernels are as fast).  30000 tokens, combine
+// and its gradient, registers against bulk: two rows of 512 bytes 9.4 and 17.6
+// against 10.9 and 21.7 us, of 768 bytes 17.4 and 49.3 (by four) against 13.9 and
+// 29.1; eight rows of 256 bytes 12.6 and 32.8 against 18.2 and 68.4, of 512 bytes
+// 36.1 and 58.6 against 28.8 and 52.4.  Off the words, where the registers take an
+// element at a time: two rows of 31 bf16 6.7 and 15.3 against 9.7 and 17.9, of 47
+// 11.0 and 30.1 against 10.7 and 19.2, of 259 42.5 and 122.2 against 18.1 and 29.6.
 int bulkSlab(int64_t cols, int type, bool loose, int64_t choices, int rows, int most) {
   const int size = elemBytes(type), step = loose ? 1 : 16 / size;
-  if (choices < 1 || choices > kBulkChoices || cols * size < kBulkLeast)
+  if (choices < 1 || choices > kBulkChoices || (loose ? cols < 48 : cols * size < (choices <= 2 ? 768 : 512)))
     return 0;
   const int64_t room = most / rows - (loose ? 32 : 0); // bytes of a row
   const int64_t slabs = (cols * size + room - 1) / room;
@@ -1142,20 +1148,22 @@ int bulkTokens(int64_t tokens, int64_t bytesEach, int64_t entriesEach, int most)
 }
 
 // ----------------------------------------------------------- combine_grad ---
-// The threads of a token read dout once for up to four choices, whose rows are
+// The threads of a token read dout once for up to N choices, whose rows are
 // in flight together; each keeps its share of their dot products, which meet at
 // the end in a fixed tree: shuffles that halve the values along with the lanes,
 // then the token's warps in order.
-constexpr int kChoices = 4;
-constexpr int kChoiceBits = 2;
-
-template <typename A> struct Choices {
-  int32_t at[kChoices];
-  A weight[kChoices];
+//
+// Two at a time for tokens of one or two choices, whose threads then hold half
+// as much and leave room for more blocks: 30000 tokens with two rows of 512
+// bytes 24.5 us by four, 17.6 us by two; with eight such rows 58.6 us by four,
+// 62.1 us by two.
+template <int N, typename A> struct Choices {
+  int32_t at[N];
+  A weight[N];
   __device__ __forceinline__ void read(const int32_t *__restrict__ place, const void *__restrict__ weights,
                                        int weight_type, int64_t entry, int64_t left) {
 #pragma unroll
-    for (int j = 0; j < kChoices; ++j) {
+    for (int j = 0; j < N; ++j) {
       at[j] = j < left ? __ldg(place + entry + j) : -1;
       weight[j] = weights && j < left ? scalar_at<A>(weights, weight_type, entry + j) : A(1);
     }
@@ -1187,33 +1195,35 @@ template <int N, typename A> __device__ __forceinline__ void meet(A (&v)[N], int
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, int N>
 __global__ void __launch_bounds__(kThreads, 4)
     nmb_combine_rows_grad(const T *__restrict__ dout, int64_t tokens, int64_t stride, const T *__restrict__ ys,
                           int64_t y_rows, int64_t y_stride, int64_t k, const int32_t *__restrict__ place,
                           const int32_t *__restrict__ kept, const void *__restrict__ weights, int weight_type,
                           T *__restrict__ dys, int64_t dy_rows, int64_t dy_stride, void *dweights, int64_t vecs,
                           int lane_bits) {
+  static_assert(N == 2 || N == 4, "the lanes' halvings are written for these");
+  constexpr int kBits = N / 2;
   using A = typename Acc<T>::type;
-  __shared__ A parts[kThreads / 32][kChoices];
+  __shared__ A parts[kThreads / 32][N];
   const int lanes = 1 << lane_bits;
   const int lane = threadIdx.x & (lanes - 1);
   const int64_t t = (int64_t)blockIdx.x * (kThreads >> lane_bits) + (threadIdx.x >> lane_bits);
   const bool token = t < tokens; // every thread stays for the shuffles and barriers
   const int64_t live = min((int64_t)__ldg(kept), y_rows);
-  Choices<A> c;
-  for (int64_t j0 = 0; j0 < k; j0 += kChoices) {
+  Choices<N, A> c;
+  for (int64_t j0 = 0; j0 < k; j0 += N) {
     c.read(place, weights, weight_type, t * k + j0, token ? k - j0 : 0);
-    A dot[kChoices] = {};
+    A dot[N] = {};
     for (int64_t col = token ? lane : vecs; col < vecs; col += lanes) {
       const Pack<T, V> d = load<T, V>(dout + t * stride + col * V);
-      Pack<T, V> y[kChoices];
+      Pack<T, V> y[N];
 #pragma unroll
-      for (int j = 0; j < kChoices; ++j)
+      for (int j = 0; j < N; ++j)
         if (c.at[j] >= 0 && c.at[j] < live)
           y[j] = load<T, V>(ys + c.at[j] * y_stride + col * V);
 #pragma unroll
-      for (int j = 0; j < kChoices; ++j)
+      for (int j = 0; j < N; ++j)
         if (c.at[j] >= 0 && c.at[j] < dy_rows) {
           Pack<T, V> r{};
           if (c.at[j] < live) {
@@ -1227,17 +1237,17 @@ __global__ void __launch_bounds__(kThreads, 4)
         }
     }
     meet(dot, lanes);
-    const int halvings = lane_bits < kChoiceBits ? lane_bits : kChoiceBits;
+    const int halvings = lane_bits < kBits ? lane_bits : kBits;
     int mine = 0; // the first of the values that this lane ends up with
     for (int b = 0; b < halvings; ++b)
-      mine |= (lane >> b & 1) << (kChoiceBits - 1 - b);
-    const int held = kChoices >> halvings;
+      mine |= (lane >> b & 1) << (kBits - 1 - b);
+    const int held = N >> halvings;
     if (lanes > 32) {
       const int warp = threadIdx.x >> 5;
-      if ((threadIdx.x & 31) < kChoices)
+      if ((threadIdx.x & 31) < N)
         parts[warp][mine] = dot[0];
       __syncthreads();
-      if (lane < kChoices) {
+      if (lane < N) {
         A sum = A(0);
         for (int w = 0; w < lanes / 32; ++w)
           sum += parts[warp + w][lane];
@@ -1247,7 +1257,7 @@ __global__ void __launch_bounds__(kThreads, 4)
       __syncthreads();
     } else if (token && lane < (1 << halvings) && dweights) {
 #pragma unroll
-      for (int i = 0; i < kChoices; ++i)
+      for (int i = 0; i < N; ++i)
         if (i < held && j0 + mine + i < k)
           set_scalar<A>(dweights, weight_type, t * k + j0 + mine + i, dot[i]);
     }
@@ -1256,15 +1266,19 @@ __global__ void __launch_bounds__(kThreads, 4)
 
 // The same with the rows fetched by bulk copies, dout's first.  A block takes a
 // whole token; columns beyond a slab come in turns through the same memory.
-template <typename T, bool LOOSE, int CHOICES>
+template <typename T, bool LOOSE>
 __global__ void __launch_bounds__(kBulkThreads)
-    nmb_combine_rows_grad_bulk(const T *__restrict__ dout, int64_t tokens, int64_t stride, const T *__restrict__ ys, int64_t y_rows,
-                               int64_t y_stride, int k, const int32_t *__restrict__ place,
+    nmb_combine_rows_grad_bulk(const T *__restrict__ dout, int64_t tokens, int64_t stride,
+                               const T *__restrict__ ys, int64_t y_rows, int64_t y_stride, int k, const int32_t *__restrict__ place,
                                const int32_t *__restrict__ kept, const void *__restrict__ weights, int weight_type,
                                T *__restrict__ dys, int64_t dy_rows, int64_t dy_stride, void *dweights, int64_t cols,
                                int slab, int each, const Bounds<T> dbounds, const Bounds<T> ybounds, uint32_t *status) {
   using A = typename Acc<T>::type;
   constexpr int V = kBulkElems<LOOSE, T>, kWarps = kBulkThreads / 32, kPairs = V > 1 ? V / 2 : 1;
+  // Choices read against dout at a time: what more of them hold in registers is
+  // blocks less on the way.  30000 tokens with eight rows of 1.5 KB took 149 us by
+  // two, 162 us by four, 236 us by eight.
+  constexpr int kTogether = 2;
   extern __shared__ __align__(128) unsigned char rows[]; // [each][1 + k] rows, dout's first
   __shared__ BulkChoices<A> c;
   __shared__ int begin[2 * kBulkChoices]; // where each row's first element is
@@ -1308,13 +1322,13 @@ __global__ void __launch_bounds__(kBulkThreads)
       return; // every thread gives up by itself: no barrier is left waiting
     const int row0 = token * (k + 1), entry0 = token * k;
     const T *drow = reinterpret_cast<const T *>(rows + row0 * bytes) + (LOOSE ? begin[row0] : 0);
-    for (int j0 = 0; j0 < k && token < here_tokens; j0 += CHOICES) {
-      int32_t to[CHOICES];
-      A w[CHOICES];
-      const T *yrow[CHOICES];
-      typename Two<A>::type dots[CHOICES] = {};
+    for (int j0 = 0; j0 < k && token < here_tokens; j0 += kTogether) {
+      int32_t to[kTogether];
+      A w[kTogether];
+      const T *yrow[kTogether];
+      typename Two<A>::type dots[kTogether] = {};
 #pragma unroll
-      for (int i = 0; i < CHOICES; ++i) {
+      for (int i = 0; i < kTogether; ++i) {
         to[i] = j0 + i < k ? c.at[entry0 + j0 + i] : -1;
         w[i] = j0 + i < k ? c.weight[entry0 + j0 + i] : A(0);
         yrow[i] = reinterpret_cast<const T *>(rows + (row0 + j0 + i + 1) * bytes);
@@ -1332,7 +1346,7 @@ __global__ void __launch_bounds__(kBulkThreads)
             d[e].x = up(x.v[0]);
         }
 #pragma unroll
-        for (int i = 0; i < CHOICES; ++i)
+        for (int i = 0; i < kTogether; ++i)
           if (to[i] >= 0) {
             Pack<T, V> r{};
             if (to[i] < live) {
@@ -1351,14 +1365,13 @@ __global__ void __launch_bounds__(kBulkThreads)
             store<T, V>(dys + to[i] * dy_stride + first + col, r);
           }
       }
-      A dot[CHOICES];
+      A dot[kTogether];
 #pragma unroll
-      for (int i = 0; i < CHOICES; ++i)
+      for (int i = 0; i < kTogether; ++i)
         dot[i] = dots[i].x + dots[i].y;
       meet(dot, 32);
-      const int which = CHOICES == 8 ? (lane & 1) << 2 | (lane & 2) | (lane & 4) >> 2 : lane & 1; // see meet
-      if (lane < CHOICES && j0 + which < k)
-        parts[warp][j0 + which] += dot[0];
+      if (lane < kTogether && j0 + lane < k) // see meet
+        parts[warp][j0 + lane] += dot[0];
     }
     __syncthreads(); // the slab's memory is free again, the sums are in place
   }
@@ -1824,12 +1837,9 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_grad_device(void *queue, const GPU
     const int bits = laneBits(vecs, kThreadBits);
     const bool loose = v < mostElems<T>();
     if (const int slab = bulkSlab(dout->cols, dout->type, loose, k, (int)k + 1, kBulkGradBytes)) {
-      // with one or two choices a thread needs half the registers of eight, and
-      // that many more blocks have their rows on the way
-      const auto kernel = k <= 2 ? (loose ? nmb_combine_rows_grad_bulk<T, true, 2> : nmb_combine_rows_grad_bulk<T, false, 2>)
-                                 : (loose ? nmb_combine_rows_grad_bulk<T, true, 8> : nmb_combine_rows_grad_bulk<T, false, 8>);
+      const auto kernel = loose ? nmb_combine_rows_grad_bulk<T, true> : nmb_combine_rows_grad_bulk<T, false>;
       const int64_t bytes = (k + 1) * (loose ? fetched_bytes<true, T>(slab) : fetched_bytes<false, T>(slab));
-      const int each = slab >= dout->cols ? bulkTokens(dout->rows, bytes, k, kBulkGradBytes / 2) : 1;
+      const int each = slab >= dout->cols ? bulkTokens(dout->rows, bytes, k, kBulkGradBytes) : 1;
       kernel<<<(unsigned)((dout->rows + each - 1) / each), kBulkThreads, (size_t)(each * bytes), s.stream>>>(
           static_cast<const T *>(dout->data), dout->rows, dout->stride, static_cast<const T *>(ys->data), ys->rows, ys->stride,
           (int)k, place, kept, weights, weightType, static_cast<T *>(dys->data), dys->rows, dys->stride, dweights,
@@ -1837,7 +1847,8 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_grad_device(void *queue, const GPU
       return;
     }
     withElems<mostElems<T>()>(v, [&](auto V) {
-      nmb_combine_rows_grad<T, V.value><<<blocksFor(dout->rows, bits), kThreads, 0, s.stream>>>(
+      const auto kernel = k <= 2 ? nmb_combine_rows_grad<T, V.value, 2> : nmb_combine_rows_grad<T, V.value, 4>;
+      kernel<<<blocksFor(dout->rows, bits), kThreads, 0, s.stream>>>(
           static_cast<const T *>(dout->data), dout->rows, dout->stride, static_cast<const T *>(ys->data), ys->rows,
           ys->stride, k, place, kept, weights, weightType, static_cast<T *>(dys->data), dys->rows, dys->stride,
           dweights, vecs, bits);
