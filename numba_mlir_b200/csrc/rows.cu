@@ -1037,12 +1037,13 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// The same with the rows fetched by bulk copies: a block takes a token (or a
-// slab of its columns), brings the rows of all its choices into shared memory
-// at once and adds them up from there.  Copies in flight cost no registers: with
+// The same with the rows fetched by bulk copies: a block takes a token, a few of
+// narrow rows or a slab of its columns, brings the rows of all their choices into
+// shared memory at once and adds them up from there.  Copies in flight cost no registers: with
 // the rows in registers eight choices left room for one block a multiprocessor,
 // and batches of four reached 4.5 of the 6.5 TB/s that a copy reaches.
 constexpr int kBulkThreads = 128;
+constexpr int kBulkBits = 7;
 constexpr int kBulkChoices = 32;        // most choices of a token
 // Most bytes in flight per block.  combine: 16384 tokens with eight rows of 4 KB
 // took 94.5 us at 16 KB (two slabs a token), 98.1 us at 32 KB.  combine_grad: a
@@ -1061,15 +1062,15 @@ __global__ void __launch_bounds__(kBulkThreads)
     nmb_combine_rows_bulk(const T *__restrict__ ys, int64_t y_rows, int64_t stride, int k,
                           const int32_t *__restrict__ place, const int32_t *__restrict__ kept,
                           const void *__restrict__ weights, int weight_type, T *__restrict__ out, int64_t tokens,
-                          int64_t out_stride, int64_t cols, int slab, int each, const Bounds<T> bounds,
+                          int64_t out_stride, int64_t cols, int slab, int each_bits, const Bounds<T> bounds,
                           uint32_t *status) {
   using A = typename Acc<T>::type;
   constexpr int V = kBulkElems<LOOSE, T>;
-  extern __shared__ __align__(128) unsigned char rows[]; // [each][k] rows
+  extern __shared__ __align__(128) unsigned char rows[]; // [1 << each_bits][k] rows
   __shared__ BulkChoices<A> c;
-  const int64_t t0 = (int64_t)blockIdx.x * each, first = (int64_t)blockIdx.y * slab;
+  const int64_t t0 = (int64_t)blockIdx.x << each_bits, first = (int64_t)blockIdx.y * slab;
   const int here = (int)min((int64_t)slab, cols - first), bytes = fetched_bytes<LOOSE, T>(slab);
-  const int entries = k * (int)min((int64_t)each, tokens - t0);
+  const int entries = k * (int)min((int64_t)1 << each_bits, tokens - t0);
   const int j = threadIdx.x;
   int32_t at = -1;
   if (j < entries) {
@@ -1093,13 +1094,13 @@ __global__ void __launch_bounds__(kBulkThreads)
   __syncthreads();
   if (!bulk_arrived(&c.bar, 0, status))
     return;
-  const int threads = kBulkThreads / each, token = j / threads; // of a token
+  const int bits = kBulkBits - each_bits, threads = 1 << bits, token = j >> bits; // a token's threads
   if (t0 + token >= tokens)
     return;
   const int32_t *begin = c.at + token * k;
   const A *weight = c.weight + token * k;
   T *dst = out + (t0 + token) * out_stride + first;
-  for (int col = (j - token * threads) * V; col < here; col += threads * V) {
+  for (int col = (j & (threads - 1)) * V; col < here; col += threads * V) {
     A sum[V] = {};
 #pragma unroll 4
     for (int i = 0; i < k; ++i)
@@ -1136,15 +1137,15 @@ int bulkSlab(int64_t cols, int type, bool loose, int64_t choices, int rows, int 
   return slabs <= 65535 ? (int)slab : 0;
 }
 
-// Tokens of a block where their rows are so narrow that a block of one token is
-// mostly its own beginning: up to four, as long as `most` bytes and the choices
-// hold them and four blocks a multiprocessor are left.  30000 tokens with two
-// rows of 1 KB took 29.2 us with a block each.
-int bulkTokens(int64_t tokens, int64_t bytesEach, int64_t entriesEach, int most) {
-  int each = 4;
-  while (each > 1 && (each * bytesEach > most || each * entriesEach > kBulkChoices || tokens / each < 148 * 4))
-    each /= 2;
-  return each;
+// Tokens of a block (their log2) where their rows are so narrow that a block of
+// one token is mostly its own beginning: up to four, as long as `most` bytes and
+// the choices hold them and four blocks a multiprocessor are left.  30000 tokens
+// with two rows of 1 KB: 16.6 us by four, 29.2 us by one.
+int bulkTokens(int64_t tokens, int64_t bytesEach, int64_t choices, int most) {
+  int bits = 2;
+  while (bits > 0 && (bytesEach << bits > most || choices << bits > kBulkChoices || tokens >> bits < 148 * 4))
+    --bits;
+  return bits;
 }
 
 // ----------------------------------------------------------- combine_grad ---
@@ -1264,29 +1265,31 @@ __global__ void __launch_bounds__(kThreads, 4)
   }
 }
 
-// The same with the rows fetched by bulk copies, dout's first.  A block takes a
-// whole token; columns beyond a slab come in turns through the same memory.
+// The same with the rows fetched by bulk copies, dout's first.  A block takes
+// whole tokens; columns beyond a slab come in turns through the same memory.
 template <typename T, bool LOOSE>
 __global__ void __launch_bounds__(kBulkThreads)
     nmb_combine_rows_grad_bulk(const T *__restrict__ dout, int64_t tokens, int64_t stride,
                                const T *__restrict__ ys, int64_t y_rows, int64_t y_stride, int k, const int32_t *__restrict__ place,
                                const int32_t *__restrict__ kept, const void *__restrict__ weights, int weight_type,
                                T *__restrict__ dys, int64_t dy_rows, int64_t dy_stride, void *dweights, int64_t cols,
-                               int slab, int each, const Bounds<T> dbounds, const Bounds<T> ybounds, uint32_t *status) {
+                               int slab, int each_bits, const Bounds<T> dbounds, const Bounds<T> ybounds,
+                               uint32_t *status) {
   using A = typename Acc<T>::type;
   constexpr int V = kBulkElems<LOOSE, T>, kWarps = kBulkThreads / 32, kPairs = V > 1 ? V / 2 : 1;
   // Choices read against dout at a time: what more of them hold in registers is
   // blocks less on the way.  30000 tokens with eight rows of 1.5 KB took 149 us by
   // two, 162 us by four, 236 us by eight.
   constexpr int kTogether = 2;
-  extern __shared__ __align__(128) unsigned char rows[]; // [each][1 + k] rows, dout's first
+  extern __shared__ __align__(128) unsigned char rows[]; // [1 << each_bits][1 + k] rows, dout's first
   __shared__ BulkChoices<A> c;
   __shared__ int begin[2 * kBulkChoices]; // where each row's first element is
   __shared__ A parts[kWarps][kBulkChoices];
-  const int64_t t0 = (int64_t)blockIdx.x * each;
+  const int64_t t0 = (int64_t)blockIdx.x << each_bits;
   const int j = threadIdx.x, lane = j & 31, warp = j >> 5, bytes = fetched_bytes<LOOSE, T>(slab);
-  const int here_tokens = (int)min((int64_t)each, tokens - t0), entries = here_tokens * k;
-  const int threads = kBulkThreads / each, token = j / threads, mine = j - token * threads; // a token's threads
+  const int here_tokens = (int)min((int64_t)1 << each_bits, tokens - t0), entries = here_tokens * k;
+  const int bits = kBulkBits - each_bits, threads = 1 << bits; // a token's threads
+  const int token = j >> bits, mine = j & (threads - 1);
   const int64_t live = min((int64_t)__ldg(kept), y_rows);
   // thread j fetches dout's row of a token or that of a choice
   const int fetches = here_tokens * (k + 1), ftoken = j / (k + 1), fchoice = j - ftoken * (k + 1) - 1;
@@ -1377,7 +1380,7 @@ __global__ void __launch_bounds__(kBulkThreads)
   }
   if (j < entries && dweights) {
     // a token's warps in order
-    const int of = j / k, warps = kWarps / each;
+    const int of = j / k, warps = kWarps >> each_bits;
     A sum = A(0);
     for (int w = 0; w < warps; ++w)
       sum += parts[of * warps + w][j - of * k];
@@ -1797,11 +1800,11 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows
     if (const int slab = bulkSlab(out->cols, out->type, loose, k, (int)k, kBulkBytes)) {
       const auto kernel = loose ? nmb_combine_rows_bulk<T, true> : nmb_combine_rows_bulk<T, false>;
       const int64_t bytes = k * (loose ? fetched_bytes<true, T>(slab) : fetched_bytes<false, T>(slab));
-      const int each = slab >= out->cols ? bulkTokens(out->rows, bytes, k, kBulkBytes) : 1;
-      kernel<<<dim3((unsigned)((out->rows + each - 1) / each), (unsigned)((out->cols + slab - 1) / slab)), kBulkThreads,
-               (size_t)(each * bytes), s.stream>>>(
+      const int many = slab >= out->cols ? bulkTokens(out->rows, bytes, k, kBulkBytes) : 0;
+      kernel<<<dim3((unsigned)((out->rows + (1 << many) - 1) >> many), (unsigned)((out->cols + slab - 1) / slab)), kBulkThreads,
+               (size_t)(bytes << many), s.stream>>>(
           static_cast<const T *>(ys->data), ys->rows, ys->stride, (int)k, place, kept, weights, weightType,
-          static_cast<T *>(out->data), out->rows, out->stride, out->cols, slab, each, boundsOf<T>(ys), status);
+          static_cast<T *>(out->data), out->rows, out->stride, out->cols, slab, many, boundsOf<T>(ys), status);
       return;
     }
     withElems<mostElems<T>()>(v, [&](auto V) {
@@ -1839,11 +1842,11 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_grad_device(void *queue, const GPU
     if (const int slab = bulkSlab(dout->cols, dout->type, loose, k, (int)k + 1, kBulkGradBytes)) {
       const auto kernel = loose ? nmb_combine_rows_grad_bulk<T, true> : nmb_combine_rows_grad_bulk<T, false>;
       const int64_t bytes = (k + 1) * (loose ? fetched_bytes<true, T>(slab) : fetched_bytes<false, T>(slab));
-      const int each = slab >= dout->cols ? bulkTokens(dout->rows, bytes, k, kBulkGradBytes) : 1;
-      kernel<<<(unsigned)((dout->rows + each - 1) / each), kBulkThreads, (size_t)(each * bytes), s.stream>>>(
+      const int many = slab >= dout->cols ? bulkTokens(dout->rows, bytes, k, kBulkGradBytes) : 0;
+      kernel<<<(unsigned)((dout->rows + (1 << many) - 1) >> many), kBulkThreads, (size_t)(bytes << many), s.stream>>>(
           static_cast<const T *>(dout->data), dout->rows, dout->stride, static_cast<const T *>(ys->data), ys->rows, ys->stride,
           (int)k, place, kept, weights, weightType, static_cast<T *>(dys->data), dys->rows, dys->stride, dweights,
-          dout->cols, slab, each, boundsOf<T>(dout), boundsOf<T>(ys), status);
+          dout->cols, slab, many, boundsOf<T>(dout), boundsOf<T>(ys), status);
       return;
     }
     withElems<mostElems<T>()>(v, [&](auto V) {
