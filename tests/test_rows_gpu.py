@@ -363,6 +363,49 @@ def test_combine_rows_grad(queue, name, tokens, k, groups, dim, pad):
     assert_near(dw.copy_to_host().astype(np.float64), terms.sum(-1), (dim + 1) * u * np.abs(terms).sum(-1), "float32")
 
 
+# Narrow rows of many tokens: two or four tokens share a block, the last block has
+# fewer; widths on both sides of where the bulk copies begin.
+SHARED = [(2371, 2, 16, 400, 0), (2369, 1, 5, 520, 8), (1187, 3, 16, 264, 0), (2371, 8, 9, 256, 0), (2370, 2, 16, 99, 0),
+          (1187, 4, 9, 48, 1), (2371, 2, 16, 47, 0), (2371, 5, 9, 515, 0), (2375, 9, 10, 128, 0), (1186, 12, 13, 72, 1)]
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("tokens,k,groups,dim,pad", SHARED)
+def test_tokens_that_share_a_block(queue, name, tokens, k, groups, dim, pad):
+    test_combine_rows(queue, name, tokens, k, groups, dim, pad)
+    test_combine_rows_grad(queue, name, tokens, k, groups, dim, pad)
+
+
+@pytest.mark.parametrize("tokens,k,dim", [(2371, 2, 512), (2371, 2, 515), (2370, 3, 264), (1187, 1, 99), (2371, 2, 64)])
+def test_memory_around_the_results_is_left_alone(queue, tokens, k, dim):
+    """Results are parts of larger arrays whose other rows and columns keep what
+    they hold, bit for bit, also behind the last token of a shared block."""
+    import numba_mlir_b200 as nm
+
+    rng = np.random.default_rng(tokens + dim)
+    ids = route(tokens, k, 9, rng)
+    plan = plan_on_device(ids, 9)
+    ys = dev(rng.standard_normal((tokens * k, dim)).astype(np.float32))
+    dout = dev(rng.standard_normal((tokens, dim)).astype(np.float32))
+    w = dev(rng.random((tokens, k)).astype(np.float32))
+    whole = {n: dev(np.full((rows + 7, dim + 9), -7.5, np.float32)) for n, rows in (("out", tokens), ("dys", tokens * k))}
+    dwhole = dev(np.full((tokens + 7, k), -7.5, np.float32))
+    parts = {"out": whole["out"][3:3 + tokens, 5:5 + dim], "dys": whole["dys"][3:3 + tokens * k, 5:5 + dim]}
+    nm.combine_rows(ys, plan, w, out=parts["out"])
+    nm.combine_rows_grad(dout, ys, plan, w, out=parts["dys"], dweights=dwhole[3:3 + tokens])
+    for n, rows in (("out", tokens), ("dys", tokens * k)):
+        got = whole[n].copy_to_host()
+        inside = got[3:3 + rows, 5:5 + dim].copy()
+        assert not (inside == -7.5).any()
+        got[3:3 + rows, 5:5 + dim] = -7.5
+        assert (got == -7.5).all()
+    got = dwhole.copy_to_host()
+    assert (got[:3] == -7.5).all() and (got[3 + tokens:] == -7.5).all() and not (got[3:3 + tokens] == -7.5).any()
+    # the same call once more gives the same bits (one with another alignment may add in another order)
+    again = nm.combine_rows_grad(dout, ys, plan, w, out=parts["dys"])[1].copy_to_host()
+    assert again.tobytes() == got[3:3 + tokens].tobytes()
+
+
 @pytest.mark.parametrize("wname", ["float16", "bfloat16", "float64"])
 def test_weights_of_other_types(queue, wname):
     import numba_mlir_b200 as nm
