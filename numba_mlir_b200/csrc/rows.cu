@@ -1048,8 +1048,10 @@ constexpr int kBulkThreads = 128;
 constexpr int kBulkBits = 7;
 constexpr int kBulkChoices = 32;        // most choices of a token
 // Most bytes in flight per block.  combine: 16384 tokens with eight rows of 4 KB
-// took 94.5 us at 16 KB (two slabs a token), 98.1 us at 32 KB.  combine_grad: a
-// token with eight such rows 175.7 us in one turn of 36 KB, 203 us in two.
+// took 92.1 us at 16 KB (two slabs a token), 95.8 us at 32 KB.  combine_grad: a
+// token with eight such rows 173.5 us in one turn of 36 KB or in two of half of
+// it; 30000 tokens with two rows of 2 KB, which share blocks where they fit,
+// 49.8 us at 45 KB, 56.3 us at half.
 constexpr int kBulkBytes = 16384, kBulkGradBytes = 46080;
 
 // What the threads of a block share about a token's choices.
@@ -1142,7 +1144,7 @@ int bulkSlab(int64_t cols, int type, bool loose, int64_t choices, int rows, int 
 // Tokens of a block (their log2) where their rows are so narrow that a block of
 // one token is mostly its own beginning: up to four, as long as `most` bytes and
 // the choices hold them and four blocks a multiprocessor are left.  30000 tokens
-// with two rows of 1 KB: 16.6 us by four, 29.2 us by one.
+// with two rows of 1 KB: 15.6 us by four, 29.2 us by one.
 int bulkTokens(int64_t tokens, int64_t bytesEach, int64_t choices, int most) {
   int bits = 2;
   while (bits > 0 && (bytesEach << bits > most || choices << bits > kBulkChoices || tokens >> bits < 148 * 4))
