@@ -284,7 +284,7 @@ struct Pass {
   int64_t n;
   int blocks, shift, bins, digit_bits;
   // an entry's key in two steps: what is read, and what is made of it
-  __device__ __forceinline__ int64_t raw(int64_t i) const { return keysIn ? (int64_t)keysIn[i] : ids.raw(i); }
+  __device__ __forceinline__ int64_t raw(int64_t i) const { return keysIn ? (int64_t)nmb::rows::made(keysIn + i) : ids.raw(i); }
   __device__ __forceinline__ uint32_t cooked(int64_t id) const { return ids.cooked(id); }
   __device__ __forceinline__ uint32_t key(int64_t i) const { return cooked(raw(i)); }
   __device__ __forceinline__ uint32_t digit(uint32_t k) const { return (k >> shift) & (uint32_t)(bins - 1); }
@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kThreads)
   auto read_counts = [&](int b0) {
 #pragma unroll
     for (int u = 0; u < 16; ++u)
-      c[u] = b0 + u * share < p.blocks ? __ldg(from + (int64_t)(b0 + u * share) * pairs) : 0;
+      c[u] = b0 + u * share < p.blocks ? nmb::rows::made(from + (int64_t)(b0 + u * share) * pairs) : 0;
   };
   if (!p.added)
     read_counts(part);
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kThreads)
   for (int u = 0; u < PER; ++u) {
     const int64_t i = begin + u * 32;
     id[u] = i < p.n ? p.raw(i) : 0;
-    entry[u] = i < p.n && p.entriesIn ? p.entriesIn[i] : (int32_t)i;
+    entry[u] = i < p.n && p.entriesIn ? nmb::rows::made(p.entriesIn + i) : (int32_t)i;
   }
   if (!p.added) {
     uint2 mine = make_uint2(0, 0), all = make_uint2(0, 0);

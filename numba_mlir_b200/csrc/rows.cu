@@ -33,6 +33,7 @@ using nmb::rows::checkRows;
 using nmb::rows::elemBytes;
 using nmb::rows::laneBits;
 using nmb::rows::launched;
+using nmb::rows::made;
 using nmb::rows::Stream;
 
 constexpr int kThreads = 256;
@@ -363,11 +364,10 @@ struct GradPlan {
   uint32_t *status;
 };
 
-__device__ __forceinline__ int64_t lower_bound(const uint32_t *__restrict__ keys, int64_t lo, int64_t hi,
-                                               uint32_t key) {
+__device__ __forceinline__ int64_t lower_bound(const uint32_t *keys, int64_t lo, int64_t hi, uint32_t key) {
   while (lo < hi) {
     const int64_t mid = (lo + hi) / 2;
-    if (__ldg(keys + mid) < key)
+    if (made(keys + mid) < key)
       lo = mid + 1;
     else
       hi = mid;
@@ -377,12 +377,11 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t *__restrict__ keys
 
 // The same for a warp that looks for one key: 32 places at a time, so four
 // dependent reads where halving takes fifteen (an L2 access is about 0.4 us).
-__device__ __forceinline__ int64_t warp_lower_bound(const uint32_t *__restrict__ keys, int64_t lo, int64_t hi,
-                                                    uint32_t key) {
+__device__ __forceinline__ int64_t warp_lower_bound(const uint32_t *keys, int64_t lo, int64_t hi, uint32_t key) {
   const int lane = threadIdx.x & 31;
   while (lo < hi) {
     const int64_t step = (hi - lo + 31) / 32, at = lo + lane * step;
-    const int below = __popc(__ballot_sync(kAll, at < hi && __ldg(keys + (at < hi ? at : lo)) < key));
+    const int below = __popc(__ballot_sync(kAll, at < hi && made(keys + (at < hi ? at : lo)) < key));
     if (below == 0)
       return lo;
     hi = min(hi, lo + below * step);
@@ -395,33 +394,33 @@ __device__ __forceinline__ int64_t warp_lower_bound(const uint32_t *__restrict__
 // that keys[at - 1] belongs to, for the threads of a warp or for one.  Most runs
 // end nearby: a warp looks at 1024 places first (two reads), a thread at ever
 // longer steps.
-__device__ __forceinline__ int64_t warp_run_end(const uint32_t *__restrict__ keys, int64_t at, int64_t n, uint32_t key) {
+__device__ __forceinline__ int64_t warp_run_end(const uint32_t *keys, int64_t at, int64_t n, uint32_t key) {
   const int64_t probe = at + (threadIdx.x & 31) * 32 + 31;
-  const unsigned past = __ballot_sync(kAll, probe >= n || __ldg(keys + (probe < n ? probe : at)) != key);
+  const unsigned past = __ballot_sync(kAll, probe >= n || made(keys + (probe < n ? probe : at)) != key);
   if (past == 0)
     return warp_lower_bound(keys, at + 1024, n, key + 1);
   const int64_t first = at + (int64_t)(__ffs(past) - 1) * 32, place = first + (threadIdx.x & 31);
-  return first + __popc(__ballot_sync(kAll, place < n && __ldg(keys + (place < n ? place : at)) == key));
+  return first + __popc(__ballot_sync(kAll, place < n && made(keys + (place < n ? place : at)) == key));
 }
-__device__ __forceinline__ int64_t warp_run_begin(const uint32_t *__restrict__ keys, int64_t at, uint32_t key) {
+__device__ __forceinline__ int64_t warp_run_begin(const uint32_t *keys, int64_t at, uint32_t key) {
   const int64_t probe = at - 32 - (threadIdx.x & 31) * 32;
-  const unsigned past = __ballot_sync(kAll, probe < 0 || __ldg(keys + (probe < 0 ? at - 1 : probe)) != key);
+  const unsigned past = __ballot_sync(kAll, probe < 0 || made(keys + (probe < 0 ? at - 1 : probe)) != key);
   if (past == 0)
     return warp_lower_bound(keys, 0, at - 1024, key);
   const int64_t last = at - (int64_t)(__ffs(past) - 1) * 32, place = last - 1 - (threadIdx.x & 31);
-  return last - __popc(__ballot_sync(kAll, place >= 0 && __ldg(keys + (place < 0 ? at - 1 : place)) == key));
+  return last - __popc(__ballot_sync(kAll, place >= 0 && made(keys + (place < 0 ? at - 1 : place)) == key));
 }
-__device__ __forceinline__ int64_t run_end(const uint32_t *__restrict__ keys, int64_t at, int64_t n, uint32_t key) {
+__device__ __forceinline__ int64_t run_end(const uint32_t *keys, int64_t at, int64_t n, uint32_t key) {
   int64_t step = 1;
-  while (at + step < n && __ldg(keys + at + step) == key) {
+  while (at + step < n && made(keys + at + step) == key) {
     at += step;
     step *= 2;
   }
   return lower_bound(keys, at, min(at + step, n), key + 1);
 }
-__device__ __forceinline__ int64_t run_begin(const uint32_t *__restrict__ keys, int64_t at, uint32_t key) {
+__device__ __forceinline__ int64_t run_begin(const uint32_t *keys, int64_t at, uint32_t key) {
   int64_t step = 1;
-  while (at - step >= 0 && __ldg(keys + at - step) == key) {
+  while (at - step >= 0 && made(keys + at - step) == key) {
     at -= step;
     step *= 2;
   }
@@ -610,8 +609,8 @@ __device__ __forceinline__ void walk_registers(const I *__restrict__ src, int64_
 #pragma unroll
   for (int u = 0; u < kGradBatch; ++u)
     if (u < count) {
-      at[u] = __ldg(p.order + w.at(u));
-      key[u] = __ldg(p.keys + w.at(u));
+      at[u] = made(p.order + w.at(u));
+      key[u] = made(p.keys + w.at(u));
     }
   for (int64_t i = 0; i < count; i += kGradBatch) {
     Pack<I, V> x[kGradBatch];
@@ -623,8 +622,8 @@ __device__ __forceinline__ void walk_registers(const I *__restrict__ src, int64_
     for (int u = 0; u < kGradBatch; ++u) {
       next[u] = key[u];
       if (i + kGradBatch + u < count) {
-        at[u] = __ldg(p.order + w.at(i + kGradBatch + u));
-        key[u] = __ldg(p.keys + w.at(i + kGradBatch + u));
+        at[u] = made(p.order + w.at(i + kGradBatch + u));
+        key[u] = made(p.keys + w.at(i + kGradBatch + u));
       }
     }
     add_rows<false>(x, next, (int)min((int64_t)kGradBatch, count - i), column, row, sum);
@@ -655,8 +654,8 @@ __device__ __forceinline__ bool walk_bulk(const I *__restrict__ src, int64_t str
   auto look = [&](int64_t turn) { // the entry that this thread fetches in a turn
     const int64_t i = turn * kTurnRows + r;
     if (r < kTurnRows && i < count) {
-      at = __ldg(p.order + w.at(i));
-      key = __ldg(p.keys + w.at(i));
+      at = made(p.order + w.at(i));
+      key = made(p.keys + w.at(i));
     }
   };
   auto fetch = [&](int64_t turn) {
@@ -768,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, BULK ? 4 : 3)
       bool absent = v < p.to_clear;
       if (absent) {
         const int64_t at = lower_bound(p.keys, lo, hi, (uint32_t)v);
-        absent = at >= hi || __ldg(p.keys + at) != (uint32_t)v;
+        absent = at >= hi || made(p.keys + at) != (uint32_t)v;
       }
       const uint32_t mask = __ballot_sync(kAll, absent);
       if (threadIdx.x == 0)
@@ -793,9 +792,9 @@ __global__ void __launch_bounds__(kThreads, BULK ? 4 : 3)
   if (begin >= p.n)
     return;
   const int64_t end = min(begin + p.span, p.n);
-  const uint32_t first_key = __ldg(p.keys + begin), last_key = __ldg(p.keys + end - 1);
-  const uint32_t prev_key = begin > 0 ? __ldg(p.keys + begin - 1) : 0xffffffffu;
-  const uint32_t next_key = end < p.n ? __ldg(p.keys + end) : 0xffffffffu;
+  const uint32_t first_key = made(p.keys + begin), last_key = made(p.keys + end - 1);
+  const uint32_t prev_key = begin > 0 ? made(p.keys + begin - 1) : 0xffffffffu;
+  const uint32_t next_key = end < p.n ? made(p.keys + end) : 0xffffffffu;
   if (first_key >= rows)
     return;
   const GradColumn<O, V, ADD, LOOSE, A> column{out + col, out_stride, scale, active, active ? mine : 0, group.lanes};
@@ -821,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, BULK ? 4 : 3)
       walk.tail = end + inner * p.span;
     }
   }
-  uint32_t row = __ldg(p.keys + walk.begin);
+  uint32_t row = made(p.keys + walk.begin);
   Sums<A, V> sum;
   sum.clear();
   if constexpr (BULK) {
@@ -887,14 +886,14 @@ int gradSpan(int64_t n, int64_t vecs) {
 template <typename U, int V>
 __global__ void __launch_bounds__(kThreads)
     nmb_dispatch_rows(const U *__restrict__ x, int64_t tokens, int64_t stride, int64_t k,
-                      const int32_t *__restrict__ place, const int32_t *__restrict__ kept, U *__restrict__ out,
+                      const int32_t *place, const int32_t *kept, U *__restrict__ out,
                       int64_t out_rows, int64_t out_stride, int64_t vecs, int lane_bits) {
   const int lane = threadIdx.x & ((1 << lane_bits) - 1);
   const int64_t t = (int64_t)blockIdx.x * (kThreads >> lane_bits) + (threadIdx.x >> lane_bits);
   nmb::rows::wait_for_previous();
   if (t >= tokens)
     return;
-  const int64_t live = *kept;
+  const int64_t live = made(kept);
   for (int64_t c = lane; c < vecs; c += 1 << lane_bits) {
     const Pack<U, V> row = load<U, V>(x + t * stride + c * V);
 #pragma unroll 4
@@ -911,8 +910,8 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kCopyThreads = 128, kCopyBytes = 8192;
 template <typename U>
 __global__ void __launch_bounds__(kCopyThreads)
-    nmb_dispatch_rows_bulk(const U *__restrict__ x, int64_t stride, int64_t k, const int32_t *__restrict__ place,
-                           const int32_t *__restrict__ kept, U *__restrict__ out, int64_t out_rows, int64_t out_stride,
+    nmb_dispatch_rows_bulk(const U *__restrict__ x, int64_t stride, int64_t k, const int32_t *place,
+                           const int32_t *kept, U *__restrict__ out, int64_t out_rows, int64_t out_stride,
                            int64_t cols, int slab, const Bounds<U> bounds, uint32_t *status) {
   extern __shared__ __align__(128) unsigned char memory[];
   __shared__ uint64_t bar;
@@ -926,12 +925,12 @@ __global__ void __launch_bounds__(kCopyThreads)
     begin = fetch_row<true>(x + t * stride + first, here, memory, &bar, bounds);
   }
   __syncthreads();
-  const int64_t live = __ldg(kept);
+  const int64_t live = made(kept);
   if (!bulk_arrived(&bar, 0, status))
     return;
   const U *row = reinterpret_cast<const U *>(memory) + begin;
   for (int64_t j = 0; j < k; ++j) {
-    const int64_t at = __ldg(place + t * k + j);
+    const int64_t at = place[t * k + j];
     if (at < 0 || at >= out_rows)
       continue;
     U *to = out + at * out_stride + first;

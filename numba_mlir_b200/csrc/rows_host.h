@@ -127,6 +127,12 @@ inline void launchBehind(K kernel, dim3 grid, unsigned threads, size_t shared, c
 // launched behind another waits for it: so a wait covers all kernels before.
 __device__ __forceinline__ void let_next_begin() { cudaTriggerProgrammaticLaunchCompletion(); }
 __device__ __forceinline__ void wait_for_previous() { cudaGridDependencySynchronize(); }
+// What the kernels before this one of the same call have written.  This kernel's
+// blocks may be on their multiprocessors while it is being written, so it is never
+// read through the read-only path (__ldg, or a pointer that is const and
+// __restrict__), which is for memory that nobody writes while the kernel lives:
+// from L2, where those writes are.
+template <typename T> __device__ __forceinline__ T made(const T *p) { return __ldcg(p); }
 #endif
 
 // Lets a kernel use more than 48 KB of shared memory; once per kernel and device.

@@ -1,0 +1,62 @@
+"""Rules on memory that the kernels of the row operators keep, read from their
+source: a kernel that is on the multiprocessors while another writes what it
+reads, and copies that the two proxies of shared memory make, go wrong too rarely
+for a run to show it."""
+
+import os
+import re
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "numba_mlir_b200", "csrc")
+
+
+def source(name):
+    with open(os.path.join(CSRC, name)) as f:
+        return re.sub(r"//[^\n]*", "", f.read())
+
+
+def functions(text):
+    """name -> (parameters, body) of the functions at the top of a file and of
+    the structs in it."""
+    found = {}
+    for m in re.finditer(r"(\w+)\s*\(", text):
+        at = close(text, m.end() - 1, "()")
+        rest = re.match(r"\s*(const)?\s*(:[^{;]*)?\{", text[at:])
+        if rest and m.group(1) not in ("if", "for", "while", "switch"):
+            begin = at + rest.end() - 1
+            found[m.group(1)] = (text[m.end():at - 1], text[begin:close(text, begin, "{}")])
+    return found
+
+
+def close(text, at, pair):
+    depth = 0
+    for i in range(at, len(text)):
+        depth += (text[i] == pair[0]) - (text[i] == pair[1])
+        if depth == 0:
+            return i + 1
+    raise AssertionError("unbalanced")
+
+
+# what the sort's kernels leave for the kernels behind them
+MADE = ("keys", "order", "place", "kept", "counts", "from", "keysIn", "entriesIn", "p.keys", "p.order", "p.counts")
+
+
+@pytest.mark.parametrize("file", ["rows.cu", "row_sort.cu"])
+def test_what_a_predecessor_writes_is_not_read_as_constant(file):
+    every = functions(source(file))
+    behind = {n: f for n, f in every.items() if "wait_for_previous()" in f[1]}
+    assert {"rows.cu": {"nmb_take_rows_grad", "nmb_dispatch_rows", "nmb_dispatch_rows_bulk"},
+            "row_sort.cu": {"nmb_sort_scatter"}}[file] == set(behind)
+    # the functions that those call, and what those call
+    reached, new = dict(behind), dict(behind)
+    while new:
+        called = {n: f for n, f in every.items() for _, body in new.values() if re.search(rf"\b{n}\b\s*[<(]", body)}
+        new = {n: f for n, f in called.items() if n not in reached}
+        reached.update(new)
+    for name, (params, body) in reached.items():
+        for m in re.finditer(r"__ldg\(", body):
+            read = body[m.end():close(body, m.end() - 1, "()") - 1]
+            assert not re.match(rf"({'|'.join(map(re.escape, MADE))})\b", read.strip()), f"{name}: __ldg({read})"
+        for m in re.finditer(r"const\s+\w+\s*\*\s*__restrict__\s*(\w+)", params):
+            assert m.group(1) not in MADE, f"{name}: {m.group(0)}"
