@@ -177,7 +177,9 @@ __device__ __forceinline__ bool bulk_arrived(uint64_t *bar, uint32_t phase, uint
 // A row's way into shared memory, issued by one thread: a bulk copy starts and
 // ends on 16-byte boundaries.  LOOSE rows do not: the words they lie in are copied
 // as a whole, neighbours' elements included, as far as the operand's memory
-// reaches; elements in the words at its very ends are copied one by one.  Returns
+// reaches; elements in the words at its very ends are copied one by one.  Those are
+// ordinary stores: a thread that fetches into the same place again puts
+// nmb::fence_async_smem in front, or the next copy may land before them.  Returns
 // the place of the row's first element in `to`.
 template <typename T> struct Bounds {
   const T *lo, *hi; // the operand's memory
@@ -662,6 +664,8 @@ __device__ __forceinline__ bool walk_bulk(const I *__restrict__ src, int64_t str
     if (r >= kTurnRows)
       return;
     const int b = (int)(turn & 1);
+    if (LOOSE && turn > 1)
+      nmb::fence_async_smem();
     if (turn * kTurnRows + r < count) {
       turns.key[b][r] = key;
       turns.begin[b][r] = fetch_row<LOOSE>(src + (int64_t)at * stride, here, memory + (b * kTurnRows + r) * bytes,
@@ -1315,6 +1319,8 @@ __global__ void __launch_bounds__(kBulkThreads)
     const int here = (int)min((int64_t)slab, cols - first);
     if (j < fetches) {
       unsigned char *to = rows + j * bytes;
+      if (LOOSE && first > 0)
+        nmb::fence_async_smem();
       if (fchoice < 0)
         begin[j] = fetch_row<LOOSE>(dout + (t0 + ftoken) * stride + first, here, to, &c.bar, dbounds);
       else if (at >= 0 && at < live)

@@ -60,3 +60,15 @@ def test_what_a_predecessor_writes_is_not_read_as_constant(file):
             assert not re.match(rf"({'|'.join(map(re.escape, MADE))})\b", read.strip()), f"{name}: __ldg({read})"
         for m in re.finditer(r"const\s+\w+\s*\*\s*__restrict__\s*(\w+)", params):
             assert m.group(1) not in MADE, f"{name}: {m.group(0)}"
+
+
+@pytest.mark.parametrize("name", ["walk_bulk", "nmb_combine_rows_grad_bulk"])
+def test_ordinary_stores_come_before_the_next_copy(name):
+    """Where rows are fetched in turns into the same shared memory, edge elements
+    are stored there by the thread that issues the place's next bulk copy: a
+    fence between the proxies stands in front of that copy."""
+    _, body = functions(source("rows.cu"))[name]
+    fetches = [m.start() for m in re.finditer(r"fetch_row<LOOSE>\(", body)]
+    fence = body.find("nmb::fence_async_smem()")
+    assert fetches and 0 <= fence < min(fetches)
+    assert re.search(r"if \(LOOSE && (turn > 1|first > 0)\)\s*$", body[:fence])  # from the second turn of a place on
