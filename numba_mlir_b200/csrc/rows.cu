@@ -685,8 +685,11 @@ __device__ __forceinline__ bool walk_bulk(const I *__restrict__ src, int64_t str
     __syncthreads(); // `begin` is written behind the arrivals
   for (int64_t turn = 0; turn < last; ++turn) {
     const int b = (int)(turn & 1);
-    if (!bulk_arrived(&turns.bar[b], (uint32_t)(turn >> 1) & 1, p.status))
+    if (!bulk_arrived(&turns.bar[b], (uint32_t)(turn >> 1) & 1, p.status)) {
+      if (turn + 1 < last) // the next turn's copies are on their way, too
+        (void)nmb::mbar_wait(&turns.bar[b ^ 1], (uint32_t)((turn + 1) >> 1) & 1);
       return false;
+    }
     const int live = (int)min((int64_t)kTurnRows, count - turn * kTurnRows);
     Pack<I, V> x[kTurnRows];
     uint32_t keys[kTurnRows];

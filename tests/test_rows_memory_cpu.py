@@ -72,3 +72,12 @@ def test_ordinary_stores_come_before_the_next_copy(name):
     fence = body.find("nmb::fence_async_smem()")
     assert fetches and 0 <= fence < min(fetches)
     assert re.search(r"if \(LOOSE && (turn > 1|first > 0)\)\s*$", body[:fence])  # from the second turn of a place on
+
+
+def test_a_block_that_gives_up_waits_for_both_turns():
+    """walk_bulk has two turns of copies on their way: a block that gives up on
+    one stays for the other, or its copies land in another block's memory."""
+    _, body = functions(source("rows.cu"))["walk_bulk"]
+    at = body.index("if (!bulk_arrived(")
+    gives_up = body[at:body.index("return false", at)]
+    assert re.search(r"if \(turn \+ 1 < last\)\s*\(void\)nmb::mbar_wait\(&turns\.bar\[b \^ 1\]", gives_up)
