@@ -228,6 +228,11 @@ uint64_t gpuxLaunchCount(void);
  * driver; count 0 clears a pending injection.  The reference has no such
  * hook; its failures abort (numba_mlir_gpu_runtime_sycl/lib/Utils.hpp:8-21). */
 void gpuxTestInjectDriverFault(const char *name, int code, int count);
+/* Test hook: how often the row operators' kernels poll for their own copies
+ * before they give up (and then wait for them all the same); 0: give up at
+ * once.  A kernel that gave up leaves its results unwritten and sets the queue's
+ * status word.  Values above the built-in bound set that. */
+void gpuxTestRowWaitSpins(uint32_t spins);
 
 /* CUDA graphs: gpuxGraphBegin starts recording everything submitted to the
  * queue (nothing runs), gpuxGraphEnd returns a replayable graph handle,

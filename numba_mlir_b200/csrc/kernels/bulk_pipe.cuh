@@ -50,8 +50,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
 constexpr uint32_t kWaitSpins = 1u << 22; // each failed poll already suspends in hardware
 
 // Bounded wait; false = gave up.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
-  for (uint32_t i = 0; i < kWaitSpins; ++i)
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint32_t spins = kWaitSpins) {
+  for (uint32_t i = 0; i < spins; ++i)
     if (mbar_try_wait(bar, parity))
       return true;
   return false;

@@ -18,6 +18,7 @@
 #include "kernels/bulk_pipe.cuh"
 #include "rows_host.h"
 
+#include <atomic>
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -163,14 +164,27 @@ template <typename A> __device__ __forceinline__ void set_scalar(void *p, int ty
 // Rows narrower than this are not fetched by bulk copies.
 constexpr int kBulkLeast = 1024;
 
-// Waits for the block's copies.  A wait that runs out is reported in the queue's
-// status word; nothing is then written, and the block stays for its copies.
-__device__ __forceinline__ bool bulk_arrived(uint64_t *bar, uint32_t phase, uint32_t *status) {
-  if (nmb::mbar_wait(bar, phase))
+// The bound of the waits for bulk copies, and the queue's word that reports one
+// that ran out.
+struct Waits {
+  uint32_t *status;
+  uint32_t spins;
+};
+
+// Waits for the block's copies; all threads of the block come here.  Where the
+// wait of one of them runs out the whole block gives up: that is reported in the
+// queue's status word, the block stays for its copies (as long again at most), and
+// what they were for is not written.  Behind it the threads also see what the
+// others stored before it.
+__device__ __forceinline__ bool bulk_arrived(uint64_t *bar, uint32_t phase, const Waits &waits) {
+  const bool mine = nmb::mbar_wait(bar, phase, waits.spins);
+  if (__syncthreads_and(mine))
     return true;
-  if (status)
-    atomicExch(status, (uint32_t)nmb::kStatusWaitTimeout);
-  (void)nmb::mbar_wait(bar, phase);
+  if (!mine) {
+    if (waits.status)
+      atomicExch(waits.status, (uint32_t)nmb::kStatusWaitTimeout);
+    (void)nmb::mbar_wait(bar, phase);
+  }
   return false;
 }
 
@@ -268,7 +282,7 @@ template <typename I, typename O, bool LOOSE>
 __global__ void __launch_bounds__(kTakeThreads)
     nmb_take_rows_bulk(const I *__restrict__ table, int64_t rows, int64_t stride, const void *__restrict__ ids,
                        int id_bytes, int64_t n, typename Acc<I>::type scale, O *__restrict__ out, int64_t out_stride,
-                       int64_t cols, int slab, int each, const Bounds<I> bounds, uint32_t *status) {
+                       int64_t cols, int slab, int each, const Bounds<I> bounds, const Waits waits) {
   using A = typename Acc<I>::type;
   constexpr int V = kBulkElems<LOOSE, I>;
   extern __shared__ __align__(128) unsigned char memory[]; // [each] rows
@@ -289,8 +303,7 @@ __global__ void __launch_bounds__(kTakeThreads)
     else
       nmb::mbar_arrive(&bar);
   }
-  __syncthreads(); // `at` is written behind the arrivals
-  if (!bulk_arrived(&bar, 0, status))
+  if (!bulk_arrived(&bar, 0, waits))
     return;
   const int live = (int)min((int64_t)each, n - i0);
   O *dst = out + i0 * out_stride + first;
@@ -363,7 +376,7 @@ struct GradPlan {
   int64_t chunks;
   int64_t to_clear;        // rows that are not cleared yet, at the front
   int lane_bits;           // threads of a group, through registers
-  uint32_t *status;
+  Waits waits;
 };
 
 __device__ __forceinline__ int64_t lower_bound(const uint32_t *keys, int64_t lo, int64_t hi, uint32_t key) {
@@ -681,11 +694,9 @@ __device__ __forceinline__ bool walk_bulk(const I *__restrict__ src, int64_t str
   if (last > 1)
     fetch(1);
   look(2);
-  if (LOOSE)
-    __syncthreads(); // `begin` is written behind the arrivals
   for (int64_t turn = 0; turn < last; ++turn) {
     const int b = (int)(turn & 1);
-    if (!bulk_arrived(&turns.bar[b], (uint32_t)(turn >> 1) & 1, p.status)) {
+    if (!bulk_arrived(&turns.bar[b], (uint32_t)(turn >> 1) & 1, p.waits)) {
       if (turn + 1 < last) // the next turn's copies are on their way, too
         (void)nmb::mbar_wait(&turns.bar[b ^ 1], (uint32_t)((turn + 1) >> 1) & 1);
       return false;
@@ -722,8 +733,6 @@ __device__ __forceinline__ bool walk_bulk(const I *__restrict__ src, int64_t str
       fetch(turn + 2);
       look(turn + 3);
     }
-    if (LOOSE)
-      __syncthreads();
   }
   return true;
 }
@@ -919,7 +928,7 @@ template <typename U>
 __global__ void __launch_bounds__(kCopyThreads)
     nmb_dispatch_rows_bulk(const U *__restrict__ x, int64_t stride, int64_t k, const int32_t *place,
                            const int32_t *kept, U *__restrict__ out, int64_t out_rows, int64_t out_stride,
-                           int64_t cols, int slab, const Bounds<U> bounds, uint32_t *status) {
+                           int64_t cols, int slab, const Bounds<U> bounds, const Waits waits) {
   extern __shared__ __align__(128) unsigned char memory[];
   __shared__ uint64_t bar;
   __shared__ int begin;
@@ -933,7 +942,7 @@ __global__ void __launch_bounds__(kCopyThreads)
   }
   __syncthreads();
   const int64_t live = made(kept);
-  if (!bulk_arrived(&bar, 0, status))
+  if (!bulk_arrived(&bar, 0, waits))
     return;
   const U *row = reinterpret_cast<const U *>(memory) + begin;
   for (int64_t j = 0; j < k; ++j) {
@@ -1073,7 +1082,7 @@ __global__ void __launch_bounds__(kBulkThreads)
                           const int32_t *__restrict__ place, const int32_t *__restrict__ kept,
                           const void *__restrict__ weights, int weight_type, T *__restrict__ out, int64_t tokens,
                           int64_t out_stride, int64_t cols, int slab, int each_bits, const Bounds<T> bounds,
-                          uint32_t *status) {
+                          const Waits waits) {
   using A = typename Acc<T>::type;
   constexpr int V = kBulkElems<LOOSE, T>;
   extern __shared__ __align__(128) unsigned char rows[]; // [1 << each_bits][k] rows
@@ -1101,8 +1110,7 @@ __global__ void __launch_bounds__(kBulkThreads)
     else
       nmb::mbar_arrive(&c.bar);
   }
-  __syncthreads();
-  if (!bulk_arrived(&c.bar, 0, status))
+  if (!bulk_arrived(&c.bar, 0, waits))
     return;
   const int bits = kBulkBits - each_bits, threads = 1 << bits, token = j >> bits; // a token's threads
   if (t0 + token >= tokens)
@@ -1284,7 +1292,7 @@ __global__ void __launch_bounds__(kBulkThreads)
                                const int32_t *__restrict__ place, const int32_t *__restrict__ kept, const void *__restrict__ weights, int weight_type,
                                T *__restrict__ dys, int64_t dy_rows, int64_t dy_stride, void *dweights, int64_t cols,
                                int slab, int each_bits, const Bounds<T> dbounds, const Bounds<T> ybounds,
-                               uint32_t *status) {
+                               const Waits waits) {
   using A = typename Acc<T>::type;
   constexpr int V = kBulkElems<LOOSE, T>, kWarps = kBulkThreads / 32, kPairs = V > 1 ? V / 2 : 1;
   // Choices read against dout at a time: what more of them hold in registers is
@@ -1331,10 +1339,8 @@ __global__ void __launch_bounds__(kBulkThreads)
       else
         nmb::mbar_arrive(&c.bar);
     }
-    if (LOOSE)
-      __syncthreads(); // `begin` is written behind the arrivals
-    if (!bulk_arrived(&c.bar, phase, status))
-      return; // every thread gives up by itself: no barrier is left waiting
+    if (!bulk_arrived(&c.bar, phase, waits))
+      return;
     const int row0 = token * (k + 1), entry0 = token * k;
     const T *drow = reinterpret_cast<const T *>(rows + row0 * bytes) + (LOOSE ? begin[row0] : 0);
     for (int j0 = 0; j0 < k && token < here_tokens; j0 += kTogether) {
@@ -1401,6 +1407,10 @@ __global__ void __launch_bounds__(kBulkThreads)
 }
 
 // ------------------------------------------------------------------- host ---
+std::atomic<uint32_t> gSpins{nmb::kWaitSpins};
+
+Waits waitsOf(void *queue) { return {nmb::statusWordOrNull(queue), gSpins.load(std::memory_order_relaxed)}; }
+
 unsigned blocksFor(int64_t rows, int lane_bits) {
   const int64_t per = kThreads >> lane_bits;
   return (unsigned)((rows + per - 1) / per);
@@ -1509,6 +1519,10 @@ size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 } // namespace
 
+// Test hook: polls after which the row operators' kernels give up waiting for
+// their own copies (which are then waited for all the same); 0: at once.
+GPUX_EXPORT void gpuxTestRowWaitSpins(uint32_t spins) { gSpins = spins < nmb::kWaitSpins ? spins : nmb::kWaitSpins; }
+
 GPUX_EXPORT int _mlir_ciface_nmb_take_rows_device(void *queue, const GPUXRows *table, const GPUXIndex *ids,
                                                   double scale, const GPUXRows *out) {
   const char *who = "take_rows";
@@ -1524,7 +1538,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_device(void *queue, const GPUXRows *t
   Stream s(queue);
   if (!s.ok)
     return 1;
-  uint32_t *status = nmb::statusWordOrNull(queue);
+  const Waits waits = waitsOf(queue);
   withPair(table->type, out->type, [&](auto i, auto o) {
     using I = decltype(i);
     using O = decltype(o);
@@ -1544,7 +1558,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_device(void *queue, const GPUXRows *t
         kernel<<<dim3((unsigned)((out->rows + each - 1) / each), (unsigned)slabs), kTakeThreads, (size_t)each * bytes,
                  s.stream>>>(static_cast<const I *>(table->data), table->rows, table->stride, ids->data, ids->bytes,
                              ids->count, (typename Acc<I>::type)scale, static_cast<O *>(out->data), out->stride,
-                             out->cols, slab, each, boundsOf<I>(table), status);
+                             out->cols, slab, each, boundsOf<I>(table), waits);
         return;
       }
     }
@@ -1601,6 +1615,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
   nmb::rows::Workspace memory(s, who, workspace, workspaceBytes, need.total());
   if (!memory.ok)
     return 1;
+  const Waits waits = waitsOf(queue);
   unsigned char *ws = static_cast<unsigned char *>(memory.data);
   int32_t *order = reinterpret_cast<int32_t *>(ws);
   uint32_t *keys = reinterpret_cast<uint32_t *>(ws + need.entries);
@@ -1654,7 +1669,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
                         chunks,
                         clearing.left,
                         bits,
-                        nmb::statusWordOrNull(queue)};
+                        waits};
     auto go = [&](auto kernel, int threads, size_t shared) {
       nmb::rows::launchBehind(kernel, (unsigned)blocks, (unsigned)threads, shared, s.stream,
                               static_cast<const I *>(dout->data), dout->stride, plan, (typename Acc<I>::type)scale,
@@ -1707,7 +1722,7 @@ int dispatchRows(void *queue, const Stream &s, const GPUXRows *x, int64_t k, con
                  const GPUXRows *out, bool behind) {
   if (x->rows == 0 || x->cols == 0 || k == 0 || out->rows == 0)
     return 0;
-  uint32_t *status = nmb::statusWordOrNull(queue);
+  const Waits waits = waitsOf(queue);
   withCopy(x, out, [&](auto u, auto V, int64_t vecs) {
     using U = decltype(u);
     const int64_t slabs = (x->cols * (int64_t)sizeof(U) + kCopyBytes - 1) / kCopyBytes;
@@ -1719,10 +1734,10 @@ int dispatchRows(void *queue, const Stream &s, const GPUXRows *x, int64_t k, con
       U *to = static_cast<U *>(out->data);
       if (behind)
         nmb::rows::launchBehind(nmb_dispatch_rows_bulk<U>, grid, kCopyThreads, shared, s.stream, from, x->stride, k,
-                                place, kept, to, out->rows, out->stride, x->cols, slab, boundsOf<U>(x), status);
+                                place, kept, to, out->rows, out->stride, x->cols, slab, boundsOf<U>(x), waits);
       else
         nmb_dispatch_rows_bulk<U><<<grid, kCopyThreads, shared, s.stream>>>(
-            from, x->stride, k, place, kept, to, out->rows, out->stride, x->cols, slab, boundsOf<U>(x), status);
+            from, x->stride, k, place, kept, to, out->rows, out->stride, x->cols, slab, boundsOf<U>(x), waits);
       return;
     }
     const int bits = laneBits(vecs, kThreadBits);
@@ -1802,7 +1817,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows
   Stream s(queue);
   if (!s.ok)
     return 1;
-  uint32_t *status = nmb::statusWordOrNull(queue);
+  const Waits waits = waitsOf(queue);
   withType(ys->type, [&](auto e) {
     using T = decltype(e);
     const int v = accessElems(out->cols, mostElems<T>(), {ys, out});
@@ -1816,7 +1831,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows
       const dim3 grid((unsigned)((out->rows + (1 << many) - 1) >> many), (unsigned)((out->cols + slab - 1) / slab));
       kernel<<<grid, kBulkThreads, (size_t)(bytes << many), s.stream>>>(
           static_cast<const T *>(ys->data), ys->rows, ys->stride, (int)k, place, kept, weights, weightType,
-          static_cast<T *>(out->data), out->rows, out->stride, out->cols, slab, many, boundsOf<T>(ys), status);
+          static_cast<T *>(out->data), out->rows, out->stride, out->cols, slab, many, boundsOf<T>(ys), waits);
       return;
     }
     withElems<mostElems<T>()>(v, [&](auto V) {
@@ -1844,7 +1859,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_grad_device(void *queue, const GPU
   Stream s(queue);
   if (!s.ok)
     return 1;
-  uint32_t *status = nmb::statusWordOrNull(queue);
+  const Waits waits = waitsOf(queue);
   withType(ys->type, [&](auto e) {
     using T = decltype(e);
     const int v = dout->cols ? accessElems(dout->cols, mostElems<T>(), {dout, ys, dys}) : 1;
@@ -1861,7 +1876,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_grad_device(void *queue, const GPU
       kernel<<<(unsigned)((dout->rows + (1 << many) - 1) >> many), kBulkThreads, (size_t)(bytes << many), s.stream>>>(
           static_cast<const T *>(dout->data), dout->rows, dout->stride, static_cast<const T *>(ys->data), ys->rows,
           ys->stride, (int)k, place, kept, weights, weightType, static_cast<T *>(dys->data), dys->rows, dys->stride,
-          dweights, dout->cols, slab, many, boundsOf<T>(dout), boundsOf<T>(ys), status);
+          dweights, dout->cols, slab, many, boundsOf<T>(dout), boundsOf<T>(ys), waits);
       return;
     }
     withElems<mostElems<T>()>(v, [&](auto V) {

@@ -125,6 +125,7 @@ SIGNATURES = {
     "gpuxQueueGetDevice": (_i, [_vp]),
     "gpuxQueueGetSmCount": (_i, [_vp]),
     "gpuxTestInjectDriverFault": (None, [_cp, _i, _i]),
+    "gpuxTestRowWaitSpins": (None, [ctypes.c_uint32]),
     "gpuxQueueStatusPtr": (_vp, [_vp]),
     "gpuxGetLastError": (_cp, []),
     "gpuxClearLastError": (None, []),
