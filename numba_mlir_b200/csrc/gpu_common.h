@@ -44,7 +44,6 @@ void setError(const char *fmt, ...);        // sticky error + stderr
 void noteLaunch();                          // bumps gpuxLaunchCount
 void *scratchGet(void *queue, size_t bytes); // per-queue grow-only scratch
 uint32_t *statusWord(void *queue);            // per-queue device word set by timed-out waits
-uint32_t *statusWordOrNull(void *queue);      // the same, null where a capture keeps it from being made now
 
 } // namespace nmb
 

@@ -181,8 +181,7 @@ __device__ __forceinline__ bool bulk_arrived(uint64_t *bar, uint32_t phase, cons
   if (__syncthreads_and(mine))
     return true;
   if (!mine) {
-    if (waits.status)
-      atomicExch(waits.status, (uint32_t)nmb::kStatusWaitTimeout);
+    atomicExch(waits.status, (uint32_t)nmb::kStatusWaitTimeout);
     (void)nmb::mbar_wait(bar, phase);
   }
   return false;
@@ -1409,7 +1408,8 @@ __global__ void __launch_bounds__(kBulkThreads)
 // ------------------------------------------------------------------- host ---
 std::atomic<uint32_t> gSpins{nmb::kWaitSpins};
 
-Waits waitsOf(void *queue) { return {nmb::statusWordOrNull(queue), gSpins.load(std::memory_order_relaxed)}; }
+// `status` null: no word, with the error set.
+Waits waitsOf(void *queue) { return {nmb::statusWord(queue), gSpins.load(std::memory_order_relaxed)}; }
 
 unsigned blocksFor(int64_t rows, int lane_bits) {
   const int64_t per = kThreads >> lane_bits;
@@ -1539,6 +1539,8 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_device(void *queue, const GPUXRows *t
   if (!s.ok)
     return 1;
   const Waits waits = waitsOf(queue);
+  if (!waits.status)
+    return 1;
   withPair(table->type, out->type, [&](auto i, auto o) {
     using I = decltype(i);
     using O = decltype(o);
@@ -1616,6 +1618,8 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
   if (!memory.ok)
     return 1;
   const Waits waits = waitsOf(queue);
+  if (!waits.status)
+    return 1;
   unsigned char *ws = static_cast<unsigned char *>(memory.data);
   int32_t *order = reinterpret_cast<int32_t *>(ws);
   uint32_t *keys = reinterpret_cast<uint32_t *>(ws + need.entries);
@@ -1717,12 +1721,11 @@ template <typename F> void withCopy(const GPUXRows *x, const GPUXRows *out, F &&
 } // namespace
 
 namespace {
-// `behind`: right behind the sort that makes the places.
-int dispatchRows(void *queue, const Stream &s, const GPUXRows *x, int64_t k, const int32_t *place, const int32_t *kept,
-                 const GPUXRows *out, bool behind) {
+// `behind`: right behind the sort that makes the places, nothing in between.
+int dispatchRows(const Waits &waits, const Stream &s, const GPUXRows *x, int64_t k, const int32_t *place,
+                 const int32_t *kept, const GPUXRows *out, bool behind) {
   if (x->rows == 0 || x->cols == 0 || k == 0 || out->rows == 0)
     return 0;
-  const Waits waits = waitsOf(queue);
   withCopy(x, out, [&](auto u, auto V, int64_t vecs) {
     using U = decltype(u);
     const int64_t slabs = (x->cols * (int64_t)sizeof(U) + kCopyBytes - 1) / kCopyBytes;
@@ -1763,7 +1766,10 @@ GPUX_EXPORT int _mlir_ciface_nmb_dispatch_rows_device(void *queue, const GPUXRow
       !sameWidth(who, x, out) || !checkPlaces(who, x->rows, k, place, kept) || !gridFits(who, x->rows))
     return 1;
   Stream s(queue);
-  return s.ok ? dispatchRows(queue, s, x, k, place, kept, out, false) : 1;
+  if (!s.ok)
+    return 1;
+  const Waits waits = waitsOf(queue);
+  return waits.status ? dispatchRows(waits, s, x, k, place, kept, out, false) : 1;
 }
 
 GPUX_EXPORT int _mlir_ciface_nmb_sort_dispatch_rows_device(void *queue, const GPUXRows *x, const GPUXIndex *ids,
@@ -1797,11 +1803,14 @@ GPUX_EXPORT int _mlir_ciface_nmb_sort_dispatch_rows_device(void *queue, const GP
   Stream s(queue);
   if (!s.ok)
     return 1;
+  const Waits waits = waitsOf(queue);
+  if (!waits.status)
+    return 1;
   nmb::rows::Workspace ws(s, who, workspace, workspaceBytes, nmb::rows::sortBytes(ids->count, groups));
   if (!ws.ok || !nmb::rows::sortByKey(s, who, *ids, groups, order, nullptr, place, offsets, ws.data))
     return 1;
   // groups of several passes end with a kernel that lets nothing begin early
-  return dispatchRows(queue, s, x, k, place, offsets + groups, out, ids->count > 0);
+  return dispatchRows(waits, s, x, k, place, offsets + groups, out, ids->count > 0);
 }
 
 GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows *ys, int64_t k, const int32_t *place,
@@ -1818,6 +1827,8 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_device(void *queue, const GPUXRows
   if (!s.ok)
     return 1;
   const Waits waits = waitsOf(queue);
+  if (!waits.status)
+    return 1;
   withType(ys->type, [&](auto e) {
     using T = decltype(e);
     const int v = accessElems(out->cols, mostElems<T>(), {ys, out});
@@ -1860,6 +1871,8 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_grad_device(void *queue, const GPU
   if (!s.ok)
     return 1;
   const Waits waits = waitsOf(queue);
+  if (!waits.status)
+    return 1;
   withType(ys->type, [&](auto e) {
     using T = decltype(e);
     const int v = dout->cols ? accessElems(dout->cols, mostElems<T>(), {dout, ys, dys}) : 1;

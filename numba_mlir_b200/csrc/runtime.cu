@@ -650,27 +650,43 @@ void *scratchGet(void *queue, size_t bytes) {
 
 uint32_t *statusWord(void *queue) {
   Queue *q = toQueue(queue);
-  if (!q->status) {
-    void *p = nullptr;
+  if (q->status)
+    return q->status;
+  void *p = nullptr;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(q->stream, &capture) == cudaSuccess && capture == cudaStreamCaptureStatusNone) {
     CUDA_TRY(cudaMallocAsync(&p, 256, q->stream), return nullptr);
     CUDA_TRY(cudaMemsetAsync(p, 0, 256, q->stream), return nullptr);
     q->status = static_cast<uint32_t *>(p);
+    return q->status;
   }
+  (void)cudaGetLastError();
+  // The queue's first launch is being recorded into a graph: memory that recorded
+  // calls allocate is the graph's alone and a recorded clearing would run in every
+  // replay, so the word is made on a stream beside it and waited for.  (Relaxed: a
+  // recording does not forbid this thread the calls.)
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode), return nullptr);
+  cudaStream_t side = nullptr;
+  cudaError_t e = cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking);
+  if (e == cudaSuccess)
+    e = cudaMallocAsync(&p, 256, side);
+  if (e == cudaSuccess)
+    e = cudaMemsetAsync(p, 0, 256, side);
+  if (e == cudaSuccess)
+    e = cudaStreamSynchronize(side);
+  if (e != cudaSuccess && p)
+    (void)cudaFreeAsync(p, side);
+  if (side)
+    (void)cudaStreamDestroy(side);
+  (void)cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) {
+    setError("no status word for the queue: %s", cudaGetErrorString(e));
+    (void)cudaGetLastError();
+    return nullptr;
+  }
+  q->status = static_cast<uint32_t *>(p);
   return q->status;
-}
-
-// For launches that may be the queue's first and recorded into a graph: memory
-// allocated while recording belongs to the graph, so the word is not made then.
-uint32_t *statusWordOrNull(void *queue) {
-  Queue *q = toQueue(queue);
-  if (!q->status) {
-    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(q->stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
-      (void)cudaGetLastError();
-      return nullptr;
-    }
-  }
-  return statusWord(queue);
 }
 
 } // namespace nmb

@@ -128,3 +128,29 @@ def test_combine_rows_and_gradient(runtime_lib, name, tokens, k, dim):
     assert (values_of(dys.copy_to_host(), name) < 0.01 + 1e-3).all()
     want = (values_of(ys.copy_to_host(), name)[plan.place.copy_to_host()] * values_of(dout.copy_to_host(), name)[:, None]).sum(-1)
     assert np.abs(dw.copy_to_host() - want).max() <= (dim + 2) * 2.0**-24 * want.max()
+
+
+def test_a_graph_of_the_first_call_reports_too(runtime_lib):
+    """A queue whose first call is recorded into a graph: the replays report waits
+    that ran out, each anew, and the word is the queue's own afterwards."""
+    import numba_mlir_b200 as nm
+    from numba_mlir_b200.runtime import GpuRuntimeError
+
+    q = nm.runtime.Queue("cuda:0")
+    rng = np.random.default_rng(0)
+    table, ids = dev(rng.standard_normal((50, 4096)).astype(np.float32), q), dev(rng.integers(0, 50, 600).astype(np.int32), q)
+    out = marked((600, 4096), "float32", q)
+    q.synchronize()
+    with no_patience(runtime_lib):
+        q.graph_begin()
+        nm.take_rows(table, ids, out=out)
+        g = q.graph_end()
+    for _ in range(2):
+        q.graph_launch(g)
+        with pytest.raises(GpuRuntimeError, match="timed out"):
+            q.check_status()
+    assert (out.copy_to_host() == 7.0).all()
+    q.graph_destroy(g)
+    nm.take_rows(table, ids, out=out)
+    q.check_status()
+    assert np.array_equal(out.copy_to_host(), table.copy_to_host()[ids.copy_to_host()])
