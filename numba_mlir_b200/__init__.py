@@ -28,6 +28,7 @@ from .rows import (  # noqa: F401
     take_rows,
     take_rows_grad,
     take_rows_grad_workspace,
+    torch_queue,
 )
 from .streaming import HostPipeline, map_host  # noqa: F401,E402
 

@@ -6,7 +6,10 @@ What a program writes as `a[m]`, `a[m] += b` and `argsort` on rows
 routines with the scale or the weights and the conversion to the result's type
 inside.  They take device arrays or anything else that exports
 `__cuda_array_interface__`, run asynchronously on a queue, and can be called
-inside `njit` functions, whose recorded plans replay them.
+inside `njit` functions, whose recorded plans replay them.  A kernel whose wait
+for its own copies runs out (the bound is far above the time of a copy)
+leaves what it was to write as it was; `Queue.check_status` of the queue that the
+call ran on raises then (`torch_queue` names the queue of torch's tensors).
 
     out            = take_rows(table, ids, scale)
     dtable         = take_rows_grad(dout, ids, rows, scale)
@@ -277,6 +280,26 @@ def _torch_stream(device):
         with sys.modules["torch"].cuda.device(device):
             q = _stream_queues[(device, stream)] = _rt.Queue.from_stream(stream)
     return q
+
+
+def torch_queue(device=None):
+    """The queue that the row operators run on when all of their arrays are
+    torch's: one over torch's current stream of the device (torch's current one
+    by default).  Its `check_status` synchronises and raises if a kernel of theirs
+    gave up on a wait."""
+    torch = sys.modules.get("torch")
+    if torch is None:
+        raise RuntimeError("torch is not in use")
+    if device is None:
+        index = torch.cuda.current_device()
+    elif isinstance(device, int):
+        index = device
+    else:
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"{device} is not a CUDA device")
+        index = torch.cuda.current_device() if device.index is None else device.index
+    return _torch_stream(index)
 
 
 def _raw_stream(q):

@@ -154,3 +154,31 @@ def test_a_graph_of_the_first_call_reports_too(runtime_lib):
     nm.take_rows(table, ids, out=out)
     q.check_status()
     assert np.array_equal(out.copy_to_host(), table.copy_to_host()[ids.copy_to_host()])
+
+
+def test_calls_on_torch_tensors_report_to_a_queue_that_can_be_asked(runtime_lib):
+    import torch
+
+    import numba_mlir_b200 as nm
+    from numba_mlir_b200.runtime import GpuRuntimeError
+
+    table = torch.randn(50, 4096, device="cuda")
+    ids = torch.randint(0, 50, (600,), device="cuda")
+    out = torch.full((600, 4096), 7.0, device="cuda")
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            q = nm.torch_queue()
+            assert q is nm.torch_queue("cuda") and q is nm.torch_queue(table.device) and q is nm.torch_queue(0)
+            assert q.stream == stream.cuda_stream
+            out.fill_(7.0)
+            with no_patience(runtime_lib):
+                nm.take_rows(table, ids, out=out)
+                with pytest.raises(GpuRuntimeError, match="timed out"):
+                    q.check_status()
+            assert bool((out == 7.0).all())
+            nm.take_rows(table, ids, out=out)
+            q.check_status()
+            assert torch.equal(out, table[ids])
+    with pytest.raises(ValueError):
+        nm.torch_queue("cpu")
