@@ -6,7 +6,8 @@ What a program writes as `a[m]`, `a[m] += b` and `argsort` on rows
 routines with the scale or the weights and the conversion to the result's type
 inside.  They take device arrays or anything else that exports
 `__cuda_array_interface__`, run asynchronously on a queue, and can be called
-inside `njit` functions, whose recorded plans replay them.  A kernel whose wait
+inside `njit` functions, whose recorded plans replay them (there on the queue of
+the function's call, without `queue` and `workspace` of their own).  A kernel whose wait
 for its own copies runs out (the bound is far above the time of a copy)
 leaves what it was to write as it was; `Queue.check_status` of the queue that the
 call ran on raises then (`torch_queue` names the queue of torch's tensors).
@@ -417,6 +418,7 @@ def take_rows(table, ids, scale=1.0, out=None, queue=None):
     has the table's type, or one of the two is float32 and the other 16 bits
     wide; the product is rounded once, to that type."""
     if lazy.current_trace() is not None:
+        _traced(queue)
         return _trace_take(table, ids, scale, out)
     if out is not None:
         done = (_native or _fast()).rows_take(queue or _default(table), table, ids, scale, out)
@@ -452,6 +454,7 @@ def take_rows_grad(dout, ids, rows=None, scale=1.0, out=None, accumulate=False, 
     array of at least `take_rows_grad_workspace(...)` bytes; without one the call
     takes memory from the stream-ordered pool."""
     if lazy.current_trace() is not None:
+        _traced(queue, workspace)
         return _trace_take_grad(dout, ids, rows, scale, out, accumulate)
     if out is not None and rows is None and workspace is None:
         done = (_native or _fast()).rows_take_grad(queue or _default(dout), dout, ids, scale, out, bool(accumulate))
@@ -501,6 +504,7 @@ def group_rows(ids, groups, plan=None, workspace=None, queue=None):
     their order within a group; entries outside [0, groups) come last.  Returns
     RowGroups, written into the arrays of `plan` when one is given."""
     if lazy.current_trace() is not None:
+        _traced(queue, workspace)
         return _trace_group(ids, groups, plan)
     if plan is not None and workspace is None:
         done = (_native or _fast()).rows_group(queue or _default(ids), ids, groups, plan)
@@ -543,6 +547,7 @@ def dispatch_rows(x, ids, groups=None, out=None, plan=None, queue=None):
     as they are; `plan` holds arrays to write the RowGroups into.  A RowGroups in
     the place of `ids` is used as it is."""
     if lazy.current_trace() is not None:
+        _traced(queue)
         return _trace_dispatch(x, ids, groups, out, plan)
     sorted_already = isinstance(ids, RowGroups)
     if out is not None and (plan is None if sorted_already else plan is not None):
@@ -617,6 +622,7 @@ def combine_rows(ys, plan, weights=None, out=None, queue=None):
     `weights` has the shape of plan.place (ones when it is None) and any
     floating-point type; `out` (T, D) has the type of ys."""
     if lazy.current_trace() is not None:
+        _traced(queue)
         return _trace_combine(ys, plan, weights, out)
     return _combine(ys, plan, weights, out, queue, "ys")
 
@@ -657,6 +663,7 @@ def dispatch_rows_grad(dxs, plan, out=None, queue=None):
     """The gradient of `dispatch_rows` with respect to x: the sum of the rows at
     a token's places, out[t, :] = sum over j of dxs[plan.place[t, j], :]."""
     if lazy.current_trace() is not None:
+        _traced(queue)
         return _trace_combine(dxs, plan, None, out)
     return _combine(dxs, plan, None, out, queue, "dxs")
 
@@ -668,6 +675,7 @@ def combine_rows_grad(dout, ys, plan, weights=None, out=None, dweights=None, que
     Returns (dys, dweights), written into `out` and `dweights` when given;
     dweights has the type of the weights (float32 when they are None)."""
     if lazy.current_trace() is not None:
+        _traced(queue)
         return _trace_combine_grad(dout, ys, plan, weights, out, dweights)
     if out is not None and dweights is not None:
         done = (_native or _fast()).rows_combine_grad(queue or _default(dout), dout, ys, plan, weights, out, dweights)
@@ -753,6 +761,14 @@ def run_step(step, get, args):
     _tag, routine, params = step
     kwargs = {name: get(v) if how == "slot" else args[v] if how == "arg" else v for name, (how, v) in params}
     routine(**kwargs)
+
+
+def _traced(queue, workspace=None):
+    """Inside a traced function the queue is that of the function's call, in every
+    replay anew, and workspaces come from the pool."""
+    if queue is not None or workspace is not None:
+        raise ValueError("queue and workspace cannot be given inside a traced function: its steps run on the queue "
+                         "of its call and take workspaces from the pool")
 
 
 def _lift(a):
