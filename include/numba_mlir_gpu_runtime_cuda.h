@@ -368,7 +368,8 @@ int _mlir_ciface_nmb_take_rows_device(void *queue, const GPUXRows *table, const 
  * out[v,:] = scale * (sum of dout[i,:] over ids[i] == v), i ascending; with
  * `accumulate` it is added to what out holds and rows without an index stay
  * untouched.  A given workspace holds at least
- * _mlir_ciface_nmb_take_rows_grad_workspace bytes (`type`: dout's). */
+ * _mlir_ciface_nmb_take_rows_grad_workspace bytes (`type`: dout's; 0 for sizes
+ * that the call refuses, as with the other workspaces). */
 size_t _mlir_ciface_nmb_take_rows_grad_workspace(int64_t count, int64_t rows, int64_t cols, int type);
 int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRows *dout, const GPUXIndex *ids,
                                            double scale, const GPUXRows *out, int accumulate,

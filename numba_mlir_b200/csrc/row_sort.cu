@@ -655,7 +655,8 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
 } // namespace nmb
 
 GPUX_EXPORT size_t _mlir_ciface_nmb_group_rows_workspace(int64_t count, int64_t groups) {
-  return count < 0 ? 0 : nmb::rows::sortBytes(count, groups);
+  const int64_t most = 0x7fffffff; // what the entry takes
+  return count < 0 || count > most || groups < 0 || groups >= most ? 0 : nmb::rows::sortBytes(count, groups);
 }
 
 GPUX_EXPORT int _mlir_ciface_nmb_group_rows_device(void *queue, const GPUXIndex *ids, int64_t groups, int32_t *order,

@@ -1593,7 +1593,10 @@ struct GradMemory {
 } // namespace
 
 GPUX_EXPORT size_t _mlir_ciface_nmb_take_rows_grad_workspace(int64_t count, int64_t rows, int64_t cols, int type) {
-  return count < 0 || rows < 0 || cols < 0 ? 0 : GradMemory(count, rows, cols, type).total();
+  const int64_t most = 0x7fffffff; // what the entry takes
+  return count < 0 || count > most || rows < 0 || rows >= most || cols < 0 || cols > most
+             ? 0
+             : GradMemory(count, rows, cols, type).total();
 }
 
 GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRows *dout, const GPUXIndex *ids,

@@ -491,11 +491,19 @@ def take_rows_grad_workspace(count, rows, cols, dtype=np.float32):
     kind = _FLOATS.get(np.dtype(dtype).str)
     if kind is None:
         raise TypeError(f"rows of {dtype} are not supported")
+    _sizes(count=(count, 2**31), rows=(rows, 2**31 - 1), cols=(cols, 2**31))
     return int(_rt.load()._mlir_ciface_nmb_take_rows_grad_workspace(int(count), int(rows), int(cols), kind))
+
+
+def _sizes(**sizes):
+    for name, (value, end) in sizes.items():
+        if not 0 <= value < end:
+            raise ValueError(f"{name} = {value}: must be in 0 .. {end - 1}")
 
 
 def group_rows_workspace(count, groups):
     """Bytes of workspace of `group_rows` for `count` ids."""
+    _sizes(count=(count, 2**31), groups=(groups, 2**31 - 1))
     return int(_rt.load()._mlir_ciface_nmb_group_rows_workspace(int(count), int(groups)))
 
 
