@@ -632,7 +632,7 @@ bool sortByKey(const Stream &s, const char *who, const GPUXIndex &ids, int64_t g
             return false;
         }
         const Fill fill = takeRows(clearing, (int)blocks, &grid);
-        launchBehind(nmb_sort_scatter<P.value>, grid, kThreads, kScatterBytes, s.stream, p, last ? keys : keyBuf[to],
+        launchBehind(nmb_sort_scatter<P.value>, grid, kThreads, kScatterBytes, s.stream, true, p, last ? keys : keyBuf[to],
                      last ? order : entryBuf[to], last ? place : nullptr, passes == 1 ? offsets : nullptr, fill);
         if (!launched(who))
           return false;

@@ -1677,8 +1677,10 @@ GPUX_EXPORT int _mlir_ciface_nmb_take_rows_grad_device(void *queue, const GPUXRo
                         clearing.left,
                         bits,
                         waits};
+    // without entries there is no sort in front, and the kernel begins like any other
+    const bool behind = ids->count > 0;
     auto go = [&](auto kernel, int threads, size_t shared) {
-      nmb::rows::launchBehind(kernel, (unsigned)blocks, (unsigned)threads, shared, s.stream,
+      nmb::rows::launchBehind(kernel, (unsigned)blocks, (unsigned)threads, shared, s.stream, behind,
                               static_cast<const I *>(dout->data), dout->stride, plan, (typename Acc<I>::type)scale,
                               static_cast<O *>(out->data), out->rows, out->stride, out->cols, boundsOf<I>(dout));
       ok = launched(who);
@@ -1738,25 +1740,14 @@ int dispatchRows(const Waits &waits, const Stream &s, const GPUXRows *x, int64_t
       const size_t shared = (size_t)fetched_bytes<true, U>(slab);
       const U *from = static_cast<const U *>(x->data);
       U *to = static_cast<U *>(out->data);
-      if (behind)
-        nmb::rows::launchBehind(nmb_dispatch_rows_bulk<U>, grid, kCopyThreads, shared, s.stream, from, x->stride, k,
-                                place, kept, to, out->rows, out->stride, x->cols, slab, boundsOf<U>(x), waits);
-      else
-        nmb_dispatch_rows_bulk<U><<<grid, kCopyThreads, shared, s.stream>>>(
-            from, x->stride, k, place, kept, to, out->rows, out->stride, x->cols, slab, boundsOf<U>(x), waits);
+      nmb::rows::launchBehind(nmb_dispatch_rows_bulk<U>, grid, kCopyThreads, shared, s.stream, behind, from, x->stride,
+                              k, place, kept, to, out->rows, out->stride, x->cols, slab, boundsOf<U>(x), waits);
       return;
     }
     const int bits = laneBits(vecs, kThreadBits);
-    const auto kernel = nmb_dispatch_rows<U, V.value>;
-    const unsigned blocks = blocksFor(x->rows, bits);
-    const U *from = static_cast<const U *>(x->data);
-    U *to = static_cast<U *>(out->data);
-    if (behind)
-      nmb::rows::launchBehind(kernel, blocks, kThreads, 0, s.stream, from, x->rows, x->stride, k, place, kept, to,
-                              out->rows, out->stride, vecs, bits);
-    else
-      kernel<<<blocks, kThreads, 0, s.stream>>>(from, x->rows, x->stride, k, place, kept, to, out->rows, out->stride,
-                                                vecs, bits);
+    nmb::rows::launchBehind(nmb_dispatch_rows<U, V.value>, blocksFor(x->rows, bits), kThreads, 0, s.stream, behind,
+                            static_cast<const U *>(x->data), x->rows, x->stride, k, place, kept,
+                            static_cast<U *>(out->data), out->rows, out->stride, vecs, bits);
   });
   return launched("dispatch_rows") ? 0 : 1;
 }

@@ -107,9 +107,12 @@ inline bool launched(const char *who) {
 // Launches a kernel that may begin while the kernel before it in the stream, one
 // of the same call, is still running (it calls let_next_begin): its blocks are
 // set up and then wait in wait_for_previous before they read what that kernel
-// and those before it write.
+// and those before it write.  Not `behind`: the stream's last work is not this
+// call's, nobody knows what that in turn has waited for, and the kernel begins when
+// all of it is done.
 template <typename K, typename... Args>
-inline void launchBehind(K kernel, dim3 grid, unsigned threads, size_t shared, cudaStream_t stream, Args... args) {
+inline void launchBehind(K kernel, dim3 grid, unsigned threads, size_t shared, cudaStream_t stream, bool behind,
+                         Args... args) {
   cudaLaunchConfig_t config = {};
   config.gridDim = grid;
   config.blockDim = dim3(threads);
@@ -119,7 +122,7 @@ inline void launchBehind(K kernel, dim3 grid, unsigned threads, size_t shared, c
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attribute;
-  config.numAttrs = 1;
+  config.numAttrs = behind ? 1 : 0;
   (void)cudaLaunchKernelEx(&config, kernel, args...);
 }
 #ifdef __CUDACC__

@@ -81,3 +81,19 @@ def test_a_block_that_gives_up_waits_for_both_turns():
     at = body.index("if (!bulk_arrived(")
     gives_up = body[at:body.index("return false", at)]
     assert re.search(r"if \(turn \+ 1 < last\)\s*\(void\)nmb::mbar_wait\(&turns\.bar\[b \^ 1\]", gives_up)
+
+
+def test_only_kernels_of_one_call_begin_early():
+    """Every launch says whether a kernel of the same call stands in front of it:
+    the sort's scatters follow a count, a gradient follows a sort only if there are
+    entries, copies only where the call has sorted."""
+    args = {}
+    for file in ("rows.cu", "row_sort.cu"):
+        text = source(file)
+        for m in re.finditer(r"launchBehind\(", text):
+            call = text[m.end():close(text, m.end() - 1, "()") - 1]
+            args.setdefault(file, []).append(re.search(r"s\.stream,\s*(\w+),", call).group(1))
+    assert args == {"rows.cu": ["behind"] * 3, "row_sort.cu": ["true"]}
+    assert "const bool behind = ids->count > 0;" in source("rows.cu")
+    assert re.search(r"dispatchRows\(waits, s, x, k, place, offsets \+ groups, out, ids->count > 0\)", source("rows.cu"))
+    assert "config.numAttrs = behind ? 1 : 0;" in source("rows_host.h")
