@@ -960,8 +960,14 @@ __global__ void __launch_bounds__(kCopyThreads)
 // keys and the earlier ones of the same key.  That is `entries` comparisons per
 // entry, but no step waits for another block.  Rows of 2048 bfloat16, 8 of 64
 // experts: 3.0 us for 4 tokens (4.6 us in two launches), 3.3 us for 128 (7.1),
-// 10.0 us for 512 (12.5).
+// 10.0 us for 512 (12.5).  All blocks together look at tokens x entries ids, so
+// tokens of few choices end it earlier.  In two launches against one, rows of 64
+// and of 2048 bfloat16: 2048 tokens of one choice 6.5 and 10.5 against 7.4 and
+// 8.4 us, 1024 of four 9.1 and 12.2 against 9.8 and 11.2 (both within the limit);
+// 2048 of two 8.4 and 13.4 against 12.6 and 14.3, 4096 of one 8.4 and 16.7 against
+// 19.2 and 21.6 (both past it).
 constexpr int kCountEntries = 4096, kCountGroups = 1024;
+constexpr int64_t kCountWork = int64_t(1) << 22; // tokens x entries
 
 template <typename U, int V>
 __global__ void __launch_bounds__(kThreads)
@@ -1782,7 +1788,8 @@ GPUX_EXPORT int _mlir_ciface_nmb_sort_dispatch_rows_device(void *queue, const GP
   }
   if (!nmb::rows::checkGroups(who, ids, groups, order, place, offsets))
     return 1;
-  if (ids->count > 0 && ids->count <= kCountEntries && groups <= kCountGroups && x->cols > 0) {
+  if (ids->count > 0 && ids->count <= kCountEntries && groups <= kCountGroups && x->cols > 0 &&
+      x->rows * ids->count <= kCountWork) {
     Stream s(queue);
     if (!s.ok)
       return 1;

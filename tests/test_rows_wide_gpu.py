@@ -265,3 +265,23 @@ def test_two_threads_at_once(queue):
     for th in threads:
         th.join()
     assert not failed, failed[0]
+
+
+@pytest.mark.parametrize("tokens,k,one", [(4, 8, True), (512, 8, True), (1024, 4, True), (2048, 1, True), (2048, 2, False),
+                                          (4096, 1, False), (1025, 4, False), (100, 64, False)])
+def test_dispatch_in_one_launch(queue, tokens, k, one):
+    """Sort and copy are one launch where every token's block can look at all
+    entries: up to 4096 of them, and up to 2^22 tokens x entries."""
+    import numba_mlir_b200 as nm
+
+    rng = np.random.default_rng(tokens)
+    x = rng.standard_normal((tokens, 16)).astype(np.float32)
+    ids = route(tokens, k, 80, rng)
+    out, plan = nm.dispatch_rows(dev(x), dev(ids), 80)
+    before = nm.runtime.launch_count()
+    nm.dispatch_rows(dev(x), dev(ids), 80, out=out, plan=plan)
+    assert (nm.runtime.launch_count() - before == 1) == one
+    order, place, offsets = plan_of(ids, 80)
+    assert np.array_equal(out.copy_to_host()[:offsets[-1]], x[order // k][:offsets[-1]])
+    for a, b in zip(plan, (order, place, offsets)):
+        assert np.array_equal(a.copy_to_host(), b)
