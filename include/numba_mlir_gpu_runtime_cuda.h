@@ -391,7 +391,7 @@ int _mlir_ciface_nmb_dispatch_rows_device(void *queue, const GPUXRows *x, int64_
                                           const int32_t *kept, const GPUXRows *out);
 
 /* group_rows and dispatch_rows in one call (one launch for up to 4096 entries in
- * up to 1024 groups, unless tokens x entries passes 2^22): the entries of token t are ids[t * k .. t * k + k), k =
+ * up to 1024 groups, up to 64 a token, unless tokens x entries passes 2^22): the entries of token t are ids[t * k .. t * k + k), k =
  * ids->count / x->rows, and out has at least ids->count rows.  The workspace is
  * group_rows'. */
 int _mlir_ciface_nmb_sort_dispatch_rows_device(void *queue, const GPUXRows *x, const GPUXIndex *ids,

@@ -962,11 +962,14 @@ __global__ void __launch_bounds__(kCopyThreads)
 // experts: 3.0 us for 4 tokens (4.6 us in two launches), 3.3 us for 128 (7.1),
 // 10.0 us for 512 (12.5).  All blocks together look at tokens x entries ids, so
 // tokens of few choices end it earlier.  In two launches against one, rows of 64
-// and of 2048 bfloat16: 2048 tokens of one choice 6.5 and 10.5 against 7.4 and
-// 8.4 us, 1024 of four 9.1 and 12.2 against 9.8 and 11.2 (both within the limit);
+// and of 2048 bfloat16: 2048 tokens of one choice 6.5 and 10.5 against 6.6 and
+// 7.6 us, 1024 of four 9.1 and 12.2 against 9.6 and 10.9 (both within the limit);
 // 2048 of two 8.4 and 13.4 against 12.6 and 14.3, 4096 of one 8.4 and 16.7 against
-// 19.2 and 21.6 (both past it).
-constexpr int kCountEntries = 4096, kCountGroups = 1024;
+// 19.2 and 21.6 (both past it, in one launch with room for more choices a block).  A block finds its token's choices by its eight
+// warps, which ends it at 64 of them: one token of 64 of 1024 experts, rows of 64,
+// 8.3 us against 9.7 in two launches, of 128 33.5 against 15.3, of 1024 146
+// against 92.
+constexpr int kCountEntries = 4096, kCountGroups = 1024, kCountChoices = 64;
 constexpr int64_t kCountWork = int64_t(1) << 22; // tokens x entries
 
 template <typename U, int V>
@@ -975,7 +978,7 @@ __global__ void __launch_bounds__(kThreads)
                            int entries, int groups, int32_t *__restrict__ order, int32_t *__restrict__ place,
                            int32_t *__restrict__ offsets, U *__restrict__ out, int64_t out_stride, int64_t vecs) {
   __shared__ uint32_t keys[kCountEntries];
-  __shared__ int32_t to[kCountEntries];
+  __shared__ int32_t to[kCountChoices];
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kWarps = kThreads / 32;
   for (int i = threadIdx.x; i < entries; i += kThreads) {
@@ -1789,7 +1792,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_sort_dispatch_rows_device(void *queue, const GP
   if (!nmb::rows::checkGroups(who, ids, groups, order, place, offsets))
     return 1;
   if (ids->count > 0 && ids->count <= kCountEntries && groups <= kCountGroups && x->cols > 0 &&
-      x->rows * ids->count <= kCountWork) {
+      k <= kCountChoices && x->rows * ids->count <= kCountWork) {
     Stream s(queue);
     if (!s.ok)
       return 1;

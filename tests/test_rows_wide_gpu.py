@@ -285,3 +285,21 @@ def test_dispatch_in_one_launch(queue, tokens, k, one):
     assert np.array_equal(out.copy_to_host()[:offsets[-1]], x[order // k][:offsets[-1]])
     for a, b in zip(plan, (order, place, offsets)):
         assert np.array_equal(a.copy_to_host(), b)
+
+
+@pytest.mark.parametrize("tokens,k,one", [(1, 64, True), (60, 64, True), (1, 65, False), (1, 1000, False), (4, 1000, False)])
+def test_many_choices_are_sorted_apart(queue, tokens, k, one):
+    """A token's block looks for up to 64 choices."""
+    import numba_mlir_b200 as nm
+
+    rng = np.random.default_rng(k)
+    x = rng.standard_normal((tokens, 24)).astype(np.float32)
+    ids = route(tokens, k, 1000, rng)
+    out, plan = nm.dispatch_rows(dev(x), dev(ids), 1000)
+    before = nm.runtime.launch_count()
+    nm.dispatch_rows(dev(x), dev(ids), 1000, out=out, plan=plan)
+    assert (nm.runtime.launch_count() - before == 1) == one
+    order, place, offsets = plan_of(ids, 1000)
+    assert np.array_equal(out.copy_to_host()[:offsets[-1]], x[order // k][:offsets[-1]])
+    for a, b in zip(plan, (order, place, offsets)):
+        assert np.array_equal(a.copy_to_host(), b)
