@@ -43,7 +43,7 @@ inline PyObject *name(const char *text) { return PyUnicode_InternFromString(text
 struct Names {
   PyObject *dtype = name("dtype"), *shape = name("shape"), *strides = name("strides"), *stride = name("stride"),
            *addr = name("_addr"), *buf = name("_buf"), *queue = name("queue"), *data_ptr = name("data_ptr"),
-           *requires_grad = name("requires_grad"), *get_device = name("get_device"),
+           *requires_grad = name("requires_grad"), *is_neg = name("is_neg"), *get_device = name("get_device"),
            *handle = name("handle"), *device = name("device"), *raw = name("_raw_stream");
 };
 inline Names &names() {
@@ -164,8 +164,8 @@ inline bool readType(PyObject *obj, Operand &op) {
   return true;
 }
 
-inline bool isTrue(PyObject *obj, PyObject *attr) {
-  PyObject *v = PyObject_GetAttr(obj, attr);
+inline bool isTrue(PyObject *obj, PyObject *attr, bool call = false) {
+  PyObject *v = call ? PyObject_CallMethodNoArgs(obj, attr) : PyObject_GetAttr(obj, attr);
   const bool t = v == Py_True;
   Py_XDECREF(v);
   return t;
@@ -194,7 +194,8 @@ inline bool read(PyObject *obj, Queue &q, Operand &op) {
            takeInts(PyObject_GetAttr(obj, n.shape), op.shape, op.nd, 1) &&
            takeInts(PyObject_GetAttr(obj, n.strides), op.stride, strides, op.item) && strides == op.nd;
   }
-  if (!gTensorType || !PyObject_TypeCheck(obj, (PyTypeObject *)gTensorType) || isTrue(obj, n.requires_grad))
+  if (!gTensorType || !PyObject_TypeCheck(obj, (PyTypeObject *)gTensorType) || isTrue(obj, n.requires_grad) ||
+      isTrue(obj, n.is_neg, true))
     return false;
   int64_t device; // -1 for a tensor that is not on a GPU
   if (!takeInt(PyObject_CallMethodNoArgs(obj, n.get_device), device) || device != q.device)

@@ -303,3 +303,20 @@ def test_many_choices_are_sorted_apart(queue, tokens, k, one):
     assert np.array_equal(out.copy_to_host()[:offsets[-1]], x[order // k][:offsets[-1]])
     for a, b in zip(plan, (order, place, offsets)):
         assert np.array_equal(a.copy_to_host(), b)
+
+
+def test_a_lazily_negated_tensor_is_refused(queue):
+    """torch keeps the sign of such a view beside its memory."""
+    import torch
+
+    import numba_mlir_b200 as nm
+
+    ids = torch.zeros(3, dtype=torch.int32, device="cuda")
+    table = torch.complex(torch.ones(4, 1, device="cuda"), torch.ones(4, 1, device="cuda")).conj().imag
+    assert table.is_neg() and table.shape == (4, 1)
+    out = torch.empty(3, 1, device="cuda")
+    for call in (lambda: nm.take_rows(table, ids, out=out), lambda: nm.take_rows(table, ids)):
+        with pytest.raises(RuntimeError, match="resolve_neg"):
+            call()
+    nm.take_rows(table.resolve_neg(), ids, out=out)
+    assert out.tolist() == [[-1.0]] * 3
