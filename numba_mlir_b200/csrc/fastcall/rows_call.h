@@ -194,8 +194,7 @@ inline bool read(PyObject *obj, Queue &q, Operand &op) {
            takeInts(PyObject_GetAttr(obj, n.shape), op.shape, op.nd, 1) &&
            takeInts(PyObject_GetAttr(obj, n.strides), op.stride, strides, op.item) && strides == op.nd;
   }
-  if (!gTensorType || !PyObject_TypeCheck(obj, (PyTypeObject *)gTensorType) || isTrue(obj, n.requires_grad) ||
-      isTrue(obj, n.is_neg, true))
+  if (!gTensorType || !PyObject_TypeCheck(obj, (PyTypeObject *)gTensorType) || isTrue(obj, n.requires_grad))
     return false;
   int64_t device; // -1 for a tensor that is not on a GPU
   if (!takeInt(PyObject_CallMethodNoArgs(obj, n.get_device), device) || device != q.device)
@@ -209,7 +208,12 @@ inline bool read(PyObject *obj, Queue &q, Operand &op) {
       return false;
     q.torchHere = raw == q.raw;
   }
-  return q.torchHere && readType(obj, op) && takeInt(PyObject_CallMethodNoArgs(obj, n.data_ptr), op.ptr) &&
+  if (!q.torchHere || !readType(obj, op))
+    return false;
+  // the negative bit is that of parts of complex values: never of indices
+  if (op.kind >= 0 && isTrue(obj, n.is_neg, true))
+    return false;
+  return takeInt(PyObject_CallMethodNoArgs(obj, n.data_ptr), op.ptr) &&
          takeInts(PyObject_GetAttr(obj, n.shape), op.shape, op.nd, 1) &&
          takeInts(PyObject_CallMethodNoArgs(obj, n.stride), op.stride, strides, 1) && strides == op.nd;
 }

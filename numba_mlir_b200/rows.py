@@ -136,7 +136,7 @@ def _operand(obj, name):
         if known is not None and obj.is_cuda:
             if obj.requires_grad:
                 raise RuntimeError(f"{name}: a tensor that requires a gradient; use tensor.detach()")
-            if obj.is_neg():  # its memory holds the values with the other sign
+            if known[0] is not None and obj.is_neg():  # its memory holds the values with the other sign
                 raise RuntimeError(f"{name}: a tensor with the negative bit set; use tensor.resolve_neg()")
             op.kind, op.index, op.item = known
             op.ptr, op.shape, op.strides = obj.data_ptr(), tuple(obj.shape), obj.stride()
