@@ -1887,7 +1887,7 @@ GPUX_EXPORT int _mlir_ciface_nmb_combine_rows_grad_device(void *queue, const GPU
       const auto kernel = loose ? nmb_combine_rows_grad_bulk<T, true> : nmb_combine_rows_grad_bulk<T, false>;
       const int64_t bytes = (k + 1) * (loose ? fetched_bytes<true, T>(slab) : fetched_bytes<false, T>(slab));
       // Off the words, where blocks have more to compute, half the memory and more
-      // blocks: 30000 tokens with eight rows of 1027 bf16 265 us, 313 us with all
+      // blocks: 30000 tokens with eight rows of 1027 bf16 271 us, 313 us with all
       // of it.  On them 164 us (rows of 1024) with all, 166 us with half.
       const int many = slab >= dout->cols ? bulkTokens(dout->rows, bytes, k, kBulkGradBytes / (loose ? 2 : 1)) : 0;
       kernel<<<(unsigned)((dout->rows + (1 << many) - 1) >> many), kBulkThreads, (size_t)(bytes << many), s.stream>>>(
