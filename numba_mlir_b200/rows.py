@@ -8,10 +8,11 @@ inside.  They take device arrays or anything else that exports
 `__cuda_array_interface__`, run asynchronously on a queue, and can be called
 inside `njit` functions, whose recorded plans replay them (there on the queue of
 the function's call, without `queue` and `workspace` of their own; a number of
-rows or groups that is an argument of the function has it traced anew).  A kernel whose wait
-for its own copies runs out (the bound is far above the time of a copy)
-leaves what it was to write as it was; `Queue.check_status` of the queue that the
-call ran on raises then (`torch_queue` names the queue of torch's tensors).
+rows or groups that is an argument of the function has it traced anew).  A
+kernel whose wait for its own copies runs out (the bound is far above the time
+of a copy) leaves what it had not written yet as it was; `Queue.check_status` of
+the queue that the call ran on raises then (`torch_queue` names the queue of
+torch's tensors).
 
     out            = take_rows(table, ids, scale)
     dtable         = take_rows_grad(dout, ids, rows, scale)
