@@ -182,3 +182,33 @@ def test_calls_on_torch_tensors_report_to_a_queue_that_can_be_asked(runtime_lib)
             assert torch.equal(out, table[ids])
     with pytest.raises(ValueError):
         nm.torch_queue("cpu")
+
+
+def test_a_first_call_recorded_by_torch_reports_too(runtime_lib):
+    """The same under torch's recording, which forbids other threads and streams
+    more than the queue's own does."""
+    import torch
+
+    import numba_mlir_b200 as nm
+    from numba_mlir_b200.runtime import GpuRuntimeError
+
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        table, ids = torch.randn(50, 4096, device="cuda"), torch.randint(0, 50, (600,), device="cuda")
+        out = torch.full((600, 4096), 7.0, device="cuda")
+        q = nm.runtime.Queue.from_stream(st.cuda_stream)
+        st.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with no_patience(runtime_lib), torch.cuda.graph(g, stream=st):
+            nm.take_rows(table, ids, out=out, queue=q)
+        g.replay()
+        with pytest.raises(GpuRuntimeError, match="timed out"):
+            q.check_status()
+        assert bool((out == 7.0).all())
+        patient = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(patient, stream=st):
+            nm.take_rows(table, ids, out=out, queue=q)
+        patient.replay()
+        q.check_status()
+        assert torch.equal(out, table[ids])
+        del g, patient
